@@ -191,6 +191,106 @@ def adam(w, g, m, v, t, lr, b1, b2, eps, wd=0.0, gscale=1.0, clip=None, dynamic=
                                         gscale, _p(clip), _l.ADAM_DYNAMIC if dynamic else _l.ADAM_STORIES))
 
 
+def _same_device(*tensors):
+    """Refuses tensors that are not on the current CUDA device (the stream of the call belongs to it)."""
+    for t in tensors:
+        if t is not None and (not t.is_cuda or t.device.index != torch.cuda.current_device()):
+            raise ValueError(f"expected a tensor on the current CUDA device, got one on {t.device}")
+
+
+def _like(name, t, shape, dtype):
+    """Checks an argument's shape and element type; None passes."""
+    if t is not None and (tuple(t.shape) != tuple(shape) or t.dtype != dtype):
+        raise ValueError(f"{name}: expected {dtype} {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+
+
+ADAM_BLOCK = 256        # elements of an 8-bit optimizer state that share a scale
+
+
+class AdamTensors:
+    """The tensors of an ``adam_multi`` step, checked and laid out for the call once.
+
+    w: fp32 weights; g: gradients (all fp32, bf16 or fp16); m, v: fp32 moments, or uint8 codes with fp32 scales of
+    ceil(n / 256) elements in m_scale / v_scale; copy: bf16 or fp16 tensors that receive the new weights (optional); wd: weight
+    decay, one number or one per tensor.  Lists of equal length; tensors are contiguous and share no memory that the step
+    writes.  The object keeps the tensors alive and holds their addresses: make another one when a tensor is replaced."""
+
+    def __init__(self, w, g, m, v, m_scale=None, v_scale=None, copy=None, wd=0.0):
+        count = len(w)
+        wd = [float(wd)] * count if isinstance(wd, (int, float)) else [float(a) for a in wd]
+        for name, ts in (("g", g), ("m", m), ("v", v), ("m_scale", m_scale), ("v_scale", v_scale), ("copy", copy), ("wd", wd)):
+            if ts is not None and len(ts) != count:
+                raise ValueError(f"{name}: expected {count} entries, got {len(ts)}")
+        self.q8 = count > 0 and m[0].dtype == torch.uint8
+        if self.q8 != (m_scale is not None) or self.q8 != (v_scale is not None):
+            raise ValueError("m_scale and v_scale belong to uint8 moments, and only to them")
+        self.g_dtype = _dt(g[0]) if count else _l.F32
+        self.copy_dtype = _dt(copy[0]) if count and copy is not None else _l.BF16
+        if self.copy_dtype == _l.F32:
+            raise ValueError("copy: bf16 or fp16 tensors")
+        state = torch.uint8 if self.q8 else torch.float32
+        written = []
+        for k in range(count):
+            shape, blocks = w[k].shape, (-(-w[k].numel() // ADAM_BLOCK),)
+            _like(f"w[{k}]", w[k], shape, torch.float32)
+            _like(f"g[{k}]", g[k], shape, g[0].dtype)
+            _like(f"m[{k}]", m[k], shape, state)
+            _like(f"v[{k}]", v[k], shape, state)
+            if self.q8:
+                _like(f"m_scale[{k}]", m_scale[k], blocks, torch.float32)
+                _like(f"v_scale[{k}]", v_scale[k], blocks, torch.float32)
+            if copy is not None:
+                _like(f"copy[{k}]", copy[k], shape, copy[0].dtype)
+            for ts in (w, m, v, m_scale, v_scale, copy):
+                if ts is not None and ts[k].numel():
+                    written.append((ts[k].data_ptr(), ts[k].data_ptr() + ts[k].numel() * ts[k].element_size()))
+        written.sort()
+        if any(b[0] < a[1] for a, b in zip(written, written[1:])):
+            raise ValueError("two tensors that the step writes share memory")
+        self.items = (_l.AdamItem * count)()
+        self.count, self.wd = count, wd
+        self.tensors = (list(w), list(g), list(m), list(v), m_scale and list(m_scale), v_scale and list(v_scale), copy and list(copy))
+        for ts in self.tensors:
+            _same_device(*(ts or ()))
+        for k in range(count):
+            at = [None if ts is None else _p(ts[k]) for ts in self.tensors]
+            self.items[k] = _l.AdamItem(w[k].numel(), *at, wd[k], 0)
+
+
+def adam_multi(tensors, t, lr, b1, b2, eps, gscale=1.0, clip=None, seed=0, dynamic=True):
+    """One Adam / AdamW step over an ``AdamTensors`` list.  With 8-bit moments pass another ``seed`` every step: it decides
+    which way each stored moment is rounded."""
+    _like("clip", clip, (1,), torch.float32)
+    _same_device(clip)
+    _l.check(_l.load().ane_cuda_adam_multi_dev(_stream(), _l.ADAM_STATE_Q8 if tensors.q8 else _l.ADAM_STATE_F32, tensors.g_dtype, tensors.copy_dtype,
+                                              tensors.count, tensors.items, t, lr, b1, b2, eps, gscale, _p(clip), seed & 0xFFFFFFFF,
+                                              _l.ADAM_DYNAMIC if dynamic else _l.ADAM_STORIES))
+
+
+def adam_state_unpack(codes, scales, second=False, out=None):
+    """fp32 values of 8-bit moments (codes uint8, one scale per 256 of them)."""
+    out = torch.empty(codes.shape, dtype=torch.float32, device=codes.device) if out is None else out
+    _like("codes", codes, codes.shape, torch.uint8)
+    _like("scales", scales, (-(-codes.numel() // ADAM_BLOCK),), torch.float32)
+    _like("out", out, codes.shape, torch.float32)
+    _same_device(codes, scales, out)
+    _l.check(_l.load().ane_cuda_adam_state_unpack_dev(_stream(), codes.numel(), _p(out), _p(codes), _p(scales), int(second)))
+    return out
+
+
+def adam_state_pack(value, second=False, seed=0, codes=None, scales=None):
+    """-> (codes, scales) of fp32 moments."""
+    blocks = (-(-value.numel() // ADAM_BLOCK),)
+    codes = torch.empty(value.shape, dtype=torch.uint8, device=value.device) if codes is None else codes
+    scales = torch.empty(blocks, dtype=torch.float32, device=value.device) if scales is None else scales
+    _like("value", value, value.shape, torch.float32)
+    _like("codes", codes, value.shape, torch.uint8)
+    _like("scales", scales, blocks, torch.float32)
+    _same_device(value, codes, scales)
+    _l.check(_l.load().ane_cuda_adam_state_pack_dev(_stream(), value.numel(), _p(codes), _p(scales), _p(value), int(second), seed & 0xFFFFFFFF))
+    return codes, scales
+
+
 def grad_norm_sq(g, gscale=1.0, out=None):
     out = torch.empty(1, dtype=torch.float32, device=g.device) if out is None else out
     _l.check(_l.load().ane_cuda_grad_norm_sq_dev(_stream(), g.numel(), _p(g), gscale, _p(out)))

@@ -17,6 +17,7 @@ ID_U16, ID_I32 = 0, 1
 NORM_BWD_REFERENCE, NORM_BWD_EXACT = 0, 1
 ROPE_FORWARD, ROPE_INVERSE = 0, 1
 ADAM_STORIES, ADAM_DYNAMIC = 0, 1
+ADAM_STATE_F32, ADAM_STATE_Q8 = 0, 1
 OOR_SKIP, OOR_ZERO = 0, 2
 
 OK = 0
@@ -37,6 +38,12 @@ class AdamState(C.Structure):
 class Status(C.Structure):
     _fields_ = [("oor_ids", C.c_int32), ("nonfinite", C.c_int32), ("wait_giveups", C.c_int32),
                 ("reserved", C.c_int32)]
+
+
+class AdamItem(C.Structure):
+    """One tensor of ane_cuda_adam_multi_dev."""
+    _fields_ = [("n", C.c_size_t), ("w", C.c_void_p), ("g", C.c_void_p), ("m", C.c_void_p), ("v", C.c_void_p),
+                ("m_scale", C.c_void_p), ("v_scale", C.c_void_p), ("copy", C.c_void_p), ("wd", C.c_float), ("reserved", C.c_int)]
 
 
 _vp, _i, _u, _f, _sz = C.c_void_p, C.c_int, C.c_uint, C.c_float, C.c_size_t
@@ -113,6 +120,9 @@ PROTOTYPES = {
     "ane_cuda_embed_backward_dev": (_i, [_vp, _i, _i, _i, _i, _i, _vp, _vp, _vp, _i]),
     "ane_cuda_cross_entropy_dev": (_i, [_vp, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _f]),
     "ane_cuda_adam_dev": (_i, [_vp, _sz, _vp, _vp, _vp, _vp, _i, _f, _f, _f, _f, _f, _f, _vp, _u]),
+    "ane_cuda_adam_multi_dev": (_i, [_vp, _i, _i, _i, _i, _vp, _i, _f, _f, _f, _f, _f, _vp, _u, _u]),
+    "ane_cuda_adam_state_unpack_dev": (_i, [_vp, _sz, _vp, _vp, _vp, _i]),
+    "ane_cuda_adam_state_pack_dev": (_i, [_vp, _sz, _vp, _vp, _vp, _i, _u]),
     "ane_cuda_grad_norm_sq_dev": (_i, [_vp, _sz, _vp, _f, _vp]),
     "ane_cuda_clip_factor_dev": (_i, [_vp, _vp, _i, _f, _vp]),
     # layout helpers

@@ -59,8 +59,24 @@ typedef enum { ANE_ID_U16 = 0, ANE_ID_I32 = 1 } ane_idtype;
 #define ANE_ROPE_INVERSE       1u /* the backward rotation of training_dynamic/cpu_ops.h:168-184 */
 #define ANE_ADAM_STORIES       0u /* w -= lr*mh/(sqrt(vh)+eps)                 stories_cpu_ops.h:55-63 */
 #define ANE_ADAM_DYNAMIC       1u /* w -= lr*(mh/(sqrt(vh)+eps) + wd*w)        training_dynamic/cpu_ops.h:56-64 */
+/* ---- how an optimizer step over a list of tensors keeps its moments */
+typedef enum { ANE_ADAM_STATE_F32 = 0, ANE_ADAM_STATE_Q8 = 1 } ane_adam_state;
 #define ANE_OOR_SKIP           0u /* out-of-range id: leave the column / row untouched (stories_cpu_ops.h:115,126) */
 #define ANE_OOR_ZERO           2u /* out-of-range id: write zeros instead */
+
+/* One tensor of ane_cuda_adam_multi_dev: n elements, all pointers on the device.  m and v are fp32, or one byte per element
+ * with an fp32 scale per 256 elements (the last block may be shorter) in m_scale / v_scale.  copy (may be NULL) receives the
+ * new weights rounded to 16 bits.  wd is the tensor's own weight decay.  n = 0 skips the entry. */
+typedef struct {
+    size_t n;
+    float *w;
+    const void *g;
+    void *m, *v;
+    float *m_scale, *v_scale;
+    void *copy;
+    float wd;
+    int reserved;
+} ane_adam_item;
 
 /* AdamState, laid out as in training/stories_config.h:56-59 and training_dynamic/config.h:46. */
 typedef struct { float *m, *v; size_t n; } AdamState;
@@ -293,6 +309,26 @@ int ane_cuda_cross_entropy_dev(void *stream, ane_idtype idtype, int B, int V, in
 int ane_cuda_adam_dev(void *stream, size_t n, float *w, const float *g, float *m, float *v, int t,
                       float lr, float b1, float b2, float eps, float wd, float gscale,
                       const float *clip_dev, unsigned flags);
+/* The same step over a list of tensors in one launch (per 400 tensors).  items is a HOST array, read during the call: it
+ * travels in the kernel's parameters, so a captured graph holds it by value.  state = ANE_ADAM_STATE_F32: m and v as above,
+ * the results are those of ane_cuda_adam_dev.  state = ANE_ADAM_STATE_Q8: one byte per element and moment, see
+ * ane_adam_item.  Codes are floats without infinities (first moment: sign, 4 exponent bits of bias 7, 3 mantissa bits;
+ * second: 5 exponent bits of bias 15, 3 mantissa bits) times their block's scale = largest magnitude / (480 or 122880).  The
+ * weights are updated from the exact fp32 moments; the stored ones are rounded up or down at random, with the probability
+ * that keeps their mean, by 20 bits of a hash of (seed, index of the tensor in the list, index of the element): pass another
+ * seed every step.  A second moment above zero never becomes zero.  A block whose largest magnitude is below 2^-100 is
+ * stored as zeros; a NaN or infinity makes its whole block NaN.  The rounding noise of v is averaged over 1 / (1 - b2)
+ * steps; b2 <= 0.99 keeps it small.  g has g_dtype; copies have copy_dtype (ANE_BF16 or ANE_F16).  Tensors of a list must
+ * not share memory (checked with tuning knob "check_extents" only).  No counterpart in the reference, which calls
+ * adam_update once per tensor (training_dynamic/train.m:839-847). */
+int ane_cuda_adam_multi_dev(void *stream, ane_adam_state state, ane_dtype g_dtype, ane_dtype copy_dtype, int count,
+                            const ane_adam_item *items, int t, float lr, float b1, float b2, float eps, float gscale,
+                            const float *clip_dev, unsigned seed, unsigned flags);
+/* 8-bit moments to fp32 and back (checkpoint files hold fp32 moments); second = 0 or 1 picks the code.  pack rounds with the
+ * hash of (seed, 0, element) and drops the sign of a second moment. */
+int ane_cuda_adam_state_unpack_dev(void *stream, size_t n, float *out, const void *codes, const float *scales, int second);
+int ane_cuda_adam_state_pack_dev(void *stream, size_t n, void *codes, float *scales, const float *value, int second,
+                                 unsigned seed);
 /* a13: *out_dev = sum_i (g[i]*gscale)^2, fixed summation order.        train.m:770-788 */
 int ane_cuda_grad_norm_sq_dev(void *stream, size_t n, const float *g, float gscale, float *out_dev);
 /* a13: *factor_dev = clip/norm if clip > 0 and norm > clip else 1, norm = sqrt(sum of the
