@@ -38,6 +38,19 @@ def _bcs(t):
     raise ValueError("expected [B, C, S] or [C, S]")
 
 
+def _same_device(*tensors):
+    """Refuses tensors that are not on the current CUDA device (the stream of the call belongs to it)."""
+    for t in tensors:
+        if t is not None and (not t.is_cuda or t.device.index != torch.cuda.current_device()):
+            raise ValueError(f"expected a tensor on the current CUDA device, got one on {t.device}")
+
+
+def _like(name, t, shape, dtype):
+    """Checks an argument's shape and element type; None passes."""
+    if t is not None and (tuple(t.shape) != tuple(shape) or t.dtype != dtype):
+        raise ValueError(f"{name}: expected {dtype} {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+
+
 def rmsnorm(x, w, eps=1e-5, out=None):
     out = torch.empty_like(x) if out is None else out
     B, Cn, S = _bcs(x)
@@ -73,6 +86,50 @@ def residual_rmsnorm(x, f, w, alpha, eps=1e-5, x2=None, x2norm=None):
     _l.check(_l.load().ane_cuda_residual_rmsnorm_dev(_stream(), _dt(x), B, Cn, S, _p(x2), _p(x2norm), _p(x), _p(f),
                                                     _p(w), alpha, eps))
     return x2, x2norm
+
+
+def _block_norm_args(x, f, w_pre, w_post, gate):
+    B, Cn, S = _bcs(x)
+    _like("f", f, x.shape, x.dtype)
+    _like("w_pre", w_pre, (Cn,), torch.float32)
+    _like("w_post", w_post, (Cn,), torch.float32)
+    per_seq = gate is not None and gate.dim() == 2
+    _like("gate", gate, (B, Cn) if per_seq else (Cn,), torch.float32)
+    return B, Cn, S, int(per_seq)
+
+
+def block_norm(x, f, w_pre, w_post=None, gate=None, alpha=1.0, eps=1e-5, x2=None, y=None):
+    """(x2, y): x2 = x + alpha * gate * rmsnorm(f; w_post), y = rmsnorm(x2; w_pre).  Without w_post the block's output f is
+    taken as it is; gate is fp32, [C] or one per sequence [B, C].  x2 may be x."""
+    x2 = torch.empty_like(x) if x2 is None else x2
+    y = torch.empty_like(x) if y is None else y
+    B, Cn, S, per_seq = _block_norm_args(x, f, w_pre, w_post, gate)
+    _like("x2", x2, x.shape, x.dtype)
+    _like("y", y, x.shape, x.dtype)
+    _same_device(x, f, w_pre, w_post, gate, x2, y)
+    _l.check(_l.load().ane_cuda_block_norm_dev(_stream(), _dt(x), B, Cn, S, _p(x2), _p(y), _p(x), _p(f), _p(w_post), _p(gate), per_seq,
+                                              _p(w_pre), alpha, eps))
+    return x2, y
+
+
+def block_norm_bwd(dy, x2, f, w_pre, dw_pre, w_post=None, dw_post=None, gate=None, dgate=None, dx2=None, alpha=1.0, eps=1e-5,
+                   dx=None, df=None):
+    """(dx, df) of ``block_norm`` from the gradients of its outputs, dy and dx2 (None: none); dw_pre, dw_post and dgate are
+    accumulated into (None: not wanted).  dx is the gradient of x and of x2; it may be dx2, and df may be f."""
+    dx = torch.empty_like(x2) if dx is None else dx
+    df = torch.empty_like(x2) if df is None else df
+    B, Cn, S, per_seq = _block_norm_args(x2, f, w_pre, w_post, gate)
+    for name, t in (("dy", dy), ("dx2", dx2), ("dx", dx), ("df", df)):
+        _like(name, t, x2.shape, x2.dtype)
+    _like("dw_pre", dw_pre, (Cn,), torch.float32)
+    _like("dw_post", dw_post, (Cn,), torch.float32)
+    if (dw_post is not None and w_post is None) or (dgate is not None and gate is None):
+        raise ValueError("dw_post needs w_post and dgate needs gate")
+    _like("dgate", dgate, () if gate is None else gate.shape, torch.float32)
+    _same_device(dy, x2, f, w_pre, dw_pre, w_post, dw_post, gate, dgate, dx2, dx, df)
+    _l.check(_l.load().ane_cuda_block_norm_bwd_dev(_stream(), _dt(x2), B, Cn, S, _p(dx), _p(df), _p(dw_post), _p(dgate), _p(dw_pre), _p(dy),
+                                                  _p(dx2), _p(x2), _p(f), _p(w_post), _p(gate), per_seq, _p(w_pre), alpha, eps))
+    return dx, df
 
 
 def swiglu(h1, h3, out=None):
@@ -189,19 +246,6 @@ def cross_entropy(logits, targets, grad_scale=1.0, dlogits=None):
 def adam(w, g, m, v, t, lr, b1, b2, eps, wd=0.0, gscale=1.0, clip=None, dynamic=True):
     _l.check(_l.load().ane_cuda_adam_dev(_stream(), w.numel(), _p(w), _p(g), _p(m), _p(v), t, lr, b1, b2, eps, wd,
                                         gscale, _p(clip), _l.ADAM_DYNAMIC if dynamic else _l.ADAM_STORIES))
-
-
-def _same_device(*tensors):
-    """Refuses tensors that are not on the current CUDA device (the stream of the call belongs to it)."""
-    for t in tensors:
-        if t is not None and (not t.is_cuda or t.device.index != torch.cuda.current_device()):
-            raise ValueError(f"expected a tensor on the current CUDA device, got one on {t.device}")
-
-
-def _like(name, t, shape, dtype):
-    """Checks an argument's shape and element type; None passes."""
-    if t is not None and (tuple(t.shape) != tuple(shape) or t.dtype != dtype):
-        raise ValueError(f"{name}: expected {dtype} {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
 
 
 ADAM_BLOCK = 256        # elements of an 8-bit optimizer state that share a scale

@@ -107,6 +107,8 @@ PROTOTYPES = {
     "ane_cuda_residual_dev": (_i, [_vp, _i, _sz, _vp, _vp, _vp, _f]),
     "ane_cuda_scale_dev": (_i, [_vp, _i, _sz, _vp, _vp, _f]),
     "ane_cuda_residual_rmsnorm_dev": (_i, [_vp, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _f, _f]),
+    "ane_cuda_block_norm_dev": (_i, [_vp, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _f, _f]),
+    "ane_cuda_block_norm_bwd_dev": (_i, [_vp, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _f, _f]),
     "ane_cuda_swiglu_dev": (_i, [_vp, _i, _sz, _vp, _vp, _vp]),
     "ane_cuda_swiglu_bwd_dev": (_i, [_vp, _i, _sz, _vp, _vp, _vp, _vp, _vp]),
     "ane_cuda_rope_dev": (_i, [_vp, _i, _i, _i, _i, _i, _vp, _vp, _f, _i, _u]),

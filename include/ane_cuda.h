@@ -249,6 +249,23 @@ int ane_cuda_scale_dev(void *stream, ane_dtype dtype, size_t n, void *out, const
 int ane_cuda_residual_rmsnorm_dev(void *stream, ane_dtype dtype, int B, int C, int S,
                                   void *x2, void *x2norm, const void *x, const void *f, const float *w,
                                   float alpha, float eps);
+/* The norms around a block in one pass, with the block's gate and residual scale (between them they replace rmsnorm on the
+ * block's output, the gate, the residual and the rmsnorm of the next block; residual_rmsnorm above is the case without w_post
+ * and gate):
+ *   n = f * w_post / sqrt(mean_c f^2 + eps)        w_post NULL: n = f
+ *   x2 = x + alpha * gate * n                      gate NULL: 1; fp32 [C], or [B][C] with gate_per_seq = 1
+ *   y = x2 * w_pre / sqrt(mean_c x2^2 + eps)       of x2 as it is stored
+ * x2 may be x (in place); the other tensors are distinct. */
+int ane_cuda_block_norm_dev(void *stream, ane_dtype dtype, int B, int C, int S, void *x2, void *y, const void *x, const void *f,
+                            const float *w_post, const float *gate, int gate_per_seq, const float *w_pre, float alpha,
+                            float eps);
+/* Its backward pass, the analytic gradient.  dy, dx2: gradients of y and of x2 (dx2 NULL: none but through y); x2 and f as
+ * in the forward call.  dx (the gradient of x, and of x2) and df are overwritten; dw_post [C], dgate ([C] or [B][C], as the
+ * gate) and dw_pre [C] are accumulated into, each may be NULL.  Bit-stable from call to call.  dx may be dx2, df may be f. */
+int ane_cuda_block_norm_bwd_dev(void *stream, ane_dtype dtype, int B, int C, int S, void *dx, void *df, float *dw_post,
+                                float *dgate, float *dw_pre, const void *dy, const void *dx2, const void *x2, const void *f,
+                                const float *w_post, const float *gate, int gate_per_seq, const float *w_pre, float alpha,
+                                float eps);
 /* a4: out = h1*sigmoid(h1)*h3                                          forward.h:101,149-151
  * The sigmoid of a4 / a5 comes from the hardware's exp2 and reciprocal approximations (relative error below 1e-6; values
  * under 2^-126, i.e. h1 < -87.3, become zero); tuning knob "swiglu_exact" = 1 selects expf and an IEEE division. */
