@@ -44,8 +44,7 @@ typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t
                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 static EncodeTiledFn g_encode_tiled = nullptr;
 
-int make_bcs_tensor_map(CUtensorMap *map, ane_dtype dtype, const void *base, int B, int C, int S, int box_s, int box_c,
-                        int l2_promotion_bytes) {
+static int resolve_encode_tiled() {
     if (!g_encode_tiled) {
         void *fn = nullptr;
         cudaDriverEntryPointQueryResult q;
@@ -56,6 +55,27 @@ int make_bcs_tensor_map(CUtensorMap *map, ane_dtype dtype, const void *base, int
         }
         g_encode_tiled = reinterpret_cast<EncodeTiledFn>(fn);
     }
+    return ANE_CUDA_OK;
+}
+
+int make_matrix_map(CUtensorMap *map, ane_dtype dtype, const void *base, size_t rows, size_t cols, size_t ld, int box_rows) {
+    if (int rc = resolve_encode_tiled()) return rc;
+    if (!aligned16(base) || ld % 8 || ld < cols || rows < 1 || cols < 1 || rows > 0xffffffffull || cols > 0xffffffffull || box_rows < 1 || box_rows > 256 || dtype == ANE_F32)
+        return fail(ANE_CUDA_ERR_INVALID, "matrix map: unsupported alignment or size (%zu x %zu, ld %zu, box %d)", rows, cols, ld, box_rows);
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
+    const cuuint32_t box[2] = {64u, (cuuint32_t)box_rows};
+    const cuuint32_t estr[2] = {1u, 1u};
+    const CUresult r = g_encode_tiled(map, dtype == ANE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void *>(base), dims, strides,
+                                      box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(ANE_CUDA_ERR_CUDA, "cuTensorMapEncodeTiled failed with code %d", (int)r);
+    return ANE_CUDA_OK;
+}
+
+int make_bcs_tensor_map(CUtensorMap *map, ane_dtype dtype, const void *base, int B, int C, int S, int box_s, int box_c,
+                        int l2_promotion_bytes) {
+    if (int rc = resolve_encode_tiled()) return rc;
     const size_t e = dtype_size(dtype);
     if (!aligned16(base) || ((size_t)S * e) % 16 || ((size_t)box_s * e) % 16 || box_s > 256 || box_c > 256 || box_s < 1 || box_c < 1)
         return fail(ANE_CUDA_ERR_INVALID, "tensor map: unsupported alignment or box (S=%d box %dx%d)", S, box_s, box_c);

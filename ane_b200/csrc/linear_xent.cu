@@ -1,0 +1,683 @@
+// linear_xent.cu -- classifier product and softmax cross-entropy in one operator, forward and backward, in pieces of the
+// vocabulary and without ever keeping the logits:
+//
+//   l[v][t]   = sum_d table[v][d] * x[d][t]
+//   loss_t    = -log(exp(l[tgt] - lse_t) + 1e-10),  lse_t = log sum_v exp(l[v][t])
+//   dl[v][t]  = (exp(l[v][t] - lse_t) - [v == tgt_t]) * grad_scale / S         (0 for a token without a target)
+//   dx        = table^T dl         d_table += dl x^T
+//
+// Four matrix products on the tensor cores (fp32 accumulation):
+//   stats     l, reduced on the fly to a (max, sum of exp) pair per token and tile of 256 vocabulary rows
+//   dlogits   l once more for one piece of the vocabulary, turned into dl and written to scratch in 16 bits
+//   dx        dl x table, added to an fp32 sum over the pieces
+//   d_table   x x dl, added to the caller's fp32 gradient
+// Writing the logits and reading them back would take longer than the second product: 12 bytes per logit (write, read, write
+// dl) at 6.5 TB/s are 1.9 ps, 2 * 1024 operations at 1.5 PFLOP/s are 1.4 ps.
+//
+// Precision.  16-bit inputs enter the products as they are.  dl is rounded to 16 bits for dx, whose result is rounded to 16
+// bits as well; d_table is an fp32 sum, so dl enters it as two 16-bit numbers, the rounded value and what the rounding left
+// (17 bits and more), at the price of one more product.  fp32 inputs are split the same way into two bf16 parts and every
+// product is taken as high*high + high*low + low*high: what is dropped is below 2^-17 of a term.  In fp16 dl is scaled by 2^14
+// (|dl| * S / grad_scale <= 1 becomes 16384 at most), so that the probabilities of a large vocabulary, 1e-5 and less, do not
+// fall among fp16's subnormals.
+//
+// The accumulators of the tensor cores cut off what does not fit instead of rounding: every step of 16 along K takes half a
+// unit of the last place from the sum on average, 3e-8 of it (measured: 1.2e-5 after 345 steps).  So fp32 results leave the
+// accumulator after 2048 elements of K, 128 steps, and are added up in memory with rounding; and the products with a low part
+// go first, while the sum is small.
+//
+// A token without a target (id outside [0, V)) has zeros in place of its x, so that nothing it holds -- infinities and NaN
+// included -- reaches d_table.
+#include "common.cuh"
+#include "tma.cuh"
+
+#include <math.h>
+
+namespace ane {
+
+constexpr float LX_LOG2E = 1.4426950408889634f;
+constexpr int LX_BM = 128, LX_BN = 256, LX_BK = 64;      // tile of a block: M x N outputs, K elements per stage
+constexpr int LX_STAGES = 4;
+constexpr int LX_A_BYTES = LX_BM * LX_BK * 2, LX_B_BYTES = LX_BN * LX_BK * 2, LX_STAGE_BYTES = LX_A_BYTES + LX_B_BYTES;
+constexpr int LX_THREADS = 192;                          // copy warp, matrix warp, four epilogue warps
+constexpr size_t LX_SMEM = (size_t)LX_STAGES * LX_STAGE_BYTES + 1024;
+constexpr int LX_SPAN = 2048 / LX_BK;                    // K blocks summed in an accumulator where an fp32 result is wanted
+constexpr int LX_WAIT_LIMIT = 1 << 20;
+
+enum LxEpilogue { LX_STATS, LX_DLOGITS, LX_DX, LX_DTABLE };
+
+struct LxMaps { CUtensorMap a[3], b[3]; };               // one pair per 16-bit product that is summed
+struct LxArgs {
+    int segments;              // pairs in use
+    int kblocks;               // K blocks of one pair
+    int splits;                // shares of the K blocks, each with its own sums (dx only)
+    int span;                  // K blocks that one accumulator sums before it is added to memory (dx, d_table)
+    int m_tiles, n_tiles;
+    int m, n;                  // valid rows and columns of the output
+    uint32_t idesc;
+    // stats, dlogits: m = tokens, n = vocabulary rows of the piece from v0
+    const void *targets;       // of the first token
+    int id_u16, V, v0;
+    float2 *part; int tile0;   // stats: [vocabulary tile][ldt], this piece's first tile
+    float *hit;                // stats: the target's logit per token
+    const float *lse2;         // dlogits: lse * log2(e)
+    void *hi, *lo; size_t ldl; // dlogits: [token][ldl], lo may be null
+    float dscale;
+    // dx: [split][column][ldt] sums; d_table: [column][D]
+    float *out; size_t ldt; int first;
+    float alpha;
+    int half_type;             // 1 when the 16-bit parts are fp16
+    ane_cuda_status *status;
+};
+
+// ------------------------------------------------------------------ tensor-core primitives
+// Shared-memory operand descriptor, 128-byte swizzle.  K-major: rows of 64 K elements, eight rows per 1024-byte group.
+// MN-major: 64 M (or N) elements per 128-byte row, one row per k, eight k per group, the next 64 M after `lead` bytes.
+__device__ __forceinline__ uint64_t lx_desc(uint32_t addr, uint32_t lead) {
+    return (uint64_t)((addr >> 4) & 0x3fffu) | (uint64_t)(lead >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+__device__ __forceinline__ void lx_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void lx_commit(uint64_t *bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void lx_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void lx_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void lx_arrive(uint64_t *bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void lx_load_box(uint32_t dst, const CUtensorMap *map, int x, int y, uint64_t *bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_u32(bar)) : "memory");
+}
+// 32 accumulator columns of this warp's 32 lanes: v[j] = column + j of the thread's own row.
+__device__ __forceinline__ void lx_tmem_load(uint32_t addr, float (&v)[32]) {
+    uint32_t r[32];
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, "
+                 "%20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+                   "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+                   "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(addr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ float lx_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void lx_add(float *p, float v) { asm volatile("red.global.add.f32 [%0], %1;" ::"l"(p), "f"(v) : "memory"); }
+
+// Bounded wait that also ends when another role of the block gave up.
+__device__ __forceinline__ bool lx_wait(uint64_t *bar, uint32_t parity, volatile int *abort) {
+    for (int i = 0; i < LX_WAIT_LIMIT; i++) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if (*abort) return false;
+    }
+    *abort = 1;
+    return false;
+}
+
+__device__ __forceinline__ int lx_target(const void *targets, int id_u16, int V, int t) {
+    const int id = id_u16 ? (int)static_cast<const uint16_t *>(targets)[t] : static_cast<const int32_t *>(targets)[t];
+    return id >= 0 && id < V ? id : -1;
+}
+
+// 16 fp32 values -> 16-bit high parts and, with `lo`, the 16-bit rest of each.
+__device__ __forceinline__ void lx_split2(float a, float b, int half_type, uint32_t &hi, uint32_t &lo) {
+    if (half_type) {
+        const __half2 h = __floats2half2_rn(a, b);
+        const float2 f = __half22float2(h);
+        const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
+        hi = *reinterpret_cast<const uint32_t *>(&h);
+        lo = *reinterpret_cast<const uint32_t *>(&l);
+    } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        const __nv_bfloat162 l = __floats2bfloat162_rn(a - __low2float(h), b - __high2float(h));
+        hi = *reinterpret_cast<const uint32_t *>(&h);
+        lo = *reinterpret_cast<const uint32_t *>(&l);
+    }
+}
+// 32 bytes at once: every sector of a row is written whole, although neighbouring lanes hold different rows.
+__device__ __forceinline__ void lx_store32(void *p, const uint32_t (&w)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
+}
+
+// The K blocks of one tile: the tile's share [k0, k1), in parts of `span`; within a part every operand pair in turn.
+struct LxRange {
+    int k0, k1, span, segments, part, seg, k;
+    __device__ __forceinline__ LxRange(const LxArgs &a, int tile) {
+        const int ks = tile / (a.m_tiles * a.n_tiles);
+        k0 = (int)((long long)a.kblocks * ks / a.splits);
+        k1 = (int)((long long)a.kblocks * (ks + 1) / a.splits);
+        span = a.span; segments = a.segments;
+        part = k = k0;
+        seg = 0;
+    }
+    __device__ __forceinline__ bool done() const { return part >= k1; }
+    __device__ __forceinline__ bool first() const { return seg == 0 && k == part; }      // at the beginning of a part (or past the last)
+    __device__ __forceinline__ void next() {
+        k++;
+        if (k < k1 && k < part + span) return;
+        if (++seg < segments) { k = part; return; }
+        seg = 0;
+        part += span;
+        k = part;
+    }
+};
+
+// ------------------------------------------------------------------ the product
+// Persistent blocks walk the output tiles.  One thread copies operand boxes into a ring of four stages, one thread issues the
+// matrix instructions into one of two accumulators, four warps work on the accumulator that is complete.
+template <int EPI>
+__global__ void __launch_bounds__(LX_THREADS, 1) lx_gemm_kernel(const __grid_constant__ LxMaps maps, const __grid_constant__ LxArgs a) {
+    constexpr bool A_MN = EPI == LX_DTABLE, B_MN = EPI == LX_DX || EPI == LX_DTABLE;
+    extern __shared__ uint8_t raw[];
+    const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
+    __shared__ uint64_t full[LX_STAGES], empty[LX_STAGES], acc_full[2], acc_empty[2], drained;
+    __shared__ uint32_t tmem_at;
+    __shared__ int give_up;
+    volatile int *abort = &give_up;
+
+    const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < LX_STAGES; i++) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
+        for (int i = 0; i < 2; i++) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], 4); }
+        mbar_init(&drained, 1);
+        give_up = 0;
+        mbar_init_fence();
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&tmem_at)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        lx_fence_before();
+    }
+    __syncthreads();
+    lx_fence_after();
+    const uint32_t tmem = tmem_at;
+
+    const int tiles = a.m_tiles * a.n_tiles * a.splits;
+    uint32_t issued = 0;                                  // copy warp: K blocks whose copies were started
+
+    if (warp == 0) {
+        if (lane == 0) {
+            for (int tile = blockIdx.x; tile < tiles && !*abort; tile += gridDim.x) {
+                const int mt = tile % a.m_tiles, nt = tile / a.m_tiles % a.n_tiles;
+                LxRange r(a, tile);
+                for (; !r.done(); r.next(), issued++) {
+                    const int st = issued % LX_STAGES;
+                    if (!lx_wait(&empty[st], ((issued / LX_STAGES) & 1) ^ 1, abort)) break;
+                    const int seg = r.seg, k = r.k * LX_BK;
+                    const uint32_t sa = base + st * LX_STAGE_BYTES, sb = sa + LX_A_BYTES;
+                    mbar_arrive_expect_tx(&full[st], LX_STAGE_BYTES);
+                    if constexpr (A_MN) {
+#pragma unroll
+                        for (int i = 0; i < LX_BM / 64; i++) lx_load_box(sa + i * 8192, &maps.a[seg], mt * LX_BM + i * 64, k, &full[st]);
+                    } else {
+                        lx_load_box(sa, &maps.a[seg], k, mt * LX_BM, &full[st]);
+                    }
+                    if constexpr (B_MN) {
+#pragma unroll
+                        for (int i = 0; i < LX_BN / 64; i++) lx_load_box(sb + i * 8192, &maps.b[seg], nt * LX_BN + i * 64, k, &full[st]);
+                    } else {
+                        lx_load_box(sb, &maps.b[seg], k, nt * LX_BN, &full[st]);
+                    }
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            uint32_t used = 0, turn = 0;
+            bool ok = true;
+            for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
+                LxRange r(a, tile);
+                uint32_t d = 0, more = 0;
+                for (; !r.done(); used++) {
+                    if (r.first()) {
+                        if (!(ok = lx_wait(&acc_empty[turn & 1], ((turn >> 1) & 1) ^ 1, abort))) break;
+                        lx_fence_after();
+                        d = tmem + (turn & 1) * LX_BN;
+                        more = 0;
+                    }
+                    const int st = used % LX_STAGES;
+                    if (!(ok = lx_wait(&full[st], (used / LX_STAGES) & 1, abort))) break;
+                    lx_fence_after();
+                    const uint32_t sa = base + st * LX_STAGE_BYTES, sb = sa + LX_A_BYTES;
+#pragma unroll
+                    for (int i = 0; i < LX_BK / 16; i++)
+                        lx_mma(d, lx_desc(sa + i * (A_MN ? 2048 : 32), A_MN ? 8192 : 16), lx_desc(sb + i * (B_MN ? 2048 : 32), B_MN ? 8192 : 16), a.idesc, more | i);
+                    more = 1;
+                    lx_commit(&empty[st]);
+                    r.next();
+                    if (r.first()) { lx_commit(&acc_full[turn & 1]); turn++; }      // the accumulator is complete
+                }
+            }
+            lx_commit(&drained);                            // also after a give-up: no instruction outlives the block
+            mbar_wait_bounded(&drained, 0);
+        }
+    } else {
+        const int quad = warp & 3, row = quad * 32 + lane;   // a warp reads the accumulator lanes of its place in the group of four
+        uint32_t turn = 0;
+        bool ok = true;
+        for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
+          const int mt = tile % a.m_tiles, nt = tile / a.m_tiles % a.n_tiles, ks = tile / (a.m_tiles * a.n_tiles);
+          const int m = mt * LX_BM + row, n0 = nt * LX_BN;
+          const int cols = a.n - n0 < LX_BN ? a.n - n0 : LX_BN;
+          const LxRange range(a, tile);
+          if (EPI == LX_DX && a.first && range.k0 >= range.k1 && m < a.m)          // a share without K blocks: zeros
+              for (int c = 0; c < cols; c++) a.out[((size_t)ks * a.n + n0 + c) * a.ldt + m] = 0.0f;
+          for (int part = range.k0; part < range.k1; part += a.span, turn++) {
+            if (!(ok = __all_sync(0xffffffffu, lx_wait(&acc_full[turn & 1], (turn >> 1) & 1, abort)))) break;
+            lx_fence_after();
+            const uint32_t t = tmem + (turn & 1) * LX_BN + ((uint32_t)(quad * 32) << 16);
+            if constexpr (EPI == LX_STATS) {
+                const int tgt = m < a.m ? lx_target(a.targets, a.id_u16, a.V, m) - a.v0 - n0 : -1;     // column in this tile
+                float mx = -INFINITY, sum = 0.0f;
+                for (int c = 0; c < cols; c += 32) {
+                    float v[32];
+                    lx_tmem_load(t + c, v);
+                    if (__any_sync(0xffffffffu, tgt >= c && tgt < c + 32)) {
+                        float h = 0.0f;
+#pragma unroll
+                        for (int j = 0; j < 32; j++) h = tgt == c + j ? v[j] : h;
+                        if (tgt >= c && tgt < c + 32) a.hit[m] = h;
+                    }
+                    if (c + 32 > cols) {
+#pragma unroll
+                        for (int j = 0; j < 32; j++) if (c + j >= cols) v[j] = -INFINITY;
+                    }
+                    float top = v[0];
+#pragma unroll
+                    for (int j = 1; j < 32; j++) top = fmaxf(top, v[j]);
+                    const float mnew = fmaxf(mx, top * LX_LOG2E);
+                    float part = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < 32; j++) part += lx_exp2(fmaf(v[j], LX_LOG2E, -mnew));
+                    sum = fmaf(sum, lx_exp2(mx - mnew), part);
+                    mx = mnew;
+                }
+                if (m < a.m) a.part[(size_t)(a.tile0 + nt) * a.ldt + m] = make_float2(mx, sum);
+            } else if constexpr (EPI == LX_DLOGITS) {
+                const int id = m < a.m ? lx_target(a.targets, a.id_u16, a.V, m) : -1;
+                const int tgt = id >= 0 ? id - a.v0 - n0 : -1;
+                const float lse2 = m < a.m ? a.lse2[m] : 0.0f;
+                const float scale = id >= 0 ? a.dscale : 0.0f;
+                const size_t at = (size_t)m * a.ldl + n0;
+                for (int c = 0; c < LX_BN; c += 32) {
+                    float v[32];
+                    lx_tmem_load(t + c, v);
+#pragma unroll
+                    for (int j = 0; j < 32; j++) v[j] = lx_exp2(fmaf(v[j], LX_LOG2E, -lse2)) * scale;
+                    if (__any_sync(0xffffffffu, tgt >= c && tgt < c + 32)) {
+#pragma unroll
+                        for (int j = 0; j < 32; j++) v[j] = tgt == c + j ? v[j] - scale : v[j];
+                    }
+                    if (c + 32 > cols) {
+#pragma unroll
+                        for (int j = 0; j < 32; j++) if (c + j >= cols) v[j] = 0.0f;
+                    }
+                    if (m < a.m) {
+                        if (id < 0) {                     // a masked token: zeros, whatever its logits are
+#pragma unroll
+                            for (int j = 0; j < 32; j++) v[j] = 0.0f;
+                        }
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            uint32_t hi[8], lo[8];
+#pragma unroll
+                            for (int j = 0; j < 8; j++) lx_split2(v[h * 16 + 2 * j], v[h * 16 + 2 * j + 1], a.half_type, hi[j], lo[j]);
+                            lx_store32(static_cast<uint16_t *>(a.hi) + at + c + h * 16, hi);
+                            if (a.lo) lx_store32(static_cast<uint16_t *>(a.lo) + at + c + h * 16, lo);
+                        }
+                    }
+                }
+            } else {
+                // dx: rows are tokens, columns are channels; d_table: rows are channels, columns vocabulary rows.  Either way the
+                // 32 lanes of a warp hold 32 neighbours of a contiguous row.
+                // A later part of K follows from the same thread, so the order of the additions is fixed.
+                float *out = EPI == LX_DX ? a.out + ((size_t)ks * a.n + n0) * a.ldt + m : a.out + (size_t)n0 * a.ldt + m;
+                for (int c = 0; c < cols; c += 32) {
+                    float v[32];
+                    lx_tmem_load(t + c, v);
+                    if (m < a.m) {
+                        if (EPI == LX_DX && a.first && part == range.k0) {
+#pragma unroll
+                            for (int j = 0; j < 32; j++) if (c + j < cols) out[(size_t)(c + j) * a.ldt] = v[j];
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 32; j++) if (c + j < cols) lx_add(out + (size_t)(c + j) * a.ldt, EPI == LX_DX ? v[j] : v[j] * a.alpha);
+                        }
+                    }
+                }
+            }
+            lx_fence_before();
+            __syncwarp();
+            if (lane == 0) lx_arrive(&acc_empty[turn & 1]);
+          }
+        }
+    }
+    __syncwarp();
+    lx_fence_before();
+    __syncthreads();
+    lx_fence_after();
+    if (*abort && threadIdx.x == 0) {
+        // copies still on their way into this block's shared memory: every stage's last one
+        for (uint32_t i = issued > LX_STAGES ? issued - LX_STAGES : 0; i < issued; i++) mbar_wait_bounded(&full[i % LX_STAGES], (i / LX_STAGES) & 1);
+        atomicAdd(&a.status->wait_giveups, 1);
+    }
+    __syncthreads();
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+}
+
+// ------------------------------------------------------------------ around the products
+// x of tokens [t0, t0 + tokens) -> [token][ldx] 16-bit rows, zeros for tokens without a target; fp32 as two bf16 parts.
+template <typename T, typename H>
+__global__ void __launch_bounds__(256) lx_pack_x_kernel(H *hi, H *lo, const T *__restrict__ x, const void *__restrict__ targets, int id_u16, int V, int t0, int tokens,
+                                                        int D, int S, size_t ldx) {
+    __shared__ float tile[32][33];
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    const int t = blockIdx.x * 32 + tx, d0 = blockIdx.y * 32;
+    const bool live = t < tokens && lx_target(targets, id_u16, V, t0 + t) >= 0;
+    const int b = (t0 + t) / S, s = (t0 + t) % S;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int d = d0 + ty + 8 * i;
+        tile[ty + 8 * i][tx] = live && d < D ? Elt<T>::to_f(x[((size_t)b * D + d) * S + s]) : 0.0f;
+    }
+    __syncthreads();
+    const int d = d0 + tx;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int r = blockIdx.x * 32 + ty + 8 * i;
+        if (r < tokens && d < (int)ldx) {
+            const float v = tile[tx][ty + 8 * i];
+            const H h = Elt<H>::from_f(v);
+            hi[(size_t)r * ldx + d] = h;
+            if (lo) lo[(size_t)r * ldx + d] = Elt<H>::from_f(v - Elt<H>::to_f(h));
+        }
+    }
+}
+
+// Rows of the table -> [row][lde] 16-bit rows with aligned ends; fp32 as two bf16 parts.
+template <typename T, typename H>
+__global__ void __launch_bounds__(256) lx_pack_rows_kernel(H *hi, H *lo, const T *__restrict__ src, int rows, int D, size_t lde) {
+    for (int r = blockIdx.x; r < rows; r += gridDim.x)
+        for (int d = threadIdx.x; d < (int)lde; d += 256) {
+            const float v = d < D ? Elt<T>::to_f(src[(size_t)r * D + d]) : 0.0f;
+            const H h = Elt<H>::from_f(v);
+            hi[(size_t)r * lde + d] = h;
+            if (lo) lo[(size_t)r * lde + d] = Elt<H>::from_f(v - Elt<H>::to_f(h));
+        }
+}
+
+// (max, sum) pairs of the vocabulary tiles -> lse and loss of 32 tokens per block, tiles joined in a fixed order.
+__global__ void __launch_bounds__(256) lx_join_kernel(float *__restrict__ lse2, float *__restrict__ loss_tok, const float2 *__restrict__ part, const float *__restrict__ hit,
+                                                      const void *__restrict__ targets, int id_u16, int V, int tiles, int tokens, size_t ldt, ane_cuda_status *status) {
+    __shared__ float2 sh[8][32];
+    const int cl = threadIdx.x & 31, sl = threadIdx.x >> 5;
+    const int t = blockIdx.x * 32 + cl;
+    float m = -INFINITY, s = 0.0f;
+    if (t < tokens)
+#pragma unroll 4
+        for (int i = sl; i < tiles; i += 8) {
+            const float2 p = part[(size_t)i * ldt + t];
+            const float mn = fmaxf(m, p.x);
+            s = s * lx_exp2(m - mn) + p.y * lx_exp2(p.x - mn);
+            m = mn;
+        }
+    sh[sl][cl] = make_float2(m, s);
+    __syncthreads();
+    if (sl != 0 || t >= tokens) return;
+    m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 8; i++) m = fmaxf(m, sh[i][cl].x);
+    s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) if (sh[i][cl].y != 0.0f) s += sh[i][cl].y * lx_exp2(sh[i][cl].x - m);      // slices without a tile hold (-inf, 0)
+    const float l2 = m + log2f(s);
+    lse2[t] = l2;
+    const int id = id_u16 ? (int)static_cast<const uint16_t *>(targets)[t] : static_cast<const int32_t *>(targets)[t];
+    float loss = 0.0f;
+    if (id >= 0 && id < V) {
+        loss = -logf(exp2f(fmaf(hit[t], LX_LOG2E, -l2)) + 1e-10f);
+        if (!isfinite(loss)) atomicAdd(&status->nonfinite, 1);
+    } else if (id >= V) {
+        atomicAdd(&status->oor_ids, 1);
+    }
+    loss_tok[t] = loss;
+}
+
+// dx[b][d][s] = alpha * sum over the shares of K, in order.
+template <typename T>
+__global__ void __launch_bounds__(256) lx_finish_dx_kernel(T *__restrict__ dx, const float *__restrict__ sums, int splits, int t0, int tokens, int D, int S, size_t ldt, float alpha) {
+    const int t = blockIdx.x * 256 + threadIdx.x;
+    if (t >= tokens) return;
+    const int b = (t0 + t) / S, s = (t0 + t) % S;
+    for (int d = blockIdx.y; d < D; d += gridDim.y) {
+        float v = 0.0f;
+        for (int k = 0; k < splits; k++) v += sums[((size_t)k * D + d) * ldt + t];
+        dx[((size_t)b * D + d) * S + s] = Elt<T>::from_f(v * alpha);
+    }
+}
+
+// loss_seq[b] = (sum_t loss_tok[b][t]) / S, fixed summation tree.
+__global__ void __launch_bounds__(256) lx_loss_kernel(float *__restrict__ loss_seq, const float *__restrict__ loss_tok, int S) {
+    __shared__ float sh[8];
+    const float *p = loss_tok + (size_t)blockIdx.x * S;
+    float acc = 0.0f;
+    for (int t = threadIdx.x; t < S; t += 256) acc += p[t];
+    acc = warp_sum(acc);
+    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = acc;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        float s = 0.0f;
+        for (int i = 0; i < 8; i++) s += sh[i];
+        loss_seq[blockIdx.x] = s / (float)S;
+    }
+}
+
+template <int EPI> static int lx_launch(cudaStream_t st, const LxMaps &maps, const LxArgs &a) {
+    static bool ready = false;
+    if (!ready) {
+        ANE_CUDA_TRY(cudaFuncSetAttribute(lx_gemm_kernel<EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)LX_SMEM));
+        ready = true;
+    }
+    const long long tiles = (long long)a.m_tiles * a.n_tiles * a.splits;
+    const int grid = tiles < ctx().sm_count ? (int)tiles : ctx().sm_count;
+    lx_gemm_kernel<EPI><<<grid, LX_THREADS, LX_SMEM, st>>>(maps, a);
+    ANE_LAUNCH_OK(1);
+    return ANE_CUDA_OK;
+}
+
+static inline int lx_div(long long a, long long b) { return (int)((a + b - 1) / b); }
+
+// Instruction descriptor: fp32 accumulator, 16-bit operands of one type, their layouts, the tile.
+static uint32_t lx_idesc(bool half_type, bool a_mn, bool b_mn) {
+    const uint32_t f = half_type ? 0u : 1u;
+    return 1u << 4 | f << 7 | f << 10 | (a_mn ? 1u : 0u) << 15 | (b_mn ? 1u : 0u) << 16 | (uint32_t)(LX_BN >> 3) << 17 | (uint32_t)(LX_BM >> 4) << 24;
+}
+
+struct LxCall {
+    cudaStream_t st;
+    ane_dtype dtype;
+    int id_u16, B, D, V, S;
+    float *loss_seq, *loss_tok;
+    void *dx;
+    float *d_table;
+    const void *x, *table, *targets;
+    float grad_scale;
+};
+
+template <typename T, typename H> static int lx_run(const LxCall &c) {
+    const bool split = sizeof(T) == 4;                       // fp32 inputs as two parts
+    const ane_dtype part = c.dtype == ANE_F16 ? ANE_F16 : ANE_BF16;
+    const int half_type = part == ANE_F16;
+    const bool grad = c.dx || c.d_table;
+    const int T_all = c.B * c.S, D = c.D, V = c.V;
+    const size_t ldd = round_up((size_t)D, 8);
+    const bool pack_table = split || D % 8 || !aligned16(c.table);
+    // Tokens of one round and vocabulary rows of one piece: the two parts of dl stay within 64 MiB, half of L2.
+    const int chunk = T_all < 4096 ? T_all : 4096;
+    long long piece = (16ll << 20) / round_up((size_t)chunk, 128) / 256 * 256;
+    if (piece < 1024) piece = 1024;
+    if (piece > (long long)round_up((size_t)V, 256)) piece = (long long)round_up((size_t)V, 256);
+    const int vp = (int)piece;
+    const size_t ldt = round_up((size_t)chunk, 32), ldl = (size_t)vp;
+    const int v_tiles = lx_div(V, LX_BN);
+    const int segs = split ? 3 : 1;
+
+    const int dx_tiles = lx_div(chunk, LX_BM) * lx_div(D, LX_BN);
+    const int dx_blocks = segs * lx_div(vp, LX_BK);
+    int splits = ctx().sm_count / dx_tiles;
+    if (splits > dx_blocks / 4) splits = dx_blocks / 4;
+    if (splits < 1) splits = 1;
+
+    size_t off = 0;
+    auto take = [&](size_t bytes) { const size_t at = off; off += round_up(bytes, 1024); return at; };
+    const size_t o_tok = take(c.loss_tok ? 0 : (size_t)T_all * 4), o_lse = take(ldt * 4), o_hit = take(ldt * 4), o_part = take((size_t)v_tiles * ldt * 8);
+    const size_t o_xh = take((size_t)chunk * ldd * 2), o_xl = take(split ? (size_t)chunk * ldd * 2 : 0);
+    const size_t o_eh = take(pack_table ? (size_t)vp * ldd * 2 : 0), o_el = take(split ? (size_t)vp * ldd * 2 : 0);
+    const bool need_lo = c.d_table || split;
+    const size_t o_lh = take(grad ? (size_t)chunk * ldl * 2 : 0), o_ll = take(grad && need_lo ? (size_t)chunk * ldl * 2 : 0);
+    const size_t o_dx = take(c.dx ? (size_t)splits * D * ldt * 4 : 0);
+    char *ws = static_cast<char *>(workspace(off));
+    if (!ws) return fail(ANE_CUDA_ERR_NOMEM, "ane_cuda_linear_cross_entropy_dev: no scratch (%zu bytes)", off);
+    float *loss_tok = c.loss_tok ? c.loss_tok : reinterpret_cast<float *>(ws + o_tok);
+    float *lse2 = reinterpret_cast<float *>(ws + o_lse), *hit = reinterpret_cast<float *>(ws + o_hit), *dxs = reinterpret_cast<float *>(ws + o_dx);
+    float2 *parts = reinterpret_cast<float2 *>(ws + o_part);
+    H *xh = reinterpret_cast<H *>(ws + o_xh), *xl = split ? reinterpret_cast<H *>(ws + o_xl) : nullptr;
+    H *eh = reinterpret_cast<H *>(ws + o_eh), *el = split ? reinterpret_cast<H *>(ws + o_el) : nullptr;
+    void *lh = ws + o_lh, *ll = need_lo ? ws + o_ll : nullptr;
+    const size_t idb = c.id_u16 ? 2 : 4;
+    ane_cuda_status *status = ctx().status;
+
+    for (int t0 = 0; t0 < T_all; t0 += chunk) {
+        const int n_tok = T_all - t0 < chunk ? T_all - t0 : chunk;
+        const void *tg = static_cast<const char *>(c.targets) + (size_t)t0 * idb;
+        lx_pack_x_kernel<T, H><<<dim3(lx_div(n_tok, 32), lx_div(D, 32)), 256, 0, c.st>>>(xh, xl, static_cast<const T *>(c.x), c.targets, c.id_u16, V, t0, n_tok, D, c.S, ldd);
+        ANE_LAUNCH_OK(1);
+
+        LxArgs a = {};
+        a.segments = segs; a.kblocks = lx_div(D, LX_BK); a.splits = 1; a.span = 1 << 20;
+        a.m_tiles = lx_div(n_tok, LX_BM); a.m = n_tok;
+        a.idesc = lx_idesc(half_type, false, false);
+        a.targets = tg; a.id_u16 = c.id_u16; a.V = V;
+        a.part = parts; a.hit = hit; a.lse2 = lse2; a.ldt = ldt;
+        a.half_type = half_type; a.dscale = half_type ? 16384.0f : 1.0f;
+        a.status = status;
+        // x (K-major) and a piece of the table (K-major), as up to three pairs
+        auto logit_maps = [&](LxMaps &m, int v0, int nv) -> int {
+            const H *src = pack_table ? eh : reinterpret_cast<const H *>(c.table) + (size_t)v0 * D;
+            const size_t ld = pack_table ? ldd : (size_t)D;
+            if (pack_table) {
+                lx_pack_rows_kernel<T, H><<<nv < 4096 ? nv : 4096, 256, 0, c.st>>>(eh, el, static_cast<const T *>(c.table) + (size_t)v0 * D, nv, D, ldd);
+                ANE_LAUNCH_OK(1);
+            }
+            const H *as[3] = {xl, xh, xh}, *bs[3] = {src, el, src};
+            for (int i = 0; i < segs; i++) {
+                if (int rc = make_matrix_map(&m.a[i], part, as[3 - segs + i], n_tok, D, ldd, LX_BM)) return rc;
+                if (int rc = make_matrix_map(&m.b[i], part, bs[3 - segs + i], nv, D, ld, LX_BN)) return rc;
+            }
+            return ANE_CUDA_OK;
+        };
+        // statistics: the whole table in one launch, or piece by piece where it has to be packed
+        const int fstep = pack_table ? vp : V;
+        for (int v0 = 0; v0 < V; v0 += fstep) {
+            const int nv = V - v0 < fstep ? V - v0 : fstep;
+            LxMaps m;
+            if (int rc = logit_maps(m, v0, nv)) return rc;
+            a.n_tiles = lx_div(nv, LX_BN); a.n = nv; a.v0 = v0; a.tile0 = v0 / LX_BN;
+            if (int rc = lx_launch<LX_STATS>(c.st, m, a)) return rc;
+        }
+        lx_join_kernel<<<lx_div(n_tok, 32), 256, 0, c.st>>>(lse2, loss_tok + t0, parts, hit, tg, c.id_u16, V, v_tiles, n_tok, ldt, status);
+        ANE_LAUNCH_OK(1);
+        if (!grad) continue;
+
+        const float alpha = c.grad_scale / (float)c.S / a.dscale;
+        for (int v0 = 0; v0 < V; v0 += vp) {
+            const int nv = V - v0 < vp ? V - v0 : vp;
+            LxMaps m;
+            if (int rc = logit_maps(m, v0, nv)) return rc;
+            a.n_tiles = lx_div(nv, LX_BN); a.n = nv; a.v0 = v0;
+            a.hi = lh; a.lo = ll; a.ldl = ldl;
+            if (int rc = lx_launch<LX_DLOGITS>(c.st, m, a)) return rc;
+            if (c.dx) {
+                LxArgs g = a;
+                LxMaps gm;
+                const H *src = pack_table ? eh : reinterpret_cast<const H *>(c.table) + (size_t)v0 * D;
+                const void *as[3] = {ll, lh, lh};
+                const H *bs[3] = {src, el, src};
+                for (int i = 0; i < segs; i++) {
+                    if (int rc = make_matrix_map(&gm.a[i], part, as[3 - segs + i], n_tok, nv, ldl, LX_BM)) return rc;
+                    if (int rc = make_matrix_map(&gm.b[i], part, bs[3 - segs + i], nv, D, pack_table ? ldd : (size_t)D, LX_BK)) return rc;
+                }
+                g.kblocks = lx_div(nv, LX_BK); g.splits = splits;
+                if (split) g.span = LX_SPAN;                 // a 16-bit result does not show what the accumulator cuts off
+                g.n_tiles = lx_div(D, LX_BN); g.n = D;
+                g.idesc = lx_idesc(half_type, false, true);
+                g.out = dxs; g.first = v0 == 0;
+                if (int rc = lx_launch<LX_DX>(c.st, gm, g)) return rc;
+            }
+            if (c.d_table) {
+                LxArgs g = a;
+                LxMaps gm;
+                // dl in two parts always; fp32 x adds the product of its own low part
+                const H *as[3] = {xl, xh, xh};
+                const void *bs[3] = {lh, ll, lh};
+                g.segments = split ? 3 : 2;
+                for (int i = 0; i < g.segments; i++) {
+                    if (int rc = make_matrix_map(&gm.a[i], part, as[3 - g.segments + i], n_tok, D, ldd, LX_BK)) return rc;
+                    if (int rc = make_matrix_map(&gm.b[i], part, bs[3 - g.segments + i], n_tok, nv, ldl, LX_BK)) return rc;
+                }
+                g.kblocks = lx_div(n_tok, LX_BK); g.span = LX_SPAN;
+                g.m_tiles = lx_div(D, LX_BM); g.m = D;
+                g.n_tiles = lx_div(nv, LX_BN); g.n = nv;
+                g.idesc = lx_idesc(half_type, true, true);
+                g.out = c.d_table + (size_t)v0 * D; g.ldt = (size_t)D; g.alpha = alpha;
+                if (int rc = lx_launch<LX_DTABLE>(c.st, gm, g)) return rc;
+            }
+        }
+        if (c.dx) {
+            const int by = D < 1024 ? D : 1024;
+            lx_finish_dx_kernel<T><<<dim3(lx_div(n_tok, 256), by), 256, 0, c.st>>>(static_cast<T *>(c.dx), dxs, splits, t0, n_tok, D, c.S, ldt, alpha);
+            ANE_LAUNCH_OK(1);
+        }
+    }
+    lx_loss_kernel<<<c.B, 256, 0, c.st>>>(c.loss_seq, loss_tok, c.S);
+    ANE_LAUNCH_OK(1);
+    return ANE_CUDA_OK;
+}
+
+}  // namespace ane
+
+using namespace ane;
+
+extern "C" {
+
+int ane_cuda_linear_cross_entropy_dev(void *stream, ane_dtype dtype, ane_idtype idtype, int B, int D, int V, int S, float *loss_seq, float *loss_tok, void *dx,
+                                      float *d_table, const void *x, const void *table, const void *targets, float grad_scale) {
+    ANE_REQUIRE_INIT();
+    ANE_REQUIRE(loss_seq && x && table && targets, "%s: null pointer", __func__);
+    ANE_REQUIRE(dtype_ok(dtype), "%s: bad dtype %d", __func__, (int)dtype);
+    ANE_REQUIRE(idtype == ANE_ID_U16 || idtype == ANE_ID_I32, "%s: bad id type", __func__);
+    ANE_REQUIRE(B >= 1 && D >= 1 && V >= 1 && S >= 1, "%s: bad shape B=%d D=%d V=%d S=%d", __func__, B, D, V, S);
+    ANE_REQUIRE((long long)B * S < 0x7fffff00LL && V < 0x7fffff00 && D <= 65536, "%s: too many tokens, or D above 65536", __func__);
+    ANE_REQUIRE(!dx || dx != x, "%s: dx may not be x", __func__);
+    const size_t e = dtype_size(dtype), xb = (size_t)B * D * S * e;
+    ANE_CHECK_EXTENT(loss_seq, (size_t)B * 4); ANE_CHECK_EXTENT(loss_tok, (size_t)B * S * 4); ANE_CHECK_EXTENT(dx, xb); ANE_CHECK_EXTENT(x, xb);
+    ANE_CHECK_EXTENT(table, (size_t)V * D * e); ANE_CHECK_EXTENT(d_table, (size_t)V * D * 4);
+    ANE_CHECK_EXTENT(targets, (size_t)B * S * (idtype == ANE_ID_U16 ? 2 : 4));
+    const LxCall c = {(cudaStream_t)stream, dtype, idtype == ANE_ID_U16, B, D, V, S, loss_seq, loss_tok, dx, d_table, x, table, targets, grad_scale};
+    switch (dtype) {
+        case ANE_F32: return lx_run<float, __nv_bfloat16>(c);
+        case ANE_BF16: return lx_run<__nv_bfloat16, __nv_bfloat16>(c);
+        default: return lx_run<__half, __half>(c);
+    }
+}
+
+}  // extern "C"

@@ -21,6 +21,10 @@ namespace ane {
 int make_bcs_tensor_map(CUtensorMap *map, ane_dtype dtype, const void *base, int B, int C, int S, int box_s, int box_c,
                         int l2_promotion_bytes = 128);
 
+// Row-major matrix of 16-bit elements (bf16 or fp16), rows x cols with `ld` elements between rows, seen as a 2-D map with
+// 128-byte swizzled boxes of 64 columns x box_rows rows.  Rows and columns outside the matrix read as zeros.
+int make_matrix_map(CUtensorMap *map, ane_dtype dtype, const void *base, size_t rows, size_t cols, size_t ld, int box_rows);
+
 #ifdef __CUDACC__
 // ------------------------------------------------------------------ device primitives
 __device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }

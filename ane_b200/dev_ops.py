@@ -243,6 +243,30 @@ def cross_entropy(logits, targets, grad_scale=1.0, dlogits=None):
     return loss, dlogits
 
 
+def linear_cross_entropy(x, table, targets, d_table=None, grad_scale=1.0, dx=None, grad=True, loss_tok=None):
+    """Classifier product and cross-entropy without the logits: x [B, D, S], table [V, D] of the same dtype, targets [B, S];
+    returns (loss_seq [B], dx).  d_table (fp32 [V, D]) is accumulated into, None: not wanted.  grad=False computes the losses
+    alone (dx is then None).  loss_tok (fp32 [B, S]) receives the loss of every token.  A target outside [0, V) marks a token
+    without a target: no loss and no gradient."""
+    B, D, S = _bcs(x)
+    _like("table", table, (table.shape[0], D), x.dtype)
+    if tuple(targets.shape) not in ((B, S), (S,) if x.dim() == 2 else (B, S)) or targets.dtype not in _ID:
+        raise ValueError(f"targets: expected int32 or uint16 {(B, S)}, got {targets.dtype} {tuple(targets.shape)}")
+    if not grad and (dx is not None or d_table is not None):
+        raise ValueError("grad=False computes the losses alone: no dx, no d_table")
+    V = table.shape[0]
+    _like("d_table", d_table, (V, D), torch.float32)
+    _like("loss_tok", loss_tok, targets.shape, torch.float32)
+    _like("dx", dx, x.shape, x.dtype)
+    _same_device(x, table, targets, d_table, dx, loss_tok)
+    if grad and dx is None:
+        dx = torch.empty_like(x)
+    loss = torch.empty(B, dtype=torch.float32, device=x.device)
+    _l.check(_l.load().ane_cuda_linear_cross_entropy_dev(_stream(), _dt(x), _ID[targets.dtype], B, D, V, S, _p(loss), _p(loss_tok), _p(dx), _p(d_table),
+                                                        _p(x), _p(table), _p(targets), grad_scale))
+    return loss, dx
+
+
 def adam(w, g, m, v, t, lr, b1, b2, eps, wd=0.0, gscale=1.0, clip=None, dynamic=True):
     _l.check(_l.load().ane_cuda_adam_dev(_stream(), w.numel(), _p(w), _p(g), _p(m), _p(v), t, lr, b1, b2, eps, wd,
                                         gscale, _p(clip), _l.ADAM_DYNAMIC if dynamic else _l.ADAM_STORIES))

@@ -121,6 +121,7 @@ PROTOTYPES = {
     "ane_cuda_embed_lookup_dev": (_i, [_vp, _i, _i, _i, _i, _i, _vp, _vp, _vp, _i, _u]),
     "ane_cuda_embed_backward_dev": (_i, [_vp, _i, _i, _i, _i, _i, _vp, _vp, _vp, _i]),
     "ane_cuda_cross_entropy_dev": (_i, [_vp, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _f]),
+    "ane_cuda_linear_cross_entropy_dev": (_i, [_vp, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _f]),
     "ane_cuda_adam_dev": (_i, [_vp, _sz, _vp, _vp, _vp, _vp, _i, _f, _f, _f, _f, _f, _f, _vp, _u]),
     "ane_cuda_adam_multi_dev": (_i, [_vp, _i, _i, _i, _i, _vp, _i, _f, _f, _f, _f, _f, _vp, _u, _u]),
     "ane_cuda_adam_state_unpack_dev": (_i, [_vp, _sz, _vp, _vp, _vp, _i]),

@@ -320,6 +320,19 @@ int ane_cuda_embed_backward_dev(void *stream, ane_dtype dtype, ane_idtype idtype
 int ane_cuda_cross_entropy_dev(void *stream, ane_idtype idtype, int B, int V, int S,
                                float *dlogits, const float *logits, const void *targets,
                                float *loss_seq, float grad_scale);
+/* The classifier product and a11 in one operator, in pieces of the vocabulary, without the logits: what cblas_sgemm over the
+ * table, cross_entropy and the two backward products of the classifier do together (training_dynamic/train.m:490-509).
+ *   l = table x (per token), loss_t = -log(p[tgt]+1e-10), loss_seq[b] = sum_t loss_t / S,
+ *   dl = (p - onehot)/S * grad_scale, dx = table^T dl (overwritten), d_table += dl x^T (fp32)
+ * x, dx [B][D][S] and table [V][D] have dtype; loss_tok (fp32 [B][S]), dx and d_table may each be NULL; with neither dx nor
+ * d_table only the losses are computed.  A target outside [0, V) marks a token without a target (padding): no loss, a zero
+ * column in dx, nothing added to d_table, whatever its x holds -- unlike ane_cuda_cross_entropy_dev, which keeps the
+ * reference's plain-softmax gradient there.  Ids >= V are counted in the status words, negative ones are not.  The products
+ * run on the tensor cores with fp32 sums; fp32 inputs enter as two bf16 parts each, dl as two 16-bit parts in d_table and as
+ * one in a 16-bit dx.  Bit-stable from call to call.  Scratch: about 100 to 250 MiB of the library's range. */
+int ane_cuda_linear_cross_entropy_dev(void *stream, ane_dtype dtype, ane_idtype idtype, int B, int D, int V, int S,
+                                      float *loss_seq, float *loss_tok, void *dx, float *d_table, const void *x,
+                                      const void *table, const void *targets, float grad_scale);
 /* a12 (+a13 folded): Adam over a flat fp32 range.  g is first multiplied by gscale and then by
  * *clip_dev (a device scalar, NULL = 1), as train.m:750-767 and :809-825 do in two passes.
  * flags = ANE_ADAM_STORIES or ANE_ADAM_DYNAMIC. */
