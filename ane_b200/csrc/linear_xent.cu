@@ -16,14 +16,15 @@
 //
 // Precision.  16-bit inputs enter the products as they are.  dl is rounded to 16 bits for dx, whose result is rounded to 16
 // bits as well; d_table is an fp32 sum, so dl enters it as two 16-bit numbers, the rounded value and what the rounding left
-// (17 bits and more), at the price of one more product.  fp32 inputs are split the same way into two bf16 parts and every
-// product is taken as high*high + high*low + low*high: what is dropped is below 2^-17 of a term.  In fp16 dl is scaled by 2^14
-// (|dl| * S / grad_scale <= 1 becomes 16384 at most), so that the probabilities of a large vocabulary, 1e-5 and less, do not
-// fall among fp16's subnormals.
+// (17 bits and more), at the price of one more product.  fp32 inputs are split into two fp16 parts after scaling by a power of
+// two that puts the tensor's largest magnitude at 2^13: 22 bits of every number above 2^-28 of the largest.  Every product is
+// then low*high + high*low + high*high; what is dropped is below 2^-22 of a term.  Where dl is held in fp16 it is scaled by
+// 2^14 (|dl| * S / grad_scale <= 1 becomes 16384 at most), so that the probabilities of a large vocabulary, 1e-5 and less, do
+// not fall among fp16's subnormals.
 //
 // The accumulators of the tensor cores cut off what does not fit instead of rounding: every step of 16 along K takes half a
 // unit of the last place from the sum on average, 3e-8 of it (measured: 1.2e-5 after 345 steps).  So fp32 results leave the
-// accumulator after 2048 elements of K, 128 steps, and are added up in memory with rounding; and the products with a low part
+// accumulator after 512 elements of K, 32 steps, and are added up in registers with rounding; and the products with a low part
 // go first, while the sum is small.
 //
 // A token without a target (id outside [0, V)) has zeros in place of its x, so that nothing it holds -- infinities and NaN
@@ -36,13 +37,17 @@
 namespace ane {
 
 constexpr float LX_LOG2E = 1.4426950408889634f;
-constexpr int LX_BM = 128, LX_BN = 256, LX_BK = 64;      // tile of a block: M x N outputs, K elements per stage
-constexpr int LX_STAGES = 4;
-constexpr int LX_A_BYTES = LX_BM * LX_BK * 2, LX_B_BYTES = LX_BN * LX_BK * 2, LX_STAGE_BYTES = LX_A_BYTES + LX_B_BYTES;
-constexpr int LX_THREADS = 192;                          // copy warp, matrix warp, four epilogue warps
+constexpr int LX_CTA_M = 128;                            // rows of the tile in each block of a pair
+constexpr int LX_BM = 2 * LX_CTA_M, LX_BN = 256, LX_BK = 64;      // tile of a pair: M x N outputs, K elements per stage
+constexpr int LX_STAGES = 6;
+constexpr int LX_A_BYTES = LX_CTA_M * LX_BK * 2, LX_B_BYTES = LX_BN / 2 * LX_BK * 2, LX_STAGE_BYTES = LX_A_BYTES + LX_B_BYTES;
+constexpr int LX_EPI_WARPS = 8;                          // two for each 32 accumulator lanes, half of the columns each
+constexpr int LX_COLS = LX_BN / 2;                       // columns of an epilogue warp
+constexpr int LX_THREADS = 64 + 32 * LX_EPI_WARPS;       // copy warp, matrix warp, epilogue warps
 constexpr size_t LX_SMEM = (size_t)LX_STAGES * LX_STAGE_BYTES + 1024;
-constexpr int LX_SPAN = 2048 / LX_BK;                    // K blocks summed in an accumulator where an fp32 result is wanted
+constexpr int LX_SPAN = 512 / LX_BK;                     // K blocks that stay in an accumulator where an fp32 result is wanted
 constexpr int LX_WAIT_LIMIT = 1 << 20;
+constexpr float LX_HALF_SCALE = 16384.0f;                // of dl where it is held in fp16
 
 enum LxEpilogue { LX_STATS, LX_DLOGITS, LX_DX, LX_DTABLE };
 
@@ -51,14 +56,15 @@ struct LxArgs {
     int segments;              // pairs in use
     int kblocks;               // K blocks of one pair
     int splits;                // shares of the K blocks, each with its own sums (dx only)
-    int span;                  // K blocks that one accumulator sums before it is added to memory (dx, d_table)
+    int span;                  // K blocks that one accumulator sums before its values move to registers (dx, d_table)
     int m_tiles, n_tiles;
     int m, n;                  // valid rows and columns of the output
     uint32_t idesc;
     // stats, dlogits: m = tokens, n = vocabulary rows of the piece from v0
     const void *targets;       // of the first token
     int id_u16, V, v0;
-    float2 *part; int tile0;   // stats: [vocabulary tile][ldt], this piece's first tile
+    const float *scales;       // fp32 inputs: {1 / scale of x, 1 / scale of the table}; else null
+    float2 *part; int tile0;   // stats: [half vocabulary tile][ldt], this piece's first
     float *hit;                // stats: the target's logit per token
     const float *lse2;         // dlogits: lse * log2(e)
     void *hi, *lo; size_t ldl; // dlogits: [token][ldl], lo may be null
@@ -77,20 +83,32 @@ __device__ __forceinline__ uint64_t lx_desc(uint32_t addr, uint32_t lead) {
     return (uint64_t)((addr >> 4) & 0x3fffu) | (uint64_t)(lead >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
 }
 __device__ __forceinline__ void lx_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
                  ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
+// Arrives on the barrier of this offset in both blocks of the pair once the matrix instructions issued so far are done.
 __device__ __forceinline__ void lx_commit(uint64_t *bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                 ::"r"(smem_u32(bar)), "h"((uint16_t)3) : "memory");
 }
 __device__ __forceinline__ void lx_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void lx_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void lx_arrive(uint64_t *bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+// Address of the first block's copy of a shared variable.
+__device__ __forceinline__ uint32_t lx_in_leader(const void *p) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_u32(p)));
+    return r;
 }
-__device__ __forceinline__ void lx_load_box(uint32_t dst, const CUtensorMap *map, int x, int y, uint64_t *bar) {
-    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-                 ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_u32(bar)) : "memory");
+__device__ __forceinline__ void lx_arrive_at(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// A box into this block's shared memory, counted on a barrier of the pair's first block.
+__device__ __forceinline__ void lx_load_box(uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void lx_pair_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // 32 accumulator columns of this warp's 32 lanes: v[j] = column + j of the thread's own row.
 __device__ __forceinline__ void lx_tmem_load(uint32_t addr, float (&v)[32]) {
@@ -127,7 +145,7 @@ __device__ __forceinline__ int lx_target(const void *targets, int id_u16, int V,
     return id >= 0 && id < V ? id : -1;
 }
 
-// 16 fp32 values -> 16-bit high parts and, with `lo`, the 16-bit rest of each.
+// Two fp32 values -> their 16-bit roundings, and the roundings of what was left.
 __device__ __forceinline__ void lx_split2(float a, float b, int half_type, uint32_t &hi, uint32_t &lo) {
     if (half_type) {
         const __half2 h = __floats2half2_rn(a, b);
@@ -172,32 +190,38 @@ struct LxRange {
 };
 
 // ------------------------------------------------------------------ the product
-// Persistent blocks walk the output tiles.  One thread copies operand boxes into a ring of four stages, one thread issues the
-// matrix instructions into one of two accumulators, four warps work on the accumulator that is complete.
+// Pairs of blocks on neighbouring SMs walk tiles of 256 x 256 outputs: each block holds 128 rows of A, 128 of B's 256 rows and
+// the accumulators of its own 128 output rows, and the matrix instructions of the first block read both blocks' operands.  Per
+// 16 elements of K an SM then reads 8 KB of operands from shared memory in 128 clocks, where a block on its own (128 x 256)
+// reads 12.  In each block one thread copies operand boxes into a ring of six stages; in the first block one thread issues the
+// matrix instructions into one of two accumulators; eight warps work on the accumulator that is complete.
 template <int EPI>
-__global__ void __launch_bounds__(LX_THREADS, 1) lx_gemm_kernel(const __grid_constant__ LxMaps maps, const __grid_constant__ LxArgs a) {
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LX_THREADS, 1) lx_gemm_kernel(const __grid_constant__ LxMaps maps, const __grid_constant__ LxArgs a) {
     constexpr bool A_MN = EPI == LX_DTABLE, B_MN = EPI == LX_DX || EPI == LX_DTABLE;
     extern __shared__ uint8_t raw[];
-    const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
+    const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;       // the same offset in both blocks
+    // full and acc_empty are used in the first block only; the others are each block's own
     __shared__ uint64_t full[LX_STAGES], empty[LX_STAGES], acc_full[2], acc_empty[2], drained;
     __shared__ uint32_t tmem_at;
     __shared__ int give_up;
     volatile int *abort = &give_up;
 
     const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+    const int rank = blockIdx.x & 1, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
     if (threadIdx.x == 0) {
         for (int i = 0; i < LX_STAGES; i++) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
-        for (int i = 0; i < 2; i++) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], 4); }
+        for (int i = 0; i < 2; i++) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], 2 * LX_EPI_WARPS); }
         mbar_init(&drained, 1);
         give_up = 0;
         mbar_init_fence();
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&tmem_at)) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&tmem_at)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
         lx_fence_before();
     }
     __syncthreads();
+    lx_pair_sync();
     lx_fence_after();
     const uint32_t tmem = tmem_at;
 
@@ -206,35 +230,35 @@ __global__ void __launch_bounds__(LX_THREADS, 1) lx_gemm_kernel(const __grid_con
 
     if (warp == 0) {
         if (lane == 0) {
-            for (int tile = blockIdx.x; tile < tiles && !*abort; tile += gridDim.x) {
+            for (int tile = pair; tile < tiles && !*abort; tile += pairs) {
                 const int mt = tile % a.m_tiles, nt = tile / a.m_tiles % a.n_tiles;
-                LxRange r(a, tile);
-                for (; !r.done(); r.next(), issued++) {
+                const int am = mt * LX_BM + rank * LX_CTA_M, bn = nt * LX_BN + rank * (LX_BN / 2);
+                for (LxRange r(a, tile); !r.done(); r.next(), issued++) {
                     const int st = issued % LX_STAGES;
                     if (!lx_wait(&empty[st], ((issued / LX_STAGES) & 1) ^ 1, abort)) break;
                     const int seg = r.seg, k = r.k * LX_BK;
-                    const uint32_t sa = base + st * LX_STAGE_BYTES, sb = sa + LX_A_BYTES;
-                    mbar_arrive_expect_tx(&full[st], LX_STAGE_BYTES);
+                    const uint32_t sa = base + st * LX_STAGE_BYTES, sb = sa + LX_A_BYTES, bar = lx_in_leader(&full[st]);
+                    if (rank == 0) mbar_arrive_expect_tx(&full[st], 2 * LX_STAGE_BYTES);
                     if constexpr (A_MN) {
 #pragma unroll
-                        for (int i = 0; i < LX_BM / 64; i++) lx_load_box(sa + i * 8192, &maps.a[seg], mt * LX_BM + i * 64, k, &full[st]);
+                        for (int i = 0; i < LX_CTA_M / 64; i++) lx_load_box(sa + i * 8192, &maps.a[seg], am + i * 64, k, bar);
                     } else {
-                        lx_load_box(sa, &maps.a[seg], k, mt * LX_BM, &full[st]);
+                        lx_load_box(sa, &maps.a[seg], k, am, bar);
                     }
                     if constexpr (B_MN) {
 #pragma unroll
-                        for (int i = 0; i < LX_BN / 64; i++) lx_load_box(sb + i * 8192, &maps.b[seg], nt * LX_BN + i * 64, k, &full[st]);
+                        for (int i = 0; i < LX_BN / 128; i++) lx_load_box(sb + i * 8192, &maps.b[seg], bn + i * 64, k, bar);
                     } else {
-                        lx_load_box(sb, &maps.b[seg], k, nt * LX_BN, &full[st]);
+                        lx_load_box(sb, &maps.b[seg], k, bn, bar);
                     }
                 }
             }
         }
     } else if (warp == 1) {
-        if (lane == 0) {
+        if (lane == 0 && rank == 0) {
             uint32_t used = 0, turn = 0;
             bool ok = true;
-            for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
+            for (int tile = pair; tile < tiles && ok; tile += pairs) {
                 LxRange r(a, tile);
                 uint32_t d = 0, more = 0;
                 for (; !r.done(); used++) {
@@ -257,26 +281,37 @@ __global__ void __launch_bounds__(LX_THREADS, 1) lx_gemm_kernel(const __grid_con
                     if (r.first()) { lx_commit(&acc_full[turn & 1]); turn++; }      // the accumulator is complete
                 }
             }
-            lx_commit(&drained);                            // also after a give-up: no instruction outlives the block
-            mbar_wait_bounded(&drained, 0);
+            lx_commit(&drained);                            // also after a give-up: no instruction or arrival outlives the block
         }
+        if (lane == 0) mbar_wait_bounded(&drained, 0);
     } else {
         const int quad = warp & 3, row = quad * 32 + lane;   // a warp reads the accumulator lanes of its place in the group of four
+        const int c0 = warp >= 2 + LX_EPI_WARPS / 2 ? LX_COLS : 0;
         uint32_t turn = 0;
         bool ok = true;
-        for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
-          const int mt = tile % a.m_tiles, nt = tile / a.m_tiles % a.n_tiles, ks = tile / (a.m_tiles * a.n_tiles);
-          const int m = mt * LX_BM + row, n0 = nt * LX_BN;
-          const int cols = a.n - n0 < LX_BN ? a.n - n0 : LX_BN;
-          const LxRange range(a, tile);
-          if (EPI == LX_DX && a.first && range.k0 >= range.k1 && m < a.m)          // a share without K blocks: zeros
-              for (int c = 0; c < cols; c++) a.out[((size_t)ks * a.n + n0 + c) * a.ldt + m] = 0.0f;
-          for (int part = range.k0; part < range.k1; part += a.span, turn++) {
-            if (!(ok = __all_sync(0xffffffffu, lx_wait(&acc_full[turn & 1], (turn >> 1) & 1, abort)))) break;
-            lx_fence_after();
-            const uint32_t t = tmem + (turn & 1) * LX_BN + ((uint32_t)(quad * 32) << 16);
+        const float unscale = a.scales ? (EPI == LX_DTABLE ? a.scales[0] : EPI == LX_DX ? a.scales[1] : a.scales[0] * a.scales[1]) : 1.0f;
+        for (int tile = pair; tile < tiles && ok; tile += pairs) {
+            const int mt = tile % a.m_tiles, nt = tile / a.m_tiles % a.n_tiles, ks = tile / (a.m_tiles * a.n_tiles);
+            const int m = mt * LX_BM + rank * LX_CTA_M + row, n0 = nt * LX_BN + c0;
+            const int left = a.n - n0, cols = left < 0 ? 0 : left < LX_COLS ? left : LX_COLS;     // of this warp
+            const bool live = m < a.m;
+            // Waits for the accumulator of the next part and gives it back.
+            auto take = [&]() {
+                ok = __all_sync(0xffffffffu, lx_wait(&acc_full[turn & 1], (turn >> 1) & 1, abort));
+                lx_fence_after();
+                return tmem + (turn & 1) * LX_BN + c0 + ((uint32_t)(quad * 32) << 16);
+            };
+            auto give = [&]() {
+                lx_fence_before();
+                __syncwarp();
+                if (lane == 0) lx_arrive_at(lx_in_leader(&acc_empty[turn & 1]));
+                turn++;
+            };
             if constexpr (EPI == LX_STATS) {
-                const int tgt = m < a.m ? lx_target(a.targets, a.id_u16, a.V, m) - a.v0 - n0 : -1;     // column in this tile
+                const uint32_t t = take();
+                if (!ok) break;
+                const int tgt = live ? lx_target(a.targets, a.id_u16, a.V, m) - a.v0 - n0 : -1;     // column of this warp
+                const float k2 = unscale * LX_LOG2E;
                 float mx = -INFINITY, sum = 0.0f;
                 for (int c = 0; c < cols; c += 32) {
                     float v[32];
@@ -285,7 +320,7 @@ __global__ void __launch_bounds__(LX_THREADS, 1) lx_gemm_kernel(const __grid_con
                         float h = 0.0f;
 #pragma unroll
                         for (int j = 0; j < 32; j++) h = tgt == c + j ? v[j] : h;
-                        if (tgt >= c && tgt < c + 32) a.hit[m] = h;
+                        if (tgt >= c && tgt < c + 32) a.hit[m] = h * unscale;
                     }
                     if (c + 32 > cols) {
 #pragma unroll
@@ -294,38 +329,41 @@ __global__ void __launch_bounds__(LX_THREADS, 1) lx_gemm_kernel(const __grid_con
                     float top = v[0];
 #pragma unroll
                     for (int j = 1; j < 32; j++) top = fmaxf(top, v[j]);
-                    const float mnew = fmaxf(mx, top * LX_LOG2E);
+                    const float mnew = fmaxf(mx, top * k2);
                     float part = 0.0f;
 #pragma unroll
-                    for (int j = 0; j < 32; j++) part += lx_exp2(fmaf(v[j], LX_LOG2E, -mnew));
+                    for (int j = 0; j < 32; j++) part += lx_exp2(fmaf(v[j], k2, -mnew));
                     sum = fmaf(sum, lx_exp2(mx - mnew), part);
                     mx = mnew;
                 }
-                if (m < a.m) a.part[(size_t)(a.tile0 + nt) * a.ldt + m] = make_float2(mx, sum);
+                if (live && cols > 0) a.part[(size_t)(a.tile0 + 2 * nt + (c0 != 0)) * a.ldt + m] = make_float2(mx, sum);
+                give();
             } else if constexpr (EPI == LX_DLOGITS) {
-                const int id = m < a.m ? lx_target(a.targets, a.id_u16, a.V, m) : -1;
+                const uint32_t t = take();
+                if (!ok) break;
+                const int id = live ? lx_target(a.targets, a.id_u16, a.V, m) : -1;
                 const int tgt = id >= 0 ? id - a.v0 - n0 : -1;
-                const float lse2 = m < a.m ? a.lse2[m] : 0.0f;
-                const float scale = id >= 0 ? a.dscale : 0.0f;
+                const float lse2 = live ? a.lse2[m] : 0.0f;
+                const float k2 = unscale * LX_LOG2E;
                 const size_t at = (size_t)m * a.ldl + n0;
-                for (int c = 0; c < LX_BN; c += 32) {
+                for (int c = 0; c < LX_COLS; c += 32) {
                     float v[32];
                     lx_tmem_load(t + c, v);
 #pragma unroll
-                    for (int j = 0; j < 32; j++) v[j] = lx_exp2(fmaf(v[j], LX_LOG2E, -lse2)) * scale;
+                    for (int j = 0; j < 32; j++) v[j] = lx_exp2(fmaf(v[j], k2, -lse2)) * a.dscale;
                     if (__any_sync(0xffffffffu, tgt >= c && tgt < c + 32)) {
 #pragma unroll
-                        for (int j = 0; j < 32; j++) v[j] = tgt == c + j ? v[j] - scale : v[j];
+                        for (int j = 0; j < 32; j++) v[j] = tgt == c + j ? v[j] - a.dscale : v[j];
                     }
                     if (c + 32 > cols) {
 #pragma unroll
                         for (int j = 0; j < 32; j++) if (c + j >= cols) v[j] = 0.0f;
                     }
-                    if (m < a.m) {
-                        if (id < 0) {                     // a masked token: zeros, whatever its logits are
+                    if (id < 0) {                         // a masked token: zeros, whatever its logits are
 #pragma unroll
-                            for (int j = 0; j < 32; j++) v[j] = 0.0f;
-                        }
+                        for (int j = 0; j < 32; j++) v[j] = 0.0f;
+                    }
+                    if (live) {
 #pragma unroll
                         for (int h = 0; h < 2; h++) {
                             uint32_t hi[8], lo[8];
@@ -336,58 +374,90 @@ __global__ void __launch_bounds__(LX_THREADS, 1) lx_gemm_kernel(const __grid_con
                         }
                     }
                 }
+                give();
             } else {
                 // dx: rows are tokens, columns are channels; d_table: rows are channels, columns vocabulary rows.  Either way the
-                // 32 lanes of a warp hold 32 neighbours of a contiguous row.
-                // A later part of K follows from the same thread, so the order of the additions is fixed.
-                float *out = EPI == LX_DX ? a.out + ((size_t)ks * a.n + n0) * a.ldt + m : a.out + (size_t)n0 * a.ldt + m;
-                for (int c = 0; c < cols; c += 32) {
-                    float v[32];
-                    lx_tmem_load(t + c, v);
-                    if (m < a.m) {
-                        if (EPI == LX_DX && a.first && part == range.k0) {
+                // 32 lanes of a warp hold 32 neighbours of a contiguous row.  Parts of K are added up in registers.
+                float sum[LX_COLS];
 #pragma unroll
-                            for (int j = 0; j < 32; j++) if (c + j < cols) out[(size_t)(c + j) * a.ldt] = v[j];
-                        } else {
+                for (int j = 0; j < LX_COLS; j++) sum[j] = 0.0f;
+                const LxRange range(a, tile);
+                for (int part = range.k0; part < range.k1; part += a.span) {
+                    const uint32_t t = take();
+                    if (!ok) break;
 #pragma unroll
-                            for (int j = 0; j < 32; j++) if (c + j < cols) lx_add(out + (size_t)(c + j) * a.ldt, EPI == LX_DX ? v[j] : v[j] * a.alpha);
-                        }
+                    for (int c = 0; c < LX_COLS; c += 32) {
+                        float v[32];
+                        lx_tmem_load(t + c, v);
+#pragma unroll
+                        for (int j = 0; j < 32; j++) sum[c + j] += v[j];
+                    }
+                    give();
+                }
+                if (!ok) break;
+                if (live) {
+                    float *out = a.out + ((size_t)(EPI == LX_DX ? ks : 0) * a.n + n0) * a.ldt + m;
+                    const float k = EPI == LX_DTABLE ? a.alpha * unscale : unscale;
+                    if (EPI == LX_DX && a.first) {
+#pragma unroll
+                        for (int j = 0; j < LX_COLS; j++) if (j < cols) out[(size_t)j * a.ldt] = sum[j] * k;
+                    } else if (range.k0 < range.k1) {
+#pragma unroll
+                        for (int j = 0; j < LX_COLS; j++) if (j < cols) lx_add(out + (size_t)j * a.ldt, sum[j] * k);
                     }
                 }
             }
-            lx_fence_before();
-            __syncwarp();
-            if (lane == 0) lx_arrive(&acc_empty[turn & 1]);
-          }
         }
     }
     __syncwarp();
     lx_fence_before();
     __syncthreads();
-    lx_fence_after();
     if (*abort && threadIdx.x == 0) {
-        // copies still on their way into this block's shared memory: every stage's last one
-        for (uint32_t i = issued > LX_STAGES ? issued - LX_STAGES : 0; i < issued; i++) mbar_wait_bounded(&full[i % LX_STAGES], (i / LX_STAGES) & 1);
+        // copies still on their way into shared memory: every stage's last one, counted in the first block
+        if (rank == 0)
+            for (uint32_t i = issued > LX_STAGES ? issued - LX_STAGES : 0; i < issued; i++) mbar_wait_bounded(&full[i % LX_STAGES], (i / LX_STAGES) & 1);
         atomicAdd(&a.status->wait_giveups, 1);
     }
     __syncthreads();
-    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    lx_pair_sync();                                       // the other block may still arrive on, or read from, this one's memory
+    lx_fence_after();
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem));
 }
 
 // ------------------------------------------------------------------ around the products
-// x of tokens [t0, t0 + tokens) -> [token][ldx] 16-bit rows, zeros for tokens without a target; fp32 as two bf16 parts.
+// fp32 inputs: the largest finite magnitude of a tensor, as the bits of a float (which compare like integers).  x is looked
+// at where its token has a target (S and D describe its layout; the table passes no targets).
+__global__ void __launch_bounds__(256) lx_largest_kernel(uint32_t *most, const float *__restrict__ p, size_t n, const void *__restrict__ targets, int id_u16, int V, int D, int S) {
+    uint32_t top = 0;
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) {
+        const uint32_t u = __float_as_uint(p[i]) & 0x7fffffffu;
+        if (u > top && u < 0x7f800000u && (!targets || lx_target(targets, id_u16, V, (int)(i / ((size_t)D * S) * S + i % S)) >= 0)) top = u;
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if ((threadIdx.x & 31) == 0 && top) atomicMax(most, top);      // a maximum does not depend on the order
+}
+// -> scale (a power of two) in scales[0..1] as its inverse, the form the products need.
+__device__ __forceinline__ float lx_scale(uint32_t most) {
+    int e = 13 - ((int)(most >> 23) - 127);
+    e = e > 60 ? 60 : e < -60 ? -60 : e;
+    return most ? __uint_as_float((uint32_t)(127 + e) << 23) : 1.0f;
+}
+__global__ void lx_scales_kernel(float *scales, const uint32_t *most) { if (threadIdx.x < 2) scales[threadIdx.x] = 1.0f / lx_scale(most[threadIdx.x]); }
+
+// x of tokens [t0, t0 + tokens) -> [token][ldx] 16-bit rows, zeros for tokens without a target; fp32 scaled, as two parts.
 template <typename T, typename H>
-__global__ void __launch_bounds__(256) lx_pack_x_kernel(H *hi, H *lo, const T *__restrict__ x, const void *__restrict__ targets, int id_u16, int V, int t0, int tokens,
-                                                        int D, int S, size_t ldx) {
+__global__ void __launch_bounds__(256) lx_pack_x_kernel(H *hi, H *lo, const T *__restrict__ x, const uint32_t *most, const void *__restrict__ targets, int id_u16, int V, int t0,
+                                                        int tokens, int D, int S, size_t ldx) {
     __shared__ float tile[32][33];
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
     const int t = blockIdx.x * 32 + tx, d0 = blockIdx.y * 32;
     const bool live = t < tokens && lx_target(targets, id_u16, V, t0 + t) >= 0;
     const int b = (t0 + t) / S, s = (t0 + t) % S;
+    const float scale = most ? lx_scale(*most) : 1.0f;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const int d = d0 + ty + 8 * i;
-        tile[ty + 8 * i][tx] = live && d < D ? Elt<T>::to_f(x[((size_t)b * D + d) * S + s]) : 0.0f;
+        tile[ty + 8 * i][tx] = live && d < D ? Elt<T>::to_f(x[((size_t)b * D + d) * S + s]) * scale : 0.0f;
     }
     __syncthreads();
     const int d = d0 + tx;
@@ -403,12 +473,13 @@ __global__ void __launch_bounds__(256) lx_pack_x_kernel(H *hi, H *lo, const T *_
     }
 }
 
-// Rows of the table -> [row][lde] 16-bit rows with aligned ends; fp32 as two bf16 parts.
+// Rows of the table -> [row][lde] 16-bit rows with aligned ends; fp32 scaled, as two parts.
 template <typename T, typename H>
-__global__ void __launch_bounds__(256) lx_pack_rows_kernel(H *hi, H *lo, const T *__restrict__ src, int rows, int D, size_t lde) {
+__global__ void __launch_bounds__(256) lx_pack_rows_kernel(H *hi, H *lo, const T *__restrict__ src, const uint32_t *most, int rows, int D, size_t lde) {
+    const float scale = most ? lx_scale(*most) : 1.0f;
     for (int r = blockIdx.x; r < rows; r += gridDim.x)
         for (int d = threadIdx.x; d < (int)lde; d += 256) {
-            const float v = d < D ? Elt<T>::to_f(src[(size_t)r * D + d]) : 0.0f;
+            const float v = d < D ? Elt<T>::to_f(src[(size_t)r * D + d]) * scale : 0.0f;
             const H h = Elt<H>::from_f(v);
             hi[(size_t)r * lde + d] = h;
             if (lo) lo[(size_t)r * lde + d] = Elt<H>::from_f(v - Elt<H>::to_f(h));
@@ -481,6 +552,9 @@ __global__ void __launch_bounds__(256) lx_loss_kernel(float *__restrict__ loss_s
     }
 }
 
+static inline int lx_div(long long a, long long b) { return (int)((a + b - 1) / b); }
+static inline int lx_pairs() { return ctx().sm_count / 2; }
+
 template <int EPI> static int lx_launch(cudaStream_t st, const LxMaps &maps, const LxArgs &a) {
     static bool ready = false;
     if (!ready) {
@@ -488,13 +562,11 @@ template <int EPI> static int lx_launch(cudaStream_t st, const LxMaps &maps, con
         ready = true;
     }
     const long long tiles = (long long)a.m_tiles * a.n_tiles * a.splits;
-    const int grid = tiles < ctx().sm_count ? (int)tiles : ctx().sm_count;
-    lx_gemm_kernel<EPI><<<grid, LX_THREADS, LX_SMEM, st>>>(maps, a);
+    const int pairs = tiles < lx_pairs() ? (int)tiles : lx_pairs();
+    lx_gemm_kernel<EPI><<<2 * pairs, LX_THREADS, LX_SMEM, st>>>(maps, a);
     ANE_LAUNCH_OK(1);
     return ANE_CUDA_OK;
 }
-
-static inline int lx_div(long long a, long long b) { return (int)((a + b - 1) / b); }
 
 // Instruction descriptor: fp32 accumulator, 16-bit operands of one type, their layouts, the tile.
 static uint32_t lx_idesc(bool half_type, bool a_mn, bool b_mn) {
@@ -513,40 +585,75 @@ struct LxCall {
     float grad_scale;
 };
 
+// Sizes of one call: tokens of a round, vocabulary tiles of a piece, shares of K for dx.
+struct LxPlan { int chunk, piece_tiles, splits; };
+
+// A round has at most 4096 tokens.  A piece has as many vocabulary tiles as fill whole waves of the SM pairs best, counted in
+// waves of K blocks over all pieces and products (with four K blocks for the start of a launch), while the two parts of dl
+// stay within 192 MiB.  dx has few tiles and a long K: where its tiles leave pairs idle, K is cut into shares.
+static LxPlan lx_plan(int T_all, int D, int V, int segs, bool dx, bool d_table, bool two_parts) {
+    LxPlan p;
+    const int rounds = lx_div(T_all, 4096), pairs = lx_pairs();
+    p.chunk = (int)round_up((size_t)lx_div(T_all, rounds), LX_BM);
+    if (p.chunk > T_all) p.chunk = T_all;
+    const int mt = lx_div(p.chunk, LX_BM), dt = lx_div(D, LX_BN), vt = lx_div(V, LX_BN);
+    const int kd = lx_div(D, LX_BK), kt = lx_div(p.chunk, LX_BK);
+    long long most = (192ll << 20) / ((long long)p.chunk * LX_BN * (two_parts ? 4 : 2));
+    if (most < 1) most = 1;
+    if (most > vt) most = vt;
+    double best = 1e300;
+    p.piece_tiles = 1; p.splits = 1;
+    for (int n = (int)most; n >= 1 && n >= (int)most / 4; n--) {
+        const int pieces = lx_div(vt, n);
+        int splits = 1;
+        if (dx) {
+            splits = pairs / (mt * dt);
+            if (splits > n) splits = n;                     // four K blocks per share at least
+            if (splits < 1) splits = 1;
+        }
+        double cost = 0.0;
+        for (int i = 0; i < 2; i++) {                       // the whole pieces and the last
+            const int tiles = i ? vt - (pieces - 1) * n : n, times = i ? 1 : pieces - 1;
+            double c = (double)lx_div((long long)mt * tiles, pairs) * segs * kd + 4;
+            if (dx) c += (double)lx_div((long long)mt * dt * splits, pairs) * lx_div((long long)segs * tiles * 4, splits) + 4;
+            if (d_table) c += (double)lx_div((long long)dt * tiles, pairs) * (segs == 3 ? 3 : 2) * kt + 4;
+            cost += c * times;
+        }
+        if (cost < best * 0.999) { best = cost; p.piece_tiles = n; p.splits = splits; }
+    }
+    return p;
+}
+
 template <typename T, typename H> static int lx_run(const LxCall &c) {
     const bool split = sizeof(T) == 4;                       // fp32 inputs as two parts
-    const ane_dtype part = c.dtype == ANE_F16 ? ANE_F16 : ANE_BF16;
+    const ane_dtype part = c.dtype == ANE_BF16 ? ANE_BF16 : ANE_F16;
     const int half_type = part == ANE_F16;
     const bool grad = c.dx || c.d_table;
     const int T_all = c.B * c.S, D = c.D, V = c.V;
     const size_t ldd = round_up((size_t)D, 8);
     const bool pack_table = split || D % 8 || !aligned16(c.table);
-    // Tokens of one round and vocabulary rows of one piece: the two parts of dl stay within 64 MiB, half of L2.
-    const int chunk = T_all < 4096 ? T_all : 4096;
-    long long piece = (16ll << 20) / round_up((size_t)chunk, 128) / 256 * 256;
-    if (piece < 1024) piece = 1024;
-    if (piece > (long long)round_up((size_t)V, 256)) piece = (long long)round_up((size_t)V, 256);
-    const int vp = (int)piece;
-    const size_t ldt = round_up((size_t)chunk, 32), ldl = (size_t)vp;
-    const int v_tiles = lx_div(V, LX_BN);
+    const bool need_lo = c.d_table || split;
     const int segs = split ? 3 : 1;
-
-    const int dx_tiles = lx_div(chunk, LX_BM) * lx_div(D, LX_BN);
-    const int dx_blocks = segs * lx_div(vp, LX_BK);
-    int splits = ctx().sm_count / dx_tiles;
-    if (splits > dx_blocks / 4) splits = dx_blocks / 4;
-    if (splits < 1) splits = 1;
+    const LxPlan plan = lx_plan(T_all, D, V, segs, c.dx != nullptr, c.d_table != nullptr, need_lo);
+    const int chunk = plan.chunk, vp = plan.piece_tiles * LX_BN < V ? plan.piece_tiles * LX_BN : V, splits = plan.splits;
+    const size_t ldt = round_up((size_t)chunk, 32), ldl = (size_t)plan.piece_tiles * LX_BN;
+    const int halves = lx_div(V, LX_COLS);
+    // A table that has to be packed is packed once where that takes up to 256 MiB, else piece by piece.
+    const size_t row_bytes = ldd * 2 * (split ? 2 : 1);
+    const int vk = !pack_table ? 0 : (size_t)V * row_bytes <= ((size_t)256 << 20) ? V : vp;
 
     size_t off = 0;
     auto take = [&](size_t bytes) { const size_t at = off; off += round_up(bytes, 1024); return at; };
-    const size_t o_tok = take(c.loss_tok ? 0 : (size_t)T_all * 4), o_lse = take(ldt * 4), o_hit = take(ldt * 4), o_part = take((size_t)v_tiles * ldt * 8);
+    const size_t o_most = take(16), o_scales = take(16);
+    const size_t o_tok = take(c.loss_tok ? 0 : (size_t)T_all * 4), o_lse = take(ldt * 4), o_hit = take(ldt * 4), o_part = take((size_t)halves * ldt * 8);
     const size_t o_xh = take((size_t)chunk * ldd * 2), o_xl = take(split ? (size_t)chunk * ldd * 2 : 0);
-    const size_t o_eh = take(pack_table ? (size_t)vp * ldd * 2 : 0), o_el = take(split ? (size_t)vp * ldd * 2 : 0);
-    const bool need_lo = c.d_table || split;
+    const size_t o_eh = take((size_t)vk * ldd * 2), o_el = take(split ? (size_t)vk * ldd * 2 : 0);
     const size_t o_lh = take(grad ? (size_t)chunk * ldl * 2 : 0), o_ll = take(grad && need_lo ? (size_t)chunk * ldl * 2 : 0);
     const size_t o_dx = take(c.dx ? (size_t)splits * D * ldt * 4 : 0);
     char *ws = static_cast<char *>(workspace(off));
     if (!ws) return fail(ANE_CUDA_ERR_NOMEM, "ane_cuda_linear_cross_entropy_dev: no scratch (%zu bytes)", off);
+    uint32_t *most = split ? reinterpret_cast<uint32_t *>(ws + o_most) : nullptr;
+    float *scales = split ? reinterpret_cast<float *>(ws + o_scales) : nullptr;
     float *loss_tok = c.loss_tok ? c.loss_tok : reinterpret_cast<float *>(ws + o_tok);
     float *lse2 = reinterpret_cast<float *>(ws + o_lse), *hit = reinterpret_cast<float *>(ws + o_hit), *dxs = reinterpret_cast<float *>(ws + o_dx);
     float2 *parts = reinterpret_cast<float2 *>(ws + o_part);
@@ -556,10 +663,50 @@ template <typename T, typename H> static int lx_run(const LxCall &c) {
     const size_t idb = c.id_u16 ? 2 : 4;
     ane_cuda_status *status = ctx().status;
 
+    if (split) {
+        ANE_CUDA_TRY(cudaMemsetAsync(most, 0, 8, c.st));
+        const size_t nx = (size_t)T_all * D, ne = (size_t)V * D;
+        auto blocks = [&](size_t n) { const size_t b = (n + 4095) / 4096; return (unsigned)(b < 1184 ? b : 1184); };
+        lx_largest_kernel<<<blocks(nx), 256, 0, c.st>>>(most, static_cast<const float *>(c.x), nx, c.targets, c.id_u16, V, D, c.S);
+        lx_largest_kernel<<<blocks(ne), 256, 0, c.st>>>(most + 1, static_cast<const float *>(c.table), ne, nullptr, 0, 0, 1, 1);
+        lx_scales_kernel<<<1, 32, 0, c.st>>>(scales, most);
+        ANE_LAUNCH_OK(3);
+    }
+    // Rows [v0, v0 + nv) of the table as 16-bit rows with `ld` elements between them; packs them where that is needed.
+    int packed = 0;                                          // rows from 0 that stay packed
+    const H *rows_hi = nullptr, *rows_lo = nullptr;
+    size_t ld = ldd;
+    auto table_rows = [&](int v0, int nv) -> int {
+        if (!pack_table) {
+            rows_hi = reinterpret_cast<const H *>(c.table) + (size_t)v0 * D;
+            ld = (size_t)D;
+            return ANE_CUDA_OK;
+        }
+        if (vk < V || packed < V) {
+            const int lo = vk < V ? v0 : 0, n = vk < V ? nv : V;
+            lx_pack_rows_kernel<T, H><<<n < 4096 ? n : 4096, 256, 0, c.st>>>(eh, el, static_cast<const T *>(c.table) + (size_t)lo * D, split ? most + 1 : nullptr, n, D, ldd);
+            ANE_LAUNCH_OK(1);
+            if (vk == V) packed = V;
+        }
+        rows_hi = vk < V ? eh : eh + (size_t)v0 * ldd;
+        rows_lo = !split ? nullptr : vk < V ? el : el + (size_t)v0 * ldd;
+        return ANE_CUDA_OK;
+    };
+    // Operand pairs, the ones with a low part first.
+    auto maps_for = [&](LxMaps &m, int n, const void *ah, const void *al, const void *bh, const void *bl, size_t arows, size_t acols, size_t lda, int abox, size_t brows,
+                        size_t bcols, size_t ldb, int bbox) -> int {
+        const void *as[3] = {al, ah, ah}, *bs[3] = {bh, bl, bh};
+        for (int i = 0; i < n; i++) {
+            if (int rc = make_matrix_map(&m.a[i], part, as[3 - n + i], arows, acols, lda, abox)) return rc;
+            if (int rc = make_matrix_map(&m.b[i], part, bs[3 - n + i], brows, bcols, ldb, bbox)) return rc;
+        }
+        return ANE_CUDA_OK;
+    };
+
     for (int t0 = 0; t0 < T_all; t0 += chunk) {
         const int n_tok = T_all - t0 < chunk ? T_all - t0 : chunk;
         const void *tg = static_cast<const char *>(c.targets) + (size_t)t0 * idb;
-        lx_pack_x_kernel<T, H><<<dim3(lx_div(n_tok, 32), lx_div(D, 32)), 256, 0, c.st>>>(xh, xl, static_cast<const T *>(c.x), c.targets, c.id_u16, V, t0, n_tok, D, c.S, ldd);
+        lx_pack_x_kernel<T, H><<<dim3(lx_div(n_tok, 32), lx_div(D, 32)), 256, 0, c.st>>>(xh, xl, static_cast<const T *>(c.x), most, c.targets, c.id_u16, V, t0, n_tok, D, c.S, ldd);
         ANE_LAUNCH_OK(1);
 
         LxArgs a = {};
@@ -567,34 +714,21 @@ template <typename T, typename H> static int lx_run(const LxCall &c) {
         a.m_tiles = lx_div(n_tok, LX_BM); a.m = n_tok;
         a.idesc = lx_idesc(half_type, false, false);
         a.targets = tg; a.id_u16 = c.id_u16; a.V = V;
+        a.scales = scales;
         a.part = parts; a.hit = hit; a.lse2 = lse2; a.ldt = ldt;
-        a.half_type = half_type; a.dscale = half_type ? 16384.0f : 1.0f;
+        a.half_type = half_type; a.dscale = half_type ? LX_HALF_SCALE : 1.0f;
         a.status = status;
-        // x (K-major) and a piece of the table (K-major), as up to three pairs
-        auto logit_maps = [&](LxMaps &m, int v0, int nv) -> int {
-            const H *src = pack_table ? eh : reinterpret_cast<const H *>(c.table) + (size_t)v0 * D;
-            const size_t ld = pack_table ? ldd : (size_t)D;
-            if (pack_table) {
-                lx_pack_rows_kernel<T, H><<<nv < 4096 ? nv : 4096, 256, 0, c.st>>>(eh, el, static_cast<const T *>(c.table) + (size_t)v0 * D, nv, D, ldd);
-                ANE_LAUNCH_OK(1);
-            }
-            const H *as[3] = {xl, xh, xh}, *bs[3] = {src, el, src};
-            for (int i = 0; i < segs; i++) {
-                if (int rc = make_matrix_map(&m.a[i], part, as[3 - segs + i], n_tok, D, ldd, LX_BM)) return rc;
-                if (int rc = make_matrix_map(&m.b[i], part, bs[3 - segs + i], nv, D, ld, LX_BN)) return rc;
-            }
-            return ANE_CUDA_OK;
-        };
-        // statistics: the whole table in one launch, or piece by piece where it has to be packed
-        const int fstep = pack_table ? vp : V;
+        // statistics: the whole table in one launch, or piece by piece where it is packed so
+        const int fstep = pack_table && vk < V ? vp : V;
         for (int v0 = 0; v0 < V; v0 += fstep) {
             const int nv = V - v0 < fstep ? V - v0 : fstep;
             LxMaps m;
-            if (int rc = logit_maps(m, v0, nv)) return rc;
-            a.n_tiles = lx_div(nv, LX_BN); a.n = nv; a.v0 = v0; a.tile0 = v0 / LX_BN;
+            if (int rc = table_rows(v0, nv)) return rc;
+            if (int rc = maps_for(m, segs, xh, xl, rows_hi, rows_lo, n_tok, D, ldd, LX_CTA_M, nv, D, ld, LX_BN / 2)) return rc;
+            a.n_tiles = lx_div(nv, LX_BN); a.n = nv; a.v0 = v0; a.tile0 = v0 / LX_COLS;
             if (int rc = lx_launch<LX_STATS>(c.st, m, a)) return rc;
         }
-        lx_join_kernel<<<lx_div(n_tok, 32), 256, 0, c.st>>>(lse2, loss_tok + t0, parts, hit, tg, c.id_u16, V, v_tiles, n_tok, ldt, status);
+        lx_join_kernel<<<lx_div(n_tok, 32), 256, 0, c.st>>>(lse2, loss_tok + t0, parts, hit, tg, c.id_u16, V, halves, n_tok, ldt, status);
         ANE_LAUNCH_OK(1);
         if (!grad) continue;
 
@@ -602,44 +736,31 @@ template <typename T, typename H> static int lx_run(const LxCall &c) {
         for (int v0 = 0; v0 < V; v0 += vp) {
             const int nv = V - v0 < vp ? V - v0 : vp;
             LxMaps m;
-            if (int rc = logit_maps(m, v0, nv)) return rc;
+            if (int rc = table_rows(v0, nv)) return rc;
+            if (int rc = maps_for(m, segs, xh, xl, rows_hi, rows_lo, n_tok, D, ldd, LX_CTA_M, nv, D, ld, LX_BN / 2)) return rc;
             a.n_tiles = lx_div(nv, LX_BN); a.n = nv; a.v0 = v0;
             a.hi = lh; a.lo = ll; a.ldl = ldl;
             if (int rc = lx_launch<LX_DLOGITS>(c.st, m, a)) return rc;
             if (c.dx) {
                 LxArgs g = a;
-                LxMaps gm;
-                const H *src = pack_table ? eh : reinterpret_cast<const H *>(c.table) + (size_t)v0 * D;
-                const void *as[3] = {ll, lh, lh};
-                const H *bs[3] = {src, el, src};
-                for (int i = 0; i < segs; i++) {
-                    if (int rc = make_matrix_map(&gm.a[i], part, as[3 - segs + i], n_tok, nv, ldl, LX_BM)) return rc;
-                    if (int rc = make_matrix_map(&gm.b[i], part, bs[3 - segs + i], nv, D, pack_table ? ldd : (size_t)D, LX_BK)) return rc;
-                }
+                if (int rc = maps_for(m, segs, lh, ll, rows_hi, rows_lo, n_tok, nv, ldl, LX_CTA_M, nv, D, ld, LX_BK)) return rc;
                 g.kblocks = lx_div(nv, LX_BK); g.splits = splits;
                 if (split) g.span = LX_SPAN;                 // a 16-bit result does not show what the accumulator cuts off
                 g.n_tiles = lx_div(D, LX_BN); g.n = D;
                 g.idesc = lx_idesc(half_type, false, true);
                 g.out = dxs; g.first = v0 == 0;
-                if (int rc = lx_launch<LX_DX>(c.st, gm, g)) return rc;
+                if (int rc = lx_launch<LX_DX>(c.st, m, g)) return rc;
             }
             if (c.d_table) {
                 LxArgs g = a;
-                LxMaps gm;
-                // dl in two parts always; fp32 x adds the product of its own low part
-                const H *as[3] = {xl, xh, xh};
-                const void *bs[3] = {lh, ll, lh};
-                g.segments = split ? 3 : 2;
-                for (int i = 0; i < g.segments; i++) {
-                    if (int rc = make_matrix_map(&gm.a[i], part, as[3 - g.segments + i], n_tok, D, ldd, LX_BK)) return rc;
-                    if (int rc = make_matrix_map(&gm.b[i], part, bs[3 - g.segments + i], n_tok, nv, ldl, LX_BK)) return rc;
-                }
+                g.segments = split ? 3 : 2;                  // dl in two parts always
+                if (int rc = maps_for(m, g.segments, xh, xl, lh, ll, n_tok, D, ldd, LX_BK, n_tok, nv, ldl, LX_BK)) return rc;
                 g.kblocks = lx_div(n_tok, LX_BK); g.span = LX_SPAN;
                 g.m_tiles = lx_div(D, LX_BM); g.m = D;
                 g.n_tiles = lx_div(nv, LX_BN); g.n = nv;
                 g.idesc = lx_idesc(half_type, true, true);
                 g.out = c.d_table + (size_t)v0 * D; g.ldt = (size_t)D; g.alpha = alpha;
-                if (int rc = lx_launch<LX_DTABLE>(c.st, gm, g)) return rc;
+                if (int rc = lx_launch<LX_DTABLE>(c.st, m, g)) return rc;
             }
         }
         if (c.dx) {
@@ -674,7 +795,7 @@ int ane_cuda_linear_cross_entropy_dev(void *stream, ane_dtype dtype, ane_idtype 
     ANE_CHECK_EXTENT(targets, (size_t)B * S * (idtype == ANE_ID_U16 ? 2 : 4));
     const LxCall c = {(cudaStream_t)stream, dtype, idtype == ANE_ID_U16, B, D, V, S, loss_seq, loss_tok, dx, d_table, x, table, targets, grad_scale};
     switch (dtype) {
-        case ANE_F32: return lx_run<float, __nv_bfloat16>(c);
+        case ANE_F32: return lx_run<float, __half>(c);
         case ANE_BF16: return lx_run<__nv_bfloat16, __nv_bfloat16>(c);
         default: return lx_run<__half, __half>(c);
     }
