@@ -24,8 +24,7 @@
 //
 // The accumulators of the tensor cores cut off what does not fit instead of rounding: every step of 16 along K takes half a
 // unit of the last place from the sum on average, 3e-8 of it (measured: 1.2e-5 after 345 steps).  So fp32 results leave the
-// accumulator after 512 elements of K, 32 steps, and are added up in registers with rounding; and the products with a low part
-// go first, while the sum is small.
+// accumulator after 32 steps and are added up in registers with rounding.
 //
 // A token without a target (id outside [0, V)) has zeros in place of its x, so that nothing it holds -- infinities and NaN
 // included -- reaches d_table.
@@ -38,25 +37,30 @@ namespace ane {
 
 constexpr float LX_LOG2E = 1.4426950408889634f;
 constexpr int LX_CTA_M = 128;                            // rows of the tile in each block of a pair
-constexpr int LX_BM = 2 * LX_CTA_M, LX_BN = 256, LX_BK = 64;      // tile of a pair: M x N outputs, K elements per stage
-constexpr int LX_STAGES = 6;
-constexpr int LX_A_BYTES = LX_CTA_M * LX_BK * 2, LX_B_BYTES = LX_BN / 2 * LX_BK * 2, LX_STAGE_BYTES = LX_A_BYTES + LX_B_BYTES;
+constexpr int LX_BM = 2 * LX_CTA_M, LX_BN = 256, LX_BK = 64;      // one accumulator: M x N outputs of a pair; K elements per stage
+constexpr int LX_BOX_BYTES = LX_CTA_M * LX_BK * 2;                // a block's 128 rows of one operand
+constexpr size_t LX_RING_BYTES = 12 * LX_BOX_BYTES;
 constexpr int LX_EPI_WARPS = 8;                          // two for each 32 accumulator lanes, half of the columns each
 constexpr int LX_COLS = LX_BN / 2;                       // columns of an epilogue warp
 constexpr int LX_THREADS = 64 + 32 * LX_EPI_WARPS;       // copy warp, matrix warp, epilogue warps
-constexpr size_t LX_SMEM = (size_t)LX_STAGES * LX_STAGE_BYTES + 1024;
-constexpr int LX_SPAN = 512 / LX_BK;                     // K blocks that stay in an accumulator where an fp32 result is wanted
+constexpr size_t LX_SMEM = LX_RING_BYTES + 1024;
+constexpr int LX_STEPS = 32;                             // of 16 along K that stay in an accumulator where an fp32 result is wanted
 constexpr int LX_WAIT_LIMIT = 1 << 20;
 constexpr float LX_HALF_SCALE = 16384.0f;                // of dl where it is held in fp16
 
 enum LxEpilogue { LX_STATS, LX_DLOGITS, LX_DX, LX_DTABLE };
+// What a stage of the ring holds and what is done with it:
+//   LX_PLAIN   A, B           one accumulator (the other one belongs to the next tile)
+//   LX_WIDE    A, B, B'       B' = the next 256 rows of the output's columns: both accumulators make one 256 x 512 tile
+//   LX_TWO     A, B, B'       B' = the low part of B: both products into one accumulator
+enum LxMode { LX_PLAIN, LX_WIDE, LX_TWO };
 
 struct LxMaps { CUtensorMap a[3], b[3]; };               // one pair per 16-bit product that is summed
 struct LxArgs {
     int segments;              // pairs in use
     int kblocks;               // K blocks of one pair
     int splits;                // shares of the K blocks, each with its own sums (dx only)
-    int span;                  // K blocks that one accumulator sums before its values move to registers (dx, d_table)
+    int span;                  // K blocks that one accumulator sums before its values move to registers
     int m_tiles, n_tiles;
     int m, n;                  // valid rows and columns of the output
     uint32_t idesc;
@@ -190,18 +194,23 @@ struct LxRange {
 };
 
 // ------------------------------------------------------------------ the product
-// Pairs of blocks on neighbouring SMs walk tiles of 256 x 256 outputs: each block holds 128 rows of A, 128 of B's 256 rows and
-// the accumulators of its own 128 output rows, and the matrix instructions of the first block read both blocks' operands.  Per
-// 16 elements of K an SM then reads 8 KB of operands from shared memory in 128 clocks, where a block on its own (128 x 256)
-// reads 12.  In each block one thread copies operand boxes into a ring of six stages; in the first block one thread issues the
-// matrix instructions into one of two accumulators; eight warps work on the accumulator that is complete.
-template <int EPI>
+// Pairs of blocks on neighbouring SMs work on accumulators of 256 x 256 outputs: each block holds 128 rows of A, 128 of B's 256
+// rows and the accumulator of its own 128 output rows, and the matrix instructions of the first block read both blocks'
+// operands.  In each block one thread copies operand boxes into a ring of stages; in the first block one thread issues the
+// matrix instructions; eight warps take the accumulators over.
+//
+// What bounds the products is the way from L2 to the SMs: with 64 bytes per SM and clock wanted by a 256 x 256 tile, the
+// tensor cores were busy 58 % of the time in all four products alike, at 8.8 TB/s of reads (8192 tokens would want 15).  So
+// the large products bring two boxes of B for each box of A (48 bytes per clock): LX_WIDE and LX_TWO.
+template <int EPI, int MODE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LX_THREADS, 1) lx_gemm_kernel(const __grid_constant__ LxMaps maps, const __grid_constant__ LxArgs a) {
     constexpr bool A_MN = EPI == LX_DTABLE, B_MN = EPI == LX_DX || EPI == LX_DTABLE;
+    constexpr int BOXES = MODE == LX_PLAIN ? 2 : 3, STAGES = 12 / BOXES, STAGE_BYTES = BOXES * LX_BOX_BYTES;
+    constexpr int ACCS = MODE == LX_WIDE ? 2 : 1, TILE_N = ACCS * LX_BN;
     extern __shared__ uint8_t raw[];
     const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;       // the same offset in both blocks
     // full and acc_empty are used in the first block only; the others are each block's own
-    __shared__ uint64_t full[LX_STAGES], empty[LX_STAGES], acc_full[2], acc_empty[2], drained;
+    __shared__ uint64_t full[STAGES], empty[STAGES], acc_full[2], acc_empty[2], drained;
     __shared__ uint32_t tmem_at;
     __shared__ int give_up;
     volatile int *abort = &give_up;
@@ -209,7 +218,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LX_THREADS, 1) lx_ge
     const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
     const int rank = blockIdx.x & 1, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < LX_STAGES; i++) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
+        for (int i = 0; i < STAGES; i++) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
         for (int i = 0; i < 2; i++) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], 2 * LX_EPI_WARPS); }
         mbar_init(&drained, 1);
         give_up = 0;
@@ -232,24 +241,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LX_THREADS, 1) lx_ge
         if (lane == 0) {
             for (int tile = pair; tile < tiles && !*abort; tile += pairs) {
                 const int mt = tile % a.m_tiles, nt = tile / a.m_tiles % a.n_tiles;
-                const int am = mt * LX_BM + rank * LX_CTA_M, bn = nt * LX_BN + rank * (LX_BN / 2);
+                const int am = mt * LX_BM + rank * LX_CTA_M, bn = nt * TILE_N + rank * (LX_BN / 2);
                 for (LxRange r(a, tile); !r.done(); r.next(), issued++) {
-                    const int st = issued % LX_STAGES;
-                    if (!lx_wait(&empty[st], ((issued / LX_STAGES) & 1) ^ 1, abort)) break;
-                    const int seg = r.seg, k = r.k * LX_BK;
-                    const uint32_t sa = base + st * LX_STAGE_BYTES, sb = sa + LX_A_BYTES, bar = lx_in_leader(&full[st]);
-                    if (rank == 0) mbar_arrive_expect_tx(&full[st], 2 * LX_STAGE_BYTES);
+                    const int st = issued % STAGES;
+                    if (!lx_wait(&empty[st], ((issued / STAGES) & 1) ^ 1, abort)) break;
+                    const int k = r.k * LX_BK;
+                    const uint32_t sa = base + st * STAGE_BYTES, bar = lx_in_leader(&full[st]);
+                    if (rank == 0) mbar_arrive_expect_tx(&full[st], 2 * STAGE_BYTES);
                     if constexpr (A_MN) {
 #pragma unroll
-                        for (int i = 0; i < LX_CTA_M / 64; i++) lx_load_box(sa + i * 8192, &maps.a[seg], am + i * 64, k, bar);
+                        for (int i = 0; i < LX_CTA_M / 64; i++) lx_load_box(sa + i * 8192, &maps.a[r.seg], am + i * 64, k, bar);
                     } else {
-                        lx_load_box(sa, &maps.a[seg], k, am, bar);
+                        lx_load_box(sa, &maps.a[r.seg], k, am, bar);
                     }
-                    if constexpr (B_MN) {
 #pragma unroll
-                        for (int i = 0; i < LX_BN / 128; i++) lx_load_box(sb + i * 8192, &maps.b[seg], bn + i * 64, k, bar);
-                    } else {
-                        lx_load_box(sb, &maps.b[seg], k, bn, bar);
+                    for (int h = 0; h < BOXES - 1; h++) {
+                        const CUtensorMap *map = &maps.b[MODE == LX_TWO ? h : r.seg];
+                        const uint32_t sb = sa + (1 + h) * LX_BOX_BYTES;
+                        const int n = bn + (MODE == LX_WIDE ? h * LX_BN : 0);
+                        if constexpr (B_MN) {
+#pragma unroll
+                            for (int i = 0; i < LX_BN / 128; i++) lx_load_box(sb + i * 8192, map, n + i * 64, k, bar);
+                        } else {
+                            lx_load_box(sb, map, k, n, bar);
+                        }
                     }
                 }
             }
@@ -258,27 +273,58 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LX_THREADS, 1) lx_ge
         if (lane == 0 && rank == 0) {
             uint32_t used = 0, turn = 0;
             bool ok = true;
-            for (int tile = pair; tile < tiles && ok; tile += pairs) {
-                LxRange r(a, tile);
-                uint32_t d = 0, more = 0;
-                for (; !r.done(); used++) {
-                    if (r.first()) {
-                        if (!(ok = lx_wait(&acc_empty[turn & 1], ((turn >> 1) & 1) ^ 1, abort))) break;
-                        lx_fence_after();
-                        d = tmem + (turn & 1) * LX_BN;
-                        more = 0;
-                    }
-                    const int st = used % LX_STAGES;
-                    if (!(ok = lx_wait(&full[st], (used / LX_STAGES) & 1, abort))) break;
-                    lx_fence_after();
-                    const uint32_t sa = base + st * LX_STAGE_BYTES, sb = sa + LX_A_BYTES;
+            // one stage's product with its box `box` of B into accumulator `acc`
+            auto product = [&](uint32_t stage, int box, uint32_t acc, uint32_t more) {
+                const uint32_t sa = base + stage % STAGES * STAGE_BYTES, sb = sa + box * LX_BOX_BYTES;
 #pragma unroll
-                    for (int i = 0; i < LX_BK / 16; i++)
-                        lx_mma(d, lx_desc(sa + i * (A_MN ? 2048 : 32), A_MN ? 8192 : 16), lx_desc(sb + i * (B_MN ? 2048 : 32), B_MN ? 8192 : 16), a.idesc, more | i);
-                    more = 1;
-                    lx_commit(&empty[st]);
-                    r.next();
-                    if (r.first()) { lx_commit(&acc_full[turn & 1]); turn++; }      // the accumulator is complete
+                for (int i = 0; i < LX_BK / 16; i++)
+                    lx_mma(tmem + acc * LX_BN, lx_desc(sa + i * (A_MN ? 2048 : 32), A_MN ? 8192 : 16), lx_desc(sb + i * (B_MN ? 2048 : 32), B_MN ? 8192 : 16), a.idesc, more | i);
+            };
+            for (int tile = pair; tile < tiles && ok; tile += pairs) {
+                if constexpr (MODE == LX_WIDE) {
+                    // Both accumulators share every box of A.  They are taken over one after the other, so the first one runs ahead:
+                    // by three K blocks at the beginning of a tile, where the second is still being read, and by two at the end.
+                    const LxRange r(a, tile);
+                    const int n = r.k1 - r.k0;
+                    for (int i = 0; i < n && ok;) {
+                        const int left = n - i, group = i == 0 ? (left < 3 ? left : 3) : left == 2 ? 2 : 1;
+                        for (int h = 0; h < 2 && ok; h++) {
+                            if (i == 0) {
+                                if (!(ok = lx_wait(&acc_empty[h], ((turn >> 1) & 1) ^ 1, abort))) break;
+                                lx_fence_after();
+                            }
+                            for (int j = 0; j < group; j++) {
+                                if (h == 0) {
+                                    if (!(ok = lx_wait(&full[(used + j) % STAGES], ((used + j) / STAGES) & 1, abort))) break;
+                                    lx_fence_after();
+                                }
+                                product(used + j, 1 + h, h, i + j > 0);
+                                if (h == 1) lx_commit(&empty[(used + j) % STAGES]);
+                            }
+                            if (ok && i + group == n) lx_commit(&acc_full[h]);
+                        }
+                        i += group;
+                        used += group;
+                    }
+                    if (n > 0) turn += 2;
+                } else {
+                    LxRange r(a, tile);
+                    uint32_t more = 0;
+                    for (; !r.done(); used++) {
+                        if (r.first()) {
+                            if (!(ok = lx_wait(&acc_empty[turn & 1], ((turn >> 1) & 1) ^ 1, abort))) break;
+                            lx_fence_after();
+                            more = 0;
+                        }
+                        if (!(ok = lx_wait(&full[used % STAGES], (used / STAGES) & 1, abort))) break;
+                        lx_fence_after();
+                        if (MODE == LX_TWO) { product(used, 2, turn & 1, more); more = 1; }
+                        product(used, 1, turn & 1, more);
+                        more = 1;
+                        lx_commit(&empty[used % STAGES]);
+                        r.next();
+                        if (r.first()) { lx_commit(&acc_full[turn & 1]); turn++; }      // the accumulator is complete
+                    }
                 }
             }
             lx_commit(&drained);                            // also after a give-up: no instruction or arrival outlives the block
@@ -292,118 +338,101 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LX_THREADS, 1) lx_ge
         const float unscale = a.scales ? (EPI == LX_DTABLE ? a.scales[0] : EPI == LX_DX ? a.scales[1] : a.scales[0] * a.scales[1]) : 1.0f;
         for (int tile = pair; tile < tiles && ok; tile += pairs) {
             const int mt = tile % a.m_tiles, nt = tile / a.m_tiles % a.n_tiles, ks = tile / (a.m_tiles * a.n_tiles);
-            const int m = mt * LX_BM + rank * LX_CTA_M + row, n0 = nt * LX_BN + c0;
-            const int left = a.n - n0, cols = left < 0 ? 0 : left < LX_COLS ? left : LX_COLS;     // of this warp
+            const int m = mt * LX_BM + rank * LX_CTA_M + row;
             const bool live = m < a.m;
-            // Waits for the accumulator of the next part and gives it back.
-            auto take = [&]() {
-                ok = __all_sync(0xffffffffu, lx_wait(&acc_full[turn & 1], (turn >> 1) & 1, abort));
-                lx_fence_after();
-                return tmem + (turn & 1) * LX_BN + c0 + ((uint32_t)(quad * 32) << 16);
-            };
-            auto give = [&]() {
-                lx_fence_before();
-                __syncwarp();
-                if (lane == 0) lx_arrive_at(lx_in_leader(&acc_empty[turn & 1]));
-                turn++;
-            };
-            if constexpr (EPI == LX_STATS) {
-                const uint32_t t = take();
-                if (!ok) break;
-                const int tgt = live ? lx_target(a.targets, a.id_u16, a.V, m) - a.v0 - n0 : -1;     // column of this warp
-                const float k2 = unscale * LX_LOG2E;
-                float mx = -INFINITY, sum = 0.0f;
-                for (int c = 0; c < cols; c += 32) {
-                    float v[32];
-                    lx_tmem_load(t + c, v);
-                    if (__any_sync(0xffffffffu, tgt >= c && tgt < c + 32)) {
-                        float h = 0.0f;
+            const LxRange range(a, tile);
+            const bool none = range.k0 >= range.k1;          // a share without K blocks
+            int id = -1;
+            float lse2 = 0.0f;
+            if constexpr (EPI == LX_STATS || EPI == LX_DLOGITS) id = live ? lx_target(a.targets, a.id_u16, a.V, m) : -1;
+            if constexpr (EPI == LX_DLOGITS) lse2 = live ? a.lse2[m] : 0.0f;
+            for (int h = 0; h < ACCS && ok; h++) {
+                const int n0 = nt * TILE_N + h * LX_BN + c0;
+                const int left = a.n - n0, cols = left < 0 ? 0 : left < LX_COLS ? left : LX_COLS;     // of this warp
+                // This warp's 128 columns into registers; the accumulator is free again before anything is computed.
+                float v[LX_COLS];
+                if constexpr (EPI == LX_DX || EPI == LX_DTABLE) {
 #pragma unroll
-                        for (int j = 0; j < 32; j++) h = tgt == c + j ? v[j] : h;
-                        if (tgt >= c && tgt < c + 32) a.hit[m] = h * unscale;
-                    }
-                    if (c + 32 > cols) {
-#pragma unroll
-                        for (int j = 0; j < 32; j++) if (c + j >= cols) v[j] = -INFINITY;
-                    }
-                    float top = v[0];
-#pragma unroll
-                    for (int j = 1; j < 32; j++) top = fmaxf(top, v[j]);
-                    const float mnew = fmaxf(mx, top * k2);
-                    float part = 0.0f;
-#pragma unroll
-                    for (int j = 0; j < 32; j++) part += lx_exp2(fmaf(v[j], k2, -mnew));
-                    sum = fmaf(sum, lx_exp2(mx - mnew), part);
-                    mx = mnew;
+                    for (int j = 0; j < LX_COLS; j++) v[j] = 0.0f;
                 }
-                if (live && cols > 0) a.part[(size_t)(a.tile0 + 2 * nt + (c0 != 0)) * a.ldt + m] = make_float2(mx, sum);
-                give();
-            } else if constexpr (EPI == LX_DLOGITS) {
-                const uint32_t t = take();
-                if (!ok) break;
-                const int id = live ? lx_target(a.targets, a.id_u16, a.V, m) : -1;
-                const int tgt = id >= 0 ? id - a.v0 - n0 : -1;
-                const float lse2 = live ? a.lse2[m] : 0.0f;
-                const float k2 = unscale * LX_LOG2E;
-                const size_t at = (size_t)m * a.ldl + n0;
-                for (int c = 0; c < LX_COLS; c += 32) {
-                    float v[32];
-                    lx_tmem_load(t + c, v);
-#pragma unroll
-                    for (int j = 0; j < 32; j++) v[j] = lx_exp2(fmaf(v[j], k2, -lse2)) * a.dscale;
-                    if (__any_sync(0xffffffffu, tgt >= c && tgt < c + 32)) {
-#pragma unroll
-                        for (int j = 0; j < 32; j++) v[j] = tgt == c + j ? v[j] - a.dscale : v[j];
-                    }
-                    if (c + 32 > cols) {
-#pragma unroll
-                        for (int j = 0; j < 32; j++) if (c + j >= cols) v[j] = 0.0f;
-                    }
-                    if (id < 0) {                         // a masked token: zeros, whatever its logits are
-#pragma unroll
-                        for (int j = 0; j < 32; j++) v[j] = 0.0f;
-                    }
-                    if (live) {
-#pragma unroll
-                        for (int h = 0; h < 2; h++) {
-                            uint32_t hi[8], lo[8];
-#pragma unroll
-                            for (int j = 0; j < 8; j++) lx_split2(v[h * 16 + 2 * j], v[h * 16 + 2 * j + 1], a.half_type, hi[j], lo[j]);
-                            lx_store32(static_cast<uint16_t *>(a.hi) + at + c + h * 16, hi);
-                            if (a.lo) lx_store32(static_cast<uint16_t *>(a.lo) + at + c + h * 16, lo);
-                        }
-                    }
-                }
-                give();
-            } else {
-                // dx: rows are tokens, columns are channels; d_table: rows are channels, columns vocabulary rows.  Either way the
-                // 32 lanes of a warp hold 32 neighbours of a contiguous row.  Parts of K are added up in registers.
-                float sum[LX_COLS];
-#pragma unroll
-                for (int j = 0; j < LX_COLS; j++) sum[j] = 0.0f;
-                const LxRange range(a, tile);
-                for (int part = range.k0; part < range.k1; part += a.span) {
-                    const uint32_t t = take();
+                for (int part = range.k0; part < range.k1; part += a.span, turn++) {
+                    ok = __all_sync(0xffffffffu, lx_wait(&acc_full[turn & 1], (turn >> 1) & 1, abort));
                     if (!ok) break;
+                    lx_fence_after();
+                    const uint32_t t = tmem + (turn & 1) * LX_BN + c0 + ((uint32_t)(quad * 32) << 16);
 #pragma unroll
                     for (int c = 0; c < LX_COLS; c += 32) {
-                        float v[32];
-                        lx_tmem_load(t + c, v);
+                        float w[32];
+                        lx_tmem_load(t + c, w);
 #pragma unroll
-                        for (int j = 0; j < 32; j++) sum[c + j] += v[j];
+                        for (int j = 0; j < 32; j++) {
+                            if constexpr (EPI == LX_DX || EPI == LX_DTABLE) v[c + j] += w[j];
+                            else v[c + j] = w[j];
+                        }
                     }
-                    give();
+                    lx_fence_before();
+                    __syncwarp();
+                    if (lane == 0) lx_arrive_at(lx_in_leader(&acc_empty[turn & 1]));
                 }
                 if (!ok) break;
-                if (live) {
+                if constexpr (EPI == LX_STATS) {
+                    const int tgt = id >= 0 ? id - a.v0 - n0 : -1;     // column of this warp
+                    const float k2 = unscale * LX_LOG2E;
+                    if (__any_sync(0xffffffffu, tgt >= 0 && tgt < LX_COLS)) {
+                        float hit = 0.0f;
+#pragma unroll
+                        for (int j = 0; j < LX_COLS; j++) hit = tgt == j ? v[j] : hit;
+                        if (tgt >= 0 && tgt < LX_COLS) a.hit[m] = hit * unscale;
+                    }
+                    if (cols < LX_COLS) {
+#pragma unroll
+                        for (int j = 0; j < LX_COLS; j++) if (j >= cols) v[j] = -INFINITY;
+                    }
+                    float top[4] = {v[0], v[1], v[2], v[3]}, sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int j = 4; j < LX_COLS; j++) top[j & 3] = fmaxf(top[j & 3], v[j]);
+                    const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * k2;
+#pragma unroll
+                    for (int j = 0; j < LX_COLS; j++) sum[j & 3] += lx_exp2(fmaf(v[j], k2, -mx));
+                    if (live && cols > 0) a.part[(size_t)(a.tile0 + (n0 / LX_COLS)) * a.ldt + m] = make_float2(mx, (sum[0] + sum[1]) + (sum[2] + sum[3]));
+                } else if constexpr (EPI == LX_DLOGITS) {
+                    const int tgt = id >= 0 ? id - a.v0 - n0 : -1;
+                    const float k2 = unscale * LX_LOG2E;
+                    const size_t at = (size_t)m * a.ldl + n0;
+                    const bool mine = __any_sync(0xffffffffu, tgt >= 0 && tgt < LX_COLS);
+                    if ((size_t)n0 < a.ldl) {             // the last 256 columns of a wide tile may lie outside the piece
+#pragma unroll
+                        for (int c = 0; c < LX_COLS; c += 16) {
+                            uint32_t hi[8], lo[8];
+                            float e[16];
+#pragma unroll
+                            for (int j = 0; j < 16; j++) e[j] = lx_exp2(fmaf(v[c + j], k2, -lse2)) * a.dscale;
+                            if (mine) {
+#pragma unroll
+                                for (int j = 0; j < 16; j++) e[j] = tgt == c + j ? e[j] - a.dscale : e[j];
+                            }
+                            // a masked token: zeros, whatever its logits are; so are the columns behind the last
+#pragma unroll
+                            for (int j = 0; j < 16; j++) if (id < 0 || c + j >= cols) e[j] = 0.0f;
+#pragma unroll
+                            for (int j = 0; j < 8; j++) lx_split2(e[2 * j], e[2 * j + 1], a.half_type, hi[j], lo[j]);
+                            if (live) {
+                                lx_store32(static_cast<uint16_t *>(a.hi) + at + c, hi);
+                                if (a.lo) lx_store32(static_cast<uint16_t *>(a.lo) + at + c, lo);
+                            }
+                        }
+                    }
+                } else if (live) {
+                    // dx: rows are tokens, columns are channels; d_table: rows are channels, columns vocabulary rows.  Either way
+                    // the 32 lanes of a warp hold 32 neighbours of a contiguous row.
                     float *out = a.out + ((size_t)(EPI == LX_DX ? ks : 0) * a.n + n0) * a.ldt + m;
                     const float k = EPI == LX_DTABLE ? a.alpha * unscale : unscale;
                     if (EPI == LX_DX && a.first) {
 #pragma unroll
-                        for (int j = 0; j < LX_COLS; j++) if (j < cols) out[(size_t)j * a.ldt] = sum[j] * k;
-                    } else if (range.k0 < range.k1) {
+                        for (int j = 0; j < LX_COLS; j++) if (j < cols) out[(size_t)j * a.ldt] = v[j] * k;
+                    } else if (!none) {
 #pragma unroll
-                        for (int j = 0; j < LX_COLS; j++) if (j < cols) lx_add(out + (size_t)j * a.ldt, sum[j] * k);
+                        for (int j = 0; j < LX_COLS; j++) if (j < cols) lx_add(out + (size_t)j * a.ldt, v[j] * k);
                     }
                 }
             }
@@ -415,7 +444,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LX_THREADS, 1) lx_ge
     if (*abort && threadIdx.x == 0) {
         // copies still on their way into shared memory: every stage's last one, counted in the first block
         if (rank == 0)
-            for (uint32_t i = issued > LX_STAGES ? issued - LX_STAGES : 0; i < issued; i++) mbar_wait_bounded(&full[i % LX_STAGES], (i / LX_STAGES) & 1);
+            for (uint32_t i = issued > STAGES ? issued - STAGES : 0; i < issued; i++) mbar_wait_bounded(&full[i % STAGES], (i / STAGES) & 1);
         atomicAdd(&a.status->wait_giveups, 1);
     }
     __syncthreads();
@@ -555,17 +584,35 @@ __global__ void __launch_bounds__(256) lx_loss_kernel(float *__restrict__ loss_s
 static inline int lx_div(long long a, long long b) { return (int)((a + b - 1) / b); }
 static inline int lx_pairs() { return ctx().sm_count / 2; }
 
-template <int EPI> static int lx_launch(cudaStream_t st, const LxMaps &maps, const LxArgs &a) {
+template <int EPI, int MODE> static int lx_start(cudaStream_t st, const LxMaps &maps, const LxArgs &a) {
     static bool ready = false;
     if (!ready) {
-        ANE_CUDA_TRY(cudaFuncSetAttribute(lx_gemm_kernel<EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)LX_SMEM));
+        ANE_CUDA_TRY(cudaFuncSetAttribute(lx_gemm_kernel<EPI, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)LX_SMEM));
         ready = true;
     }
     const long long tiles = (long long)a.m_tiles * a.n_tiles * a.splits;
     const int pairs = tiles < lx_pairs() ? (int)tiles : lx_pairs();
-    lx_gemm_kernel<EPI><<<2 * pairs, LX_THREADS, LX_SMEM, st>>>(maps, a);
+    lx_gemm_kernel<EPI, MODE><<<2 * pairs, LX_THREADS, LX_SMEM, st>>>(maps, a);
     ANE_LAUNCH_OK(1);
     return ANE_CUDA_OK;
+}
+
+// Time of a product of `tiles` accumulators of 256 x 256 (m x n of them), in K blocks of one accumulator: waves over the SM
+// pairs.  A wide tile takes the time of 1.55 plain ones.
+constexpr double LX_WIDE_COST = 1.55;
+static double lx_cost(int m, int n, int splits, bool can_be_wide, bool *wide) {
+    const double plain = lx_div((long long)m * n * splits, lx_pairs()), w = lx_div((long long)m * lx_div(n, 2) * splits, lx_pairs()) * LX_WIDE_COST;
+    const bool is = can_be_wide && w < plain;
+    if (wide) *wide = is;
+    return is ? w : plain;
+}
+// n_tiles of `a` counts accumulators; one operand pair may run wide.
+template <int EPI> static int lx_launch(cudaStream_t st, const LxMaps &maps, LxArgs a) {
+    bool wide = false;
+    lx_cost(a.m_tiles, a.n_tiles, a.splits, a.segments == 1, &wide);
+    if (!wide) return lx_start<EPI, LX_PLAIN>(st, maps, a);
+    a.n_tiles = lx_div(a.n_tiles, 2);
+    return lx_start<EPI, LX_WIDE>(st, maps, a);
 }
 
 // Instruction descriptor: fp32 accumulator, 16-bit operands of one type, their layouts, the tile.
@@ -614,9 +661,9 @@ static LxPlan lx_plan(int T_all, int D, int V, int segs, bool dx, bool d_table, 
         double cost = 0.0;
         for (int i = 0; i < 2; i++) {                       // the whole pieces and the last
             const int tiles = i ? vt - (pieces - 1) * n : n, times = i ? 1 : pieces - 1;
-            double c = (double)lx_div((long long)mt * tiles, pairs) * segs * kd + 4;
-            if (dx) c += (double)lx_div((long long)mt * dt * splits, pairs) * lx_div((long long)segs * tiles * 4, splits) + 4;
-            if (d_table) c += (double)lx_div((long long)dt * tiles, pairs) * (segs == 3 ? 3 : 2) * kt + 4;
+            double c = lx_cost(mt, tiles, 1, segs == 1, nullptr) * segs * kd + 4;
+            if (dx) c += lx_cost(mt, dt, splits, segs == 1, nullptr) * lx_div((long long)segs * tiles * 4, splits) + 4;
+            if (d_table) c += (double)lx_div((long long)dt * tiles, pairs) * (segs == 3 ? 3 : LX_WIDE_COST) * kt + 4;
             cost += c * times;
         }
         if (cost < best * 0.999) { best = cost; p.piece_tiles = n; p.splits = splits; }
@@ -745,7 +792,7 @@ template <typename T, typename H> static int lx_run(const LxCall &c) {
                 LxArgs g = a;
                 if (int rc = maps_for(m, segs, lh, ll, rows_hi, rows_lo, n_tok, nv, ldl, LX_CTA_M, nv, D, ld, LX_BK)) return rc;
                 g.kblocks = lx_div(nv, LX_BK); g.splits = splits;
-                if (split) g.span = LX_SPAN;                 // a 16-bit result does not show what the accumulator cuts off
+                if (split) g.span = LX_STEPS * 16 / LX_BK;   // a 16-bit result does not show what the accumulator cuts off
                 g.n_tiles = lx_div(D, LX_BN); g.n = D;
                 g.idesc = lx_idesc(half_type, false, true);
                 g.out = dxs; g.first = v0 == 0;
@@ -753,14 +800,20 @@ template <typename T, typename H> static int lx_run(const LxCall &c) {
             }
             if (c.d_table) {
                 LxArgs g = a;
-                g.segments = split ? 3 : 2;                  // dl in two parts always
-                if (int rc = maps_for(m, g.segments, xh, xl, lh, ll, n_tok, D, ldd, LX_BK, n_tok, nv, ldl, LX_BK)) return rc;
-                g.kblocks = lx_div(n_tok, LX_BK); g.span = LX_SPAN;
+                if (split) {
+                    if (int rc = maps_for(m, 3, xh, xl, lh, ll, n_tok, D, ldd, LX_BK, n_tok, nv, ldl, LX_BK)) return rc;
+                    g.span = LX_STEPS * 16 / LX_BK;
+                } else {                                     // both parts of dl beside one box of x: two steps for every 16 of K
+                    if (int rc = maps_for(m, 1, xh, nullptr, lh, nullptr, n_tok, D, ldd, LX_BK, n_tok, nv, ldl, LX_BK)) return rc;
+                    if (int rc = make_matrix_map(&m.b[1], part, ll, n_tok, nv, ldl, LX_BK)) return rc;
+                    g.span = LX_STEPS / 2 * 16 / LX_BK;
+                }
+                g.kblocks = lx_div(n_tok, LX_BK);
                 g.m_tiles = lx_div(D, LX_BM); g.m = D;
                 g.n_tiles = lx_div(nv, LX_BN); g.n = nv;
                 g.idesc = lx_idesc(half_type, true, true);
                 g.out = c.d_table + (size_t)v0 * D; g.ldt = (size_t)D; g.alpha = alpha;
-                if (int rc = lx_launch<LX_DTABLE>(c.st, m, g)) return rc;
+                if (int rc = split ? lx_start<LX_DTABLE, LX_PLAIN>(c.st, m, g) : lx_start<LX_DTABLE, LX_TWO>(c.st, m, g)) return rc;
             }
         }
         if (c.dx) {
