@@ -98,7 +98,7 @@ static inline void launch_dep(int cls, void (*kernel)(KArgs...), dim3 grid, dim3
     cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);      // the error, if any, is picked up by ANE_LAUNCH_OK
 }
 
-static inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+static __host__ __device__ inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 static inline size_t dtype_size(ane_dtype d) { return d == ANE_F32 ? 4 : 2; }
 static inline bool dtype_ok(ane_dtype d) { return d == ANE_F32 || d == ANE_BF16 || d == ANE_F16; }
 static inline size_t round_up(size_t x, size_t a) { return (x + a - 1) / a * a; }

@@ -36,17 +36,6 @@
 namespace ane {
 
 constexpr float LX_LOG2E = 1.4426950408889634f;
-constexpr int LX_CTA_M = 128;                            // rows of the tile in each block of a pair
-constexpr int LX_BM = 2 * LX_CTA_M, LX_BN = 256, LX_BK = 64;      // one accumulator: M x N outputs of a pair; K elements per stage
-constexpr int LX_BOX_BYTES = LX_CTA_M * LX_BK * 2;                // a block's 128 rows of one operand
-constexpr size_t LX_RING_BYTES = 12 * LX_BOX_BYTES;
-constexpr int LX_EPI_WARPS = 8;                          // two for each 32 accumulator lanes, half of the columns each
-constexpr int LX_COLS = LX_BN / 2;                       // columns of an epilogue warp
-constexpr int LX_THREADS = 64 + 32 * LX_EPI_WARPS;       // copy warp, matrix warp, epilogue warps
-constexpr size_t LX_SMEM = LX_RING_BYTES + 1024;
-constexpr int LX_STEPS = 32;                             // of 16 along K that stay in an accumulator where an fp32 result is wanted
-constexpr int LX_WAIT_LIMIT = 1 << 20;
-constexpr float LX_HALF_SCALE = 16384.0f;                // of dl where it is held in fp16
 
 enum LxEpilogue { LX_STATS, LX_DLOGITS, LX_DX, LX_DTABLE };
 // What a stage of the ring holds and what is done with it:
@@ -55,7 +44,23 @@ enum LxEpilogue { LX_STATS, LX_DLOGITS, LX_DX, LX_DTABLE };
 //   LX_TWO     A, B, B'       B' = the low part of B: both products into one accumulator
 enum LxMode { LX_PLAIN, LX_WIDE, LX_TWO };
 
-struct LxMaps { CUtensorMap a[3], b[3]; };               // one pair per 16-bit product that is summed
+constexpr int LX_CTA_M = 128;                            // rows of the tile in each block of a pair
+constexpr int LX_BM = 2 * LX_CTA_M, LX_BN = 256, LX_BK = 64;      // one accumulator: M x N outputs of a pair; K elements per stage
+constexpr int LX_BOX_BYTES = LX_CTA_M * LX_BK * 2;                // a block's 128 rows of one operand
+constexpr int LX_EPI_WARPS = 8;                          // two for each 32 accumulator lanes, half of the columns each
+constexpr int LX_COLS = LX_BN / 2;                       // columns of an epilogue warp
+constexpr int LX_THREADS = 64 + 32 * LX_EPI_WARPS;       // copy warp, matrix warp, epilogue warps
+constexpr int LX_STAGING_BYTES = 2 * 32 * 128;           // dlogits: an epilogue warp's 32 rows x 64 columns of both parts
+// Boxes in the ring of operands; the staging of dlogits takes part of it.
+constexpr int lx_ring_boxes(int epi, int mode) { return epi != LX_DLOGITS ? 12 : mode == LX_PLAIN ? 8 : 9; }
+constexpr size_t lx_smem(int epi, int mode) {
+    return (size_t)lx_ring_boxes(epi, mode) * LX_BOX_BYTES + (epi == LX_DLOGITS ? LX_EPI_WARPS * LX_STAGING_BYTES : 0) + 1024;
+}
+constexpr int LX_STEPS = 32;                             // of 16 along K that stay in an accumulator where an fp32 result is wanted
+constexpr int LX_WAIT_LIMIT = 1 << 20;
+constexpr float LX_HALF_SCALE = 16384.0f;                // of dl where it is held in fp16
+
+struct LxMaps { CUtensorMap a[3], b[3], hi, lo; };       // one pair per 16-bit product that is summed; dlogits: where dl goes
 struct LxArgs {
     int segments;              // pairs in use
     int kblocks;               // K blocks of one pair
@@ -71,7 +76,7 @@ struct LxArgs {
     float2 *part; int tile0;   // stats: [half vocabulary tile][ldt], this piece's first
     float *hit;                // stats: the target's logit per token
     const float *lse2;         // dlogits: lse * log2(e)
-    void *hi, *lo; size_t ldl; // dlogits: [token][ldl], lo may be null
+    int two_parts;             // dlogits: the low parts are wanted
     float dscale;
     // dx: [split][column][ldt] sums; d_table: [column][D]
     float *out; size_t ldt; int first;
@@ -164,11 +169,17 @@ __device__ __forceinline__ void lx_split2(float a, float b, int half_type, uint3
         lo = *reinterpret_cast<const uint32_t *>(&l);
     }
 }
-// 32 bytes at once: every sector of a row is written whole, although neighbouring lanes hold different rows.
-__device__ __forceinline__ void lx_store32(void *p, const uint32_t (&w)[8]) {
-    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
-                 ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
+__device__ __forceinline__ void lx_store_shared(uint32_t at, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
+// A box out of shared memory, columns and rows outside the matrix left out.
+__device__ __forceinline__ void lx_store_box(const CUtensorMap *map, uint32_t src, int x, int y) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];"
+                 ::"l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(src) : "memory");
+}
+__device__ __forceinline__ void lx_store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void lx_store_read_wait() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void lx_store_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
 // The K blocks of one tile: the tile's share [k0, k1), in parts of `span`; within a part every operand pair in turn.
 struct LxRange {
@@ -205,7 +216,7 @@ struct LxRange {
 template <int EPI, int MODE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LX_THREADS, 1) lx_gemm_kernel(const __grid_constant__ LxMaps maps, const __grid_constant__ LxArgs a) {
     constexpr bool A_MN = EPI == LX_DTABLE, B_MN = EPI == LX_DX || EPI == LX_DTABLE;
-    constexpr int BOXES = MODE == LX_PLAIN ? 2 : 3, STAGES = 12 / BOXES, STAGE_BYTES = BOXES * LX_BOX_BYTES;
+    constexpr int BOXES = MODE == LX_PLAIN ? 2 : 3, STAGES = lx_ring_boxes(EPI, MODE) / BOXES, STAGE_BYTES = BOXES * LX_BOX_BYTES;
     constexpr int ACCS = MODE == LX_WIDE ? 2 : 1, TILE_N = ACCS * LX_BN;
     extern __shared__ uint8_t raw[];
     const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;       // the same offset in both blocks
@@ -283,11 +294,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LX_THREADS, 1) lx_ge
             for (int tile = pair; tile < tiles && ok; tile += pairs) {
                 if constexpr (MODE == LX_WIDE) {
                     // Both accumulators share every box of A.  They are taken over one after the other, so the first one runs ahead:
-                    // by three K blocks at the beginning of a tile, where the second is still being read, and by two at the end.
+                    // by all stages but one at the beginning of a tile, where the second is still being read, and by two K blocks at the end.
                     const LxRange r(a, tile);
                     const int n = r.k1 - r.k0;
                     for (int i = 0; i < n && ok;) {
-                        const int left = n - i, group = i == 0 ? (left < 3 ? left : 3) : left == 2 ? 2 : 1;
+                        const int left = n - i, group = i == 0 ? (left < STAGES - 1 ? left : STAGES - 1) : left == 2 ? 2 : 1;
                         for (int h = 0; h < 2 && ok; h++) {
                             if (i == 0) {
                                 if (!(ok = lx_wait(&acc_empty[h], ((turn >> 1) & 1) ^ 1, abort))) break;
@@ -398,28 +409,41 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LX_THREADS, 1) lx_ge
                 } else if constexpr (EPI == LX_DLOGITS) {
                     const int tgt = id >= 0 ? id - a.v0 - n0 : -1;
                     const float k2 = unscale * LX_LOG2E;
-                    const size_t at = (size_t)m * a.ldl + n0;
+                    const float shift = log2f(a.dscale) - lse2;          // a power of two: exp2 brings it in
                     const bool mine = __any_sync(0xffffffffu, tgt >= 0 && tgt < LX_COLS);
-                    if ((size_t)n0 < a.ldl) {             // the last 256 columns of a wide tile may lie outside the piece
+                    const int row0 = mt * LX_BM + rank * LX_CTA_M + quad * 32;
+                    const uint32_t stage = base + STAGES * STAGE_BYTES + (warp - 2) * LX_STAGING_BYTES;
+                    // 64 columns at a time: one 128-byte row per lane in each part, swizzled as the copy engine expects it
 #pragma unroll
-                        for (int c = 0; c < LX_COLS; c += 16) {
-                            uint32_t hi[8], lo[8];
-                            float e[16];
+                    for (int c = 0; c < LX_COLS; c += 64) {
+                        if (c >= cols || row0 >= a.m) break;
+                        if (lane == 0) lx_store_read_wait();             // the staging is free again
+                        __syncwarp();
 #pragma unroll
-                            for (int j = 0; j < 16; j++) e[j] = lx_exp2(fmaf(v[c + j], k2, -lse2)) * a.dscale;
+                        for (int q = 0; q < 8; q++) {
+                            uint32_t hi[4], lo[4];
+                            float e[8];
+#pragma unroll
+                            for (int j = 0; j < 8; j++) e[j] = lx_exp2(fmaf(v[c + q * 8 + j], k2, shift));
                             if (mine) {
 #pragma unroll
-                                for (int j = 0; j < 16; j++) e[j] = tgt == c + j ? e[j] - a.dscale : e[j];
+                                for (int j = 0; j < 8; j++) e[j] = tgt == c + q * 8 + j ? e[j] - a.dscale : e[j];
                             }
-                            // a masked token: zeros, whatever its logits are; so are the columns behind the last
 #pragma unroll
-                            for (int j = 0; j < 16; j++) if (id < 0 || c + j >= cols) e[j] = 0.0f;
-#pragma unroll
-                            for (int j = 0; j < 8; j++) lx_split2(e[2 * j], e[2 * j + 1], a.half_type, hi[j], lo[j]);
-                            if (live) {
-                                lx_store32(static_cast<uint16_t *>(a.hi) + at + c, hi);
-                                if (a.lo) lx_store32(static_cast<uint16_t *>(a.lo) + at + c, lo);
+                            for (int j = 0; j < 4; j++) {
+                                lx_split2(e[2 * j], e[2 * j + 1], a.half_type, hi[j], lo[j]);
+                                if (id < 0) hi[j] = lo[j] = 0;           // a masked token: zeros, whatever its logits are
                             }
+                            const uint32_t at = stage + lane * 128 + ((q ^ (lane & 7)) << 4);
+                            lx_store_shared(at, hi[0], hi[1], hi[2], hi[3]);
+                            if (a.two_parts) lx_store_shared(at + 4096, lo[0], lo[1], lo[2], lo[3]);
+                        }
+                        fence_proxy_async();
+                        __syncwarp();
+                        if (lane == 0) {
+                            lx_store_box(&maps.hi, stage, n0 + c, row0);
+                            if (a.two_parts) lx_store_box(&maps.lo, stage + 4096, n0 + c, row0);
+                            lx_store_commit();
                         }
                     }
                 } else if (live) {
@@ -438,6 +462,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LX_THREADS, 1) lx_ge
             }
         }
     }
+    if (EPI == LX_DLOGITS && warp >= 2 && lane == 0) lx_store_wait();
     __syncwarp();
     lx_fence_before();
     __syncthreads();
@@ -458,10 +483,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LX_THREADS, 1) lx_ge
 // at where its token has a target (S and D describe its layout; the table passes no targets).
 __global__ void __launch_bounds__(256) lx_largest_kernel(uint32_t *most, const float *__restrict__ p, size_t n, const void *__restrict__ targets, int id_u16, int V, int D, int S) {
     uint32_t top = 0;
-    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) {
-        const uint32_t u = __float_as_uint(p[i]) & 0x7fffffffu;
+    auto look = [&](float f, size_t i) {
+        const uint32_t u = __float_as_uint(f) & 0x7fffffffu;
         if (u > top && u < 0x7f800000u && (!targets || lx_target(targets, id_u16, V, (int)(i / ((size_t)D * S) * S + i % S)) >= 0)) top = u;
+    };
+    const size_t step = (size_t)gridDim.x * 256, at = (size_t)blockIdx.x * 256 + threadIdx.x, quads = aligned16(p) ? n / 4 : 0;
+    for (size_t i = at; i < quads; i += 4 * step) {
+        float4 q[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) q[u] = i + u * step < quads ? reinterpret_cast<const float4 *>(p)[i + u * step] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const size_t j = 4 * (i + u * step);
+            look(q[u].x, j); look(q[u].y, j + 1); look(q[u].z, j + 2); look(q[u].w, j + 3);
+        }
     }
+    for (size_t i = 4 * quads + at; i < n; i += step) look(p[i], i);
     top = __reduce_max_sync(0xffffffffu, top);
     if ((threadIdx.x & 31) == 0 && top) atomicMax(most, top);      // a maximum does not depend on the order
 }
@@ -515,41 +552,51 @@ __global__ void __launch_bounds__(256) lx_pack_rows_kernel(H *hi, H *lo, const T
         }
 }
 
-// (max, sum) pairs of the vocabulary tiles -> lse and loss of 32 tokens per block, tiles joined in a fixed order.
-__global__ void __launch_bounds__(256) lx_join_kernel(float *__restrict__ lse2, float *__restrict__ loss_tok, const float2 *__restrict__ part, const float *__restrict__ hit,
-                                                      const void *__restrict__ targets, int id_u16, int V, int tiles, int tokens, size_t ldt, ane_cuda_status *status) {
-    __shared__ float2 sh[8][32];
+// (max, sum) pairs of the vocabulary tiles -> lse and loss of 32 tokens per block: 32 warps with every 32nd tile each, joined
+// in a fixed order.
+__global__ void __launch_bounds__(1024) lx_join_kernel(float *__restrict__ lse2, float *__restrict__ loss_tok, const float2 *__restrict__ part, const float *__restrict__ hit,
+                                                       const void *__restrict__ targets, int id_u16, int V, int tiles, int tokens, size_t ldt, ane_cuda_status *status) {
+    __shared__ float2 sh[32][33];
     const int cl = threadIdx.x & 31, sl = threadIdx.x >> 5;
     const int t = blockIdx.x * 32 + cl;
     float m = -INFINITY, s = 0.0f;
     if (t < tokens)
-#pragma unroll 4
-        for (int i = sl; i < tiles; i += 8) {
-            const float2 p = part[(size_t)i * ldt + t];
-            const float mn = fmaxf(m, p.x);
-            s = s * lx_exp2(m - mn) + p.y * lx_exp2(p.x - mn);
+        for (int i = sl; i < tiles; i += 128) {
+            float2 p[4];
+            float mn = m;
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                p[u] = i + 32 * u < tiles ? part[(size_t)(i + 32 * u) * ldt + t] : make_float2(-INFINITY, 0.0f);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; u++) mn = fmaxf(mn, p[u].x);
+            s *= lx_exp2(m - mn);
+#pragma unroll
+            for (int u = 0; u < 4; u++) if (p[u].y != 0.0f) s += p[u].y * lx_exp2(p[u].x - mn);
             m = mn;
         }
     sh[sl][cl] = make_float2(m, s);
     __syncthreads();
-    if (sl != 0 || t >= tokens) return;
-    m = -INFINITY;
+    // warp w joins the 32 slices of token w: a lane each, by a fixed tree
+    float2 p = sh[cl][sl];
+    float top = p.x;
 #pragma unroll
-    for (int i = 0; i < 8; i++) m = fmaxf(m, sh[i][cl].x);
-    s = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; i++) if (sh[i][cl].y != 0.0f) s += sh[i][cl].y * lx_exp2(sh[i][cl].x - m);      // slices without a tile hold (-inf, 0)
-    const float l2 = m + log2f(s);
-    lse2[t] = l2;
-    const int id = id_u16 ? (int)static_cast<const uint16_t *>(targets)[t] : static_cast<const int32_t *>(targets)[t];
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    float sum = p.y != 0.0f ? p.y * lx_exp2(p.x - top) : 0.0f;               // slices without a tile hold (-inf, 0)
+    sum = warp_sum(sum);
+    const int token = blockIdx.x * 32 + sl;
+    if (cl != 0 || token >= tokens) return;
+    const float l2 = top + log2f(sum);
+    lse2[token] = l2;
+    const int id = id_u16 ? (int)static_cast<const uint16_t *>(targets)[token] : static_cast<const int32_t *>(targets)[token];
     float loss = 0.0f;
     if (id >= 0 && id < V) {
-        loss = -logf(exp2f(fmaf(hit[t], LX_LOG2E, -l2)) + 1e-10f);
+        loss = -logf(exp2f(fmaf(hit[token], LX_LOG2E, -l2)) + 1e-10f);
         if (!isfinite(loss)) atomicAdd(&status->nonfinite, 1);
     } else if (id >= V) {
         atomicAdd(&status->oor_ids, 1);
     }
-    loss_tok[t] = loss;
+    loss_tok[token] = loss;
 }
 
 // dx[b][d][s] = alpha * sum over the shares of K, in order.
@@ -587,12 +634,12 @@ static inline int lx_pairs() { return ctx().sm_count / 2; }
 template <int EPI, int MODE> static int lx_start(cudaStream_t st, const LxMaps &maps, const LxArgs &a) {
     static bool ready = false;
     if (!ready) {
-        ANE_CUDA_TRY(cudaFuncSetAttribute(lx_gemm_kernel<EPI, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)LX_SMEM));
+        ANE_CUDA_TRY(cudaFuncSetAttribute(lx_gemm_kernel<EPI, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)lx_smem(EPI, MODE)));
         ready = true;
     }
     const long long tiles = (long long)a.m_tiles * a.n_tiles * a.splits;
     const int pairs = tiles < lx_pairs() ? (int)tiles : lx_pairs();
-    lx_gemm_kernel<EPI, MODE><<<2 * pairs, LX_THREADS, LX_SMEM, st>>>(maps, a);
+    lx_gemm_kernel<EPI, MODE><<<2 * pairs, LX_THREADS, lx_smem(EPI, MODE), st>>>(maps, a);
     ANE_LAUNCH_OK(1);
     return ANE_CUDA_OK;
 }
@@ -635,12 +682,12 @@ struct LxCall {
 // Sizes of one call: tokens of a round, vocabulary tiles of a piece, shares of K for dx.
 struct LxPlan { int chunk, piece_tiles, splits; };
 
-// A round has at most 4096 tokens.  A piece has as many vocabulary tiles as fill whole waves of the SM pairs best, counted in
+// A round has at most 8192 tokens.  A piece has as many vocabulary tiles as fill whole waves of the SM pairs best, counted in
 // waves of K blocks over all pieces and products (with four K blocks for the start of a launch), while the two parts of dl
 // stay within 192 MiB.  dx has few tiles and a long K: where its tiles leave pairs idle, K is cut into shares.
 static LxPlan lx_plan(int T_all, int D, int V, int segs, bool dx, bool d_table, bool two_parts) {
     LxPlan p;
-    const int rounds = lx_div(T_all, 4096), pairs = lx_pairs();
+    const int rounds = lx_div(T_all, 8192), pairs = lx_pairs();
     p.chunk = (int)round_up((size_t)lx_div(T_all, rounds), LX_BM);
     if (p.chunk > T_all) p.chunk = T_all;
     const int mt = lx_div(p.chunk, LX_BM), dt = lx_div(D, LX_BN), vt = lx_div(V, LX_BN);
@@ -775,7 +822,7 @@ template <typename T, typename H> static int lx_run(const LxCall &c) {
             a.n_tiles = lx_div(nv, LX_BN); a.n = nv; a.v0 = v0; a.tile0 = v0 / LX_COLS;
             if (int rc = lx_launch<LX_STATS>(c.st, m, a)) return rc;
         }
-        lx_join_kernel<<<lx_div(n_tok, 32), 256, 0, c.st>>>(lse2, loss_tok + t0, parts, hit, tg, c.id_u16, V, halves, n_tok, ldt, status);
+        lx_join_kernel<<<lx_div(n_tok, 32), 1024, 0, c.st>>>(lse2, loss_tok + t0, parts, hit, tg, c.id_u16, V, halves, n_tok, ldt, status);
         ANE_LAUNCH_OK(1);
         if (!grad) continue;
 
@@ -786,7 +833,9 @@ template <typename T, typename H> static int lx_run(const LxCall &c) {
             if (int rc = table_rows(v0, nv)) return rc;
             if (int rc = maps_for(m, segs, xh, xl, rows_hi, rows_lo, n_tok, D, ldd, LX_CTA_M, nv, D, ld, LX_BN / 2)) return rc;
             a.n_tiles = lx_div(nv, LX_BN); a.n = nv; a.v0 = v0;
-            a.hi = lh; a.lo = ll; a.ldl = ldl;
+            if (int rc = make_matrix_map(&m.hi, part, lh, n_tok, nv, ldl, 32)) return rc;
+            if (need_lo) if (int rc = make_matrix_map(&m.lo, part, ll, n_tok, nv, ldl, 32)) return rc;
+            a.two_parts = need_lo;
             if (int rc = lx_launch<LX_DLOGITS>(c.st, m, a)) return rc;
             if (c.dx) {
                 LxArgs g = a;

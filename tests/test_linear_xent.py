@@ -136,9 +136,9 @@ def test_losses_and_gradients(ops, shape, dt):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
 def test_more_tokens_than_one_round(ops, dt):
-    """4096 tokens are one round: d_table grows over several, the last of them short."""
-    x, E, t = inputs(9, 64, 700, 1000, DT[dt], seed=1)
-    dE, tok = torch.zeros(700, 64, device="cuda"), torch.zeros(9, 1000, device="cuda")
+    """8192 tokens are one round: d_table grows over several, the last of them short."""
+    x, E, t = inputs(17, 64, 700, 1000, DT[dt], seed=1)
+    dE, tok = torch.zeros(700, 64, device="cuda"), torch.zeros(17, 1000, device="cuda")
     loss, dx = ops.linear_cross_entropy(x, E, t, d_table=dE, loss_tok=tok)
     ref = reference(x, E, t)
     assert max(off(loss, ref[0])) <= 1e-5 and max(off(tok, ref[1])) <= 1e-5
