@@ -116,6 +116,12 @@ __device__ __forceinline__ void lx_load_box(uint32_t dst, const CUtensorMap *map
     asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
                  ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar) : "memory");
 }
+// One lane of a converged warp.
+__device__ __forceinline__ bool lx_elect() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
 __device__ __forceinline__ void lx_pair_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -248,14 +254,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LX_THREADS, 1) lx_ge
     const int tiles = a.m_tiles * a.n_tiles * a.splits;
     uint32_t issued = 0;                                  // copy warp: K blocks whose copies were started
 
+    // The copy warp and the matrix warp run their loops with all lanes, so that addresses and descriptors stay in uniform
+    // registers, and elect one lane for the instructions that start something.
     if (warp == 0) {
-        if (lane == 0) {
-            for (int tile = pair; tile < tiles && !*abort; tile += pairs) {
-                const int mt = tile % a.m_tiles, nt = tile / a.m_tiles % a.n_tiles;
-                const int am = mt * LX_BM + rank * LX_CTA_M, bn = nt * TILE_N + rank * (LX_BN / 2);
-                for (LxRange r(a, tile); !r.done(); r.next(), issued++) {
-                    const int st = issued % STAGES;
-                    if (!lx_wait(&empty[st], ((issued / STAGES) & 1) ^ 1, abort)) break;
+        uint32_t st = 0, phase = 1;
+        bool ok = true;
+        for (int tile = pair; tile < tiles && ok; tile += pairs) {
+            const int mt = tile % a.m_tiles, nt = tile / a.m_tiles % a.n_tiles;
+            const int am = mt * LX_BM + rank * LX_CTA_M, bn = nt * TILE_N + rank * (LX_BN / 2);
+            for (LxRange r(a, tile); !r.done(); r.next()) {
+                if (!(ok = __all_sync(0xffffffffu, lx_wait(&empty[st], phase, abort)))) break;
+                if (lx_elect()) {
                     const int k = r.k * LX_BK;
                     const uint32_t sa = base + st * STAGE_BYTES, bar = lx_in_leader(&full[st]);
                     if (rank == 0) mbar_arrive_expect_tx(&full[st], 2 * STAGE_BYTES);
@@ -278,69 +287,92 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LX_THREADS, 1) lx_ge
                         }
                     }
                 }
+                __syncwarp();
+                issued++;
+                if (++st == STAGES) { st = 0; phase ^= 1; }
             }
         }
     } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {
-            uint32_t used = 0, turn = 0;
+        if (rank == 0) {
+            uint32_t st = 0, phase = 0, turn = 0;
             bool ok = true;
-            // one stage's product with its box `box` of B into accumulator `acc`
-            auto product = [&](uint32_t stage, int box, uint32_t acc, uint32_t more) {
-                const uint32_t sa = base + stage % STAGES * STAGE_BYTES, sb = sa + box * LX_BOX_BYTES;
+            const uint64_t da = lx_desc(base, A_MN ? 8192 : 16), db = lx_desc(base, B_MN ? 8192 : 16);
+            // a stage's product with its box `box` of B into accumulator `acc`
+            auto product = [&](uint32_t stage, int box, uint32_t acc, bool more) {
+                const uint64_t sa = da + stage * (STAGE_BYTES >> 4), sb = db + (stage * (STAGE_BYTES >> 4) + box * (LX_BOX_BYTES >> 4));
 #pragma unroll
-                for (int i = 0; i < LX_BK / 16; i++)
-                    lx_mma(tmem + acc * LX_BN, lx_desc(sa + i * (A_MN ? 2048 : 32), A_MN ? 8192 : 16), lx_desc(sb + i * (B_MN ? 2048 : 32), B_MN ? 8192 : 16), a.idesc, more | i);
+                for (int i = 0; i < LX_BK / 16; i++) lx_mma(tmem + acc * LX_BN, sa + i * (A_MN ? 128 : 2), sb + i * (B_MN ? 128 : 2), a.idesc, i > 0 || more);
+            };
+            auto wait = [&](uint64_t *bar, uint32_t parity) {
+                ok = __all_sync(0xffffffffu, lx_wait(bar, parity, abort));
+                lx_fence_after();
+                return ok;
             };
             for (int tile = pair; tile < tiles && ok; tile += pairs) {
                 if constexpr (MODE == LX_WIDE) {
                     // Both accumulators share every box of A.  They are taken over one after the other, so the first one runs ahead:
-                    // by all stages but one at the beginning of a tile, where the second is still being read, and by two K blocks at the end.
+                    // by all stages but one at the beginning of a tile, where the second is still being read, and by two K blocks
+                    // at the end.
                     const LxRange r(a, tile);
                     const int n = r.k1 - r.k0;
                     for (int i = 0; i < n && ok;) {
                         const int left = n - i, group = i == 0 ? (left < STAGES - 1 ? left : STAGES - 1) : left == 2 ? 2 : 1;
-                        for (int h = 0; h < 2 && ok; h++) {
-                            if (i == 0) {
-                                if (!(ok = lx_wait(&acc_empty[h], ((turn >> 1) & 1) ^ 1, abort))) break;
-                                lx_fence_after();
-                            }
-                            for (int j = 0; j < group; j++) {
-                                if (h == 0) {
-                                    if (!(ok = lx_wait(&full[(used + j) % STAGES], ((used + j) / STAGES) & 1, abort))) break;
-                                    lx_fence_after();
-                                }
-                                product(used + j, 1 + h, h, i + j > 0);
-                                if (h == 1) lx_commit(&empty[(used + j) % STAGES]);
-                            }
-                            if (ok && i + group == n) lx_commit(&acc_full[h]);
+                        if (i == 0 && !wait(&acc_empty[0], ((turn >> 1) & 1) ^ 1)) break;
+                        uint32_t s = st, ph = phase;
+                        for (int j = 0; j < group; j++) {
+                            if (!wait(&full[s], ph)) break;
+                            if (lx_elect()) product(s, 1, 0, i + j > 0);
+                            __syncwarp();
+                            if (++s == STAGES) { s = 0; ph ^= 1; }
                         }
+                        if (!ok) break;
+                        if (i + group == n && lx_elect()) lx_commit(&acc_full[0]);
+                        __syncwarp();
+                        if (i == 0 && !wait(&acc_empty[1], ((turn >> 1) & 1) ^ 1)) break;
+                        for (int j = 0; j < group; j++) {
+                            if (lx_elect()) {
+                                product(st, 2, 1, i + j > 0);
+                                lx_commit(&empty[st]);
+                            }
+                            __syncwarp();
+                            if (++st == STAGES) { st = 0; phase ^= 1; }
+                        }
+                        if (i + group == n && lx_elect()) lx_commit(&acc_full[1]);
+                        __syncwarp();
                         i += group;
-                        used += group;
                     }
                     if (n > 0) turn += 2;
                 } else {
-                    LxRange r(a, tile);
-                    uint32_t more = 0;
-                    for (; !r.done(); used++) {
+                    bool more = false;
+                    for (LxRange r(a, tile); !r.done();) {
                         if (r.first()) {
-                            if (!(ok = lx_wait(&acc_empty[turn & 1], ((turn >> 1) & 1) ^ 1, abort))) break;
-                            lx_fence_after();
-                            more = 0;
+                            if (!wait(&acc_empty[turn & 1], ((turn >> 1) & 1) ^ 1)) break;
+                            more = false;
                         }
-                        if (!(ok = lx_wait(&full[used % STAGES], (used / STAGES) & 1, abort))) break;
-                        lx_fence_after();
-                        if (MODE == LX_TWO) { product(used, 2, turn & 1, more); more = 1; }
-                        product(used, 1, turn & 1, more);
-                        more = 1;
-                        lx_commit(&empty[used % STAGES]);
+                        if (!wait(&full[st], phase)) break;
                         r.next();
-                        if (r.first()) { lx_commit(&acc_full[turn & 1]); turn++; }      // the accumulator is complete
+                        const bool last = r.first();                  // the accumulator is complete
+                        if (lx_elect()) {
+                            if constexpr (MODE == LX_TWO) {
+                                product(st, 2, turn & 1, more);
+                                product(st, 1, turn & 1, true);
+                            } else {
+                                product(st, 1, turn & 1, more);
+                            }
+                            lx_commit(&empty[st]);
+                            if (last) lx_commit(&acc_full[turn & 1]);
+                        }
+                        __syncwarp();
+                        more = true;
+                        turn += last;
+                        if (++st == STAGES) { st = 0; phase ^= 1; }
                     }
                 }
             }
-            lx_commit(&drained);                            // also after a give-up: no instruction or arrival outlives the block
+            if (lx_elect()) lx_commit(&drained);              // also after a give-up: no instruction or arrival outlives the block
+            __syncwarp();
         }
-        if (lane == 0) mbar_wait_bounded(&drained, 0);
+        mbar_wait_bounded(&drained, 0);
     } else {
         const int quad = warp & 3, row = quad * 32 + lane;   // a warp reads the accumulator lanes of its place in the group of four
         const int c0 = warp >= 2 + LX_EPI_WARPS / 2 ? LX_COLS : 0;
