@@ -50,17 +50,14 @@ constexpr int LX_BOX_BYTES = LX_CTA_M * LX_BK * 2;                // a block's 1
 constexpr int LX_EPI_WARPS = 8;                          // two for each 32 accumulator lanes, half of the columns each
 constexpr int LX_COLS = LX_BN / 2;                       // columns of an epilogue warp
 constexpr int LX_THREADS = 64 + 32 * LX_EPI_WARPS;       // copy warp, matrix warp, epilogue warps
-constexpr int LX_STAGING_BYTES = 2 * 32 * 128;           // dlogits: an epilogue warp's 32 rows x 64 columns of both parts
-// Boxes in the ring of operands; the staging of dlogits takes part of it.
-constexpr int lx_ring_boxes(int epi, int mode) { return epi != LX_DLOGITS ? 12 : mode == LX_PLAIN ? 8 : 9; }
-constexpr size_t lx_smem(int epi, int mode) {
-    return (size_t)lx_ring_boxes(epi, mode) * LX_BOX_BYTES + (epi == LX_DLOGITS ? LX_EPI_WARPS * LX_STAGING_BYTES : 0) + 1024;
-}
+constexpr int LX_RING_BOXES = 12;                        // of operands
+constexpr int LX_STAGING_BYTES = 2 * 32 * 64;            // dlogits: an epilogue warp's 32 rows x 32 columns of both parts
+constexpr size_t lx_smem(int epi) { return (size_t)LX_RING_BOXES * LX_BOX_BYTES + (epi == LX_DLOGITS ? LX_EPI_WARPS * LX_STAGING_BYTES : 0) + 1024; }
 constexpr int LX_STEPS = 32;                             // of 16 along K that stay in an accumulator where an fp32 result is wanted
 constexpr int LX_WAIT_LIMIT = 1 << 20;
 constexpr float LX_HALF_SCALE = 16384.0f;                // of dl where it is held in fp16
 
-struct LxMaps { CUtensorMap a[3], b[3], hi, lo; };       // one pair per 16-bit product that is summed; dlogits: where dl goes
+struct LxMaps { CUtensorMap a[3], b[3]; };               // one pair per 16-bit product that is summed
 struct LxArgs {
     int segments;              // pairs in use
     int kblocks;               // K blocks of one pair
@@ -76,12 +73,12 @@ struct LxArgs {
     float2 *part; int tile0;   // stats: [half vocabulary tile][ldt], this piece's first
     float *hit;                // stats: the target's logit per token
     const float *lse2;         // dlogits: lse * log2(e)
-    int two_parts;             // dlogits: the low parts are wanted
+    void *hi, *lo; size_t ldl; // dlogits: [token][ldl]; lo null: the low parts are not wanted
     float dscale;
     // dx: [split][column][ldt] sums; d_table: [column][D]
     float *out; size_t ldt; int first;
     float alpha;
-    int half_type;             // 1 when the 16-bit parts are fp16
+    int half_type;             // 1 when the 16-bit operands are fp16
     ane_cuda_status *status;
 };
 
@@ -161,8 +158,8 @@ __device__ __forceinline__ int lx_target(const void *targets, int id_u16, int V,
 }
 
 // Two fp32 values -> their 16-bit roundings, and the roundings of what was left.
-__device__ __forceinline__ void lx_split2(float a, float b, int half_type, uint32_t &hi, uint32_t &lo) {
-    if (half_type) {
+template <bool HALF> __device__ __forceinline__ void lx_split2(float a, float b, uint32_t &hi, uint32_t &lo) {
+    if constexpr (HALF) {
         const __half2 h = __floats2half2_rn(a, b);
         const float2 f = __half22float2(h);
         const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
@@ -175,17 +172,14 @@ __device__ __forceinline__ void lx_split2(float a, float b, int half_type, uint3
         lo = *reinterpret_cast<const uint32_t *>(&l);
     }
 }
-__device__ __forceinline__ void lx_store_shared(uint32_t at, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
-    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+__device__ __forceinline__ void lx_store_shared(uint32_t at, const uint32_t (&w)[4]) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
 }
-// A box out of shared memory, columns and rows outside the matrix left out.
-__device__ __forceinline__ void lx_store_box(const CUtensorMap *map, uint32_t src, int x, int y) {
-    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];"
-                 ::"l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(src) : "memory");
+__device__ __forceinline__ uint4 lx_load_shared(uint32_t at) {
+    uint4 w;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(at) : "memory");
+    return w;
 }
-__device__ __forceinline__ void lx_store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void lx_store_read_wait() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
-__device__ __forceinline__ void lx_store_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
 // The K blocks of one tile: the tile's share [k0, k1), in parts of `span`; within a part every operand pair in turn.
 struct LxRange {
@@ -219,10 +213,10 @@ struct LxRange {
 // What bounds the products is the way from L2 to the SMs: with 64 bytes per SM and clock wanted by a 256 x 256 tile, the
 // tensor cores were busy 58 % of the time in all four products alike, at 8.8 TB/s of reads (8192 tokens would want 15).  So
 // the large products bring two boxes of B for each box of A (48 bytes per clock): LX_WIDE and LX_TWO.
-template <int EPI, int MODE>
+template <int EPI, int MODE, bool HALF>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LX_THREADS, 1) lx_gemm_kernel(const __grid_constant__ LxMaps maps, const __grid_constant__ LxArgs a) {
     constexpr bool A_MN = EPI == LX_DTABLE, B_MN = EPI == LX_DX || EPI == LX_DTABLE;
-    constexpr int BOXES = MODE == LX_PLAIN ? 2 : 3, STAGES = lx_ring_boxes(EPI, MODE) / BOXES, STAGE_BYTES = BOXES * LX_BOX_BYTES;
+    constexpr int BOXES = MODE == LX_PLAIN ? 2 : 3, STAGES = LX_RING_BOXES / BOXES, STAGE_BYTES = BOXES * LX_BOX_BYTES;
     constexpr int ACCS = MODE == LX_WIDE ? 2 : 1, TILE_N = ACCS * LX_BN;
     extern __shared__ uint8_t raw[];
     const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;       // the same offset in both blocks
@@ -445,14 +439,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LX_THREADS, 1) lx_ge
                     const bool mine = __any_sync(0xffffffffu, tgt >= 0 && tgt < LX_COLS);
                     const int row0 = mt * LX_BM + rank * LX_CTA_M + quad * 32;
                     const uint32_t stage = base + STAGES * STAGE_BYTES + (warp - 2) * LX_STAGING_BYTES;
-                    // 64 columns at a time: one 128-byte row per lane in each part, swizzled as the copy engine expects it
+                    // 32 columns at a time through shared memory (16-byte chunks swizzled against bank conflicts), so that four lanes
+                    // write 64 bytes of a row together
 #pragma unroll
-                    for (int c = 0; c < LX_COLS; c += 64) {
+                    for (int c = 0; c < LX_COLS; c += 32) {
                         if (c >= cols || row0 >= a.m) break;
-                        if (lane == 0) lx_store_read_wait();             // the staging is free again
-                        __syncwarp();
 #pragma unroll
-                        for (int q = 0; q < 8; q++) {
+                        for (int q = 0; q < 4; q++) {
                             uint32_t hi[4], lo[4];
                             float e[8];
 #pragma unroll
@@ -463,20 +456,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LX_THREADS, 1) lx_ge
                             }
 #pragma unroll
                             for (int j = 0; j < 4; j++) {
-                                lx_split2(e[2 * j], e[2 * j + 1], a.half_type, hi[j], lo[j]);
+                                lx_split2<HALF>(e[2 * j], e[2 * j + 1], hi[j], lo[j]);
                                 if (id < 0) hi[j] = lo[j] = 0;           // a masked token: zeros, whatever its logits are
                             }
-                            const uint32_t at = stage + lane * 128 + ((q ^ (lane & 7)) << 4);
-                            lx_store_shared(at, hi[0], hi[1], hi[2], hi[3]);
-                            if (a.two_parts) lx_store_shared(at + 4096, lo[0], lo[1], lo[2], lo[3]);
+                            const uint32_t at = stage + lane * 64 + ((q ^ ((lane >> 1) & 3)) << 4);
+                            lx_store_shared(at, hi);
+                            if (a.lo) lx_store_shared(at + 2048, lo);
                         }
-                        fence_proxy_async();
                         __syncwarp();
-                        if (lane == 0) {
-                            lx_store_box(&maps.hi, stage, n0 + c, row0);
-                            if (a.two_parts) lx_store_box(&maps.lo, stage + 4096, n0 + c, row0);
-                            lx_store_commit();
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const int r = i * 8 + lane / 4, q = lane & 3;
+                            const uint32_t at = stage + r * 64 + ((q ^ ((r >> 1) & 3)) << 4);
+                            const size_t to = (size_t)(row0 + r) * a.ldl + n0 + c + q * 8;
+                            if (row0 + r < a.m) {
+                                *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.hi) + to) = lx_load_shared(at);
+                                if (a.lo) *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.lo) + to) = lx_load_shared(at + 2048);
+                            }
                         }
+                        __syncwarp();
                     }
                 } else if (live) {
                     // dx: rows are tokens, columns are channels; d_table: rows are channels, columns vocabulary rows.  Either way
@@ -494,7 +492,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LX_THREADS, 1) lx_ge
             }
         }
     }
-    if (EPI == LX_DLOGITS && warp >= 2 && lane == 0) lx_store_wait();
     __syncwarp();
     lx_fence_before();
     __syncthreads();
@@ -663,17 +660,22 @@ __global__ void __launch_bounds__(256) lx_loss_kernel(float *__restrict__ loss_s
 static inline int lx_div(long long a, long long b) { return (int)((a + b - 1) / b); }
 static inline int lx_pairs() { return ctx().sm_count / 2; }
 
-template <int EPI, int MODE> static int lx_start(cudaStream_t st, const LxMaps &maps, const LxArgs &a) {
+template <int EPI, int MODE, bool HALF> static int lx_start_kernel(cudaStream_t st, const LxMaps &maps, const LxArgs &a) {
     static bool ready = false;
     if (!ready) {
-        ANE_CUDA_TRY(cudaFuncSetAttribute(lx_gemm_kernel<EPI, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)lx_smem(EPI, MODE)));
+        ANE_CUDA_TRY(cudaFuncSetAttribute(lx_gemm_kernel<EPI, MODE, HALF>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)lx_smem(EPI)));
         ready = true;
     }
     const long long tiles = (long long)a.m_tiles * a.n_tiles * a.splits;
     const int pairs = tiles < lx_pairs() ? (int)tiles : lx_pairs();
-    lx_gemm_kernel<EPI, MODE><<<2 * pairs, LX_THREADS, lx_smem(EPI, MODE), st>>>(maps, a);
+    lx_gemm_kernel<EPI, MODE, HALF><<<2 * pairs, LX_THREADS, lx_smem(EPI), st>>>(maps, a);
     ANE_LAUNCH_OK(1);
     return ANE_CUDA_OK;
+}
+// The type of the operands is the instruction's business; only dlogits writes 16-bit values itself.
+template <int EPI, int MODE> static int lx_start(cudaStream_t st, const LxMaps &maps, const LxArgs &a) {
+    if (EPI == LX_DLOGITS && a.half_type) return lx_start_kernel<EPI, MODE, EPI == LX_DLOGITS>(st, maps, a);
+    return lx_start_kernel<EPI, MODE, false>(st, maps, a);
 }
 
 // Time of a product of `tiles` accumulators of 256 x 256 (m x n of them), in K blocks of one accumulator: waves over the SM
@@ -716,7 +718,7 @@ struct LxPlan { int chunk, piece_tiles, splits; };
 
 // A round has at most 8192 tokens.  A piece has as many vocabulary tiles as fill whole waves of the SM pairs best, counted in
 // waves of K blocks over all pieces and products (with four K blocks for the start of a launch), while the two parts of dl
-// stay within 192 MiB.  dx has few tiles and a long K: where its tiles leave pairs idle, K is cut into shares.
+// stay within 384 MiB.  dx has few tiles and a long K: where its tiles leave pairs idle, K is cut into shares.
 static LxPlan lx_plan(int T_all, int D, int V, int segs, bool dx, bool d_table, bool two_parts) {
     LxPlan p;
     const int rounds = lx_div(T_all, 8192), pairs = lx_pairs();
@@ -724,7 +726,7 @@ static LxPlan lx_plan(int T_all, int D, int V, int segs, bool dx, bool d_table, 
     if (p.chunk > T_all) p.chunk = T_all;
     const int mt = lx_div(p.chunk, LX_BM), dt = lx_div(D, LX_BN), vt = lx_div(V, LX_BN);
     const int kd = lx_div(D, LX_BK), kt = lx_div(p.chunk, LX_BK);
-    long long most = (192ll << 20) / ((long long)p.chunk * LX_BN * (two_parts ? 4 : 2));
+    long long most = (384ll << 20) / ((long long)p.chunk * LX_BN * (two_parts ? 4 : 2));
     if (most < 1) most = 1;
     if (most > vt) most = vt;
     double best = 1e300;
@@ -865,9 +867,7 @@ template <typename T, typename H> static int lx_run(const LxCall &c) {
             if (int rc = table_rows(v0, nv)) return rc;
             if (int rc = maps_for(m, segs, xh, xl, rows_hi, rows_lo, n_tok, D, ldd, LX_CTA_M, nv, D, ld, LX_BN / 2)) return rc;
             a.n_tiles = lx_div(nv, LX_BN); a.n = nv; a.v0 = v0;
-            if (int rc = make_matrix_map(&m.hi, part, lh, n_tok, nv, ldl, 32)) return rc;
-            if (need_lo) if (int rc = make_matrix_map(&m.lo, part, ll, n_tok, nv, ldl, 32)) return rc;
-            a.two_parts = need_lo;
+            a.hi = lh; a.lo = ll; a.ldl = ldl;
             if (int rc = lx_launch<LX_DLOGITS>(c.st, m, a)) return rc;
             if (c.dx) {
                 LxArgs g = a;
