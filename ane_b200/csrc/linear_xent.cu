@@ -105,8 +105,10 @@ __device__ __forceinline__ uint32_t lx_in_leader(const void *p) {
     asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_u32(p)));
     return r;
 }
+// Relaxed: what has to come before it are reads of the accumulator, which have completed (a release would wait for this
+// thread's global stores as well, and hold the accumulator that long).
 __device__ __forceinline__ void lx_arrive_at(uint32_t bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 // A box into this block's shared memory, counted on a barrier of the pair's first block.
 __device__ __forceinline__ void lx_load_box(uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t bar) {
