@@ -51,8 +51,7 @@ constexpr int LX_EPI_WARPS = 8;                          // two for each 32 accu
 constexpr int LX_COLS = LX_BN / 2;                       // columns of an epilogue warp
 constexpr int LX_THREADS = 64 + 32 * LX_EPI_WARPS;       // copy warp, matrix warp, epilogue warps
 constexpr int LX_RING_BOXES = 12;                        // of operands
-constexpr int LX_STAGING_BYTES = 2 * 32 * 64;            // dlogits: an epilogue warp's 32 rows x 32 columns of both parts
-constexpr size_t lx_smem(int epi) { return (size_t)LX_RING_BOXES * LX_BOX_BYTES + (epi == LX_DLOGITS ? LX_EPI_WARPS * LX_STAGING_BYTES : 0) + 1024; }
+constexpr size_t LX_SMEM = (size_t)LX_RING_BOXES * LX_BOX_BYTES + 1024;
 constexpr int LX_STEPS = 32;                             // of 16 along K that stay in an accumulator where an fp32 result is wanted
 constexpr int LX_WAIT_LIMIT = 1 << 20;
 constexpr float LX_HALF_SCALE = 16384.0f;                // of dl where it is held in fp16
@@ -174,13 +173,10 @@ template <bool HALF> __device__ __forceinline__ void lx_split2(float a, float b,
         lo = *reinterpret_cast<const uint32_t *>(&l);
     }
 }
-__device__ __forceinline__ void lx_store_shared(uint32_t at, const uint32_t (&w)[4]) {
-    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
-}
-__device__ __forceinline__ uint4 lx_load_shared(uint32_t at) {
-    uint4 w;
-    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(at) : "memory");
-    return w;
+// 32 bytes at once: every sector of a row is written whole, although neighbouring lanes hold different rows.
+__device__ __forceinline__ void lx_store32(void *p, const uint32_t (&w)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
 }
 
 // The K blocks of one tile: the tile's share [k0, k1), in parts of `span`; within a part every operand pair in turn.
@@ -440,43 +436,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LX_THREADS, 1) lx_ge
                     const float shift = log2f(a.dscale) - lse2;          // a power of two: exp2 brings it in
                     const bool mine = __any_sync(0xffffffffu, tgt >= 0 && tgt < LX_COLS);
                     const int row0 = mt * LX_BM + rank * LX_CTA_M + quad * 32;
-                    const uint32_t stage = base + STAGES * STAGE_BYTES + (warp - 2) * LX_STAGING_BYTES;
-                    // 32 columns at a time through shared memory (16-byte chunks swizzled against bank conflicts), so that four lanes
-                    // write 64 bytes of a row together
+                    const size_t at = (size_t)m * a.ldl + n0;
+                    // 16 columns at a time straight to memory, whole sectors of 32 bytes per lane.  Rows could be written together by
+                    // way of shared memory, but its bandwidth belongs to the operands (112 of 128 bytes per clock).
 #pragma unroll
-                    for (int c = 0; c < LX_COLS; c += 32) {
+                    for (int c = 0; c < LX_COLS; c += 16) {
                         if (c >= cols || row0 >= a.m) break;
+                        uint32_t hi[8], lo[8];
+                        float e[16];
 #pragma unroll
-                        for (int q = 0; q < 4; q++) {
-                            uint32_t hi[4], lo[4];
-                            float e[8];
+                        for (int j = 0; j < 16; j++) e[j] = lx_exp2(fmaf(v[c + j], k2, shift));
+                        if (mine) {
 #pragma unroll
-                            for (int j = 0; j < 8; j++) e[j] = lx_exp2(fmaf(v[c + q * 8 + j], k2, shift));
-                            if (mine) {
-#pragma unroll
-                                for (int j = 0; j < 8; j++) e[j] = tgt == c + q * 8 + j ? e[j] - a.dscale : e[j];
-                            }
-#pragma unroll
-                            for (int j = 0; j < 4; j++) {
-                                lx_split2<HALF>(e[2 * j], e[2 * j + 1], hi[j], lo[j]);
-                                if (id < 0) hi[j] = lo[j] = 0;           // a masked token: zeros, whatever its logits are
-                            }
-                            const uint32_t at = stage + lane * 64 + ((q ^ ((lane >> 1) & 3)) << 4);
-                            lx_store_shared(at, hi);
-                            if (a.lo) lx_store_shared(at + 2048, lo);
+                            for (int j = 0; j < 16; j++) e[j] = tgt == c + j ? e[j] - a.dscale : e[j];
                         }
-                        __syncwarp();
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const int r = i * 8 + lane / 4, q = lane & 3;
-                            const uint32_t at = stage + r * 64 + ((q ^ ((r >> 1) & 3)) << 4);
-                            const size_t to = (size_t)(row0 + r) * a.ldl + n0 + c + q * 8;
-                            if (row0 + r < a.m) {
-                                *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.hi) + to) = lx_load_shared(at);
-                                if (a.lo) *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.lo) + to) = lx_load_shared(at + 2048);
-                            }
+                        for (int j = 0; j < 8; j++) {
+                            lx_split2<HALF>(e[2 * j], e[2 * j + 1], hi[j], lo[j]);
+                            if (id < 0) hi[j] = lo[j] = 0;               // a masked token: zeros, whatever its logits are
                         }
-                        __syncwarp();
+                        if (live) {
+                            lx_store32(static_cast<uint16_t *>(a.hi) + at + c, hi);
+                            if (a.lo) lx_store32(static_cast<uint16_t *>(a.lo) + at + c, lo);
+                        }
                     }
                 } else if (live) {
                     // dx: rows are tokens, columns are channels; d_table: rows are channels, columns vocabulary rows.  Either way
@@ -665,12 +647,12 @@ static inline int lx_pairs() { return ctx().sm_count / 2; }
 template <int EPI, int MODE, bool HALF> static int lx_start_kernel(cudaStream_t st, const LxMaps &maps, const LxArgs &a) {
     static bool ready = false;
     if (!ready) {
-        ANE_CUDA_TRY(cudaFuncSetAttribute(lx_gemm_kernel<EPI, MODE, HALF>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)lx_smem(EPI)));
+        ANE_CUDA_TRY(cudaFuncSetAttribute(lx_gemm_kernel<EPI, MODE, HALF>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)LX_SMEM));
         ready = true;
     }
     const long long tiles = (long long)a.m_tiles * a.n_tiles * a.splits;
     const int pairs = tiles < lx_pairs() ? (int)tiles : lx_pairs();
-    lx_gemm_kernel<EPI, MODE, HALF><<<2 * pairs, LX_THREADS, lx_smem(EPI), st>>>(maps, a);
+    lx_gemm_kernel<EPI, MODE, HALF><<<2 * pairs, LX_THREADS, LX_SMEM, st>>>(maps, a);
     ANE_LAUNCH_OK(1);
     return ANE_CUDA_OK;
 }
