@@ -242,6 +242,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LX_THREADS, 1) lx_ge
     lx_pair_sync();
     lx_fence_after();
     const uint32_t tmem = tmem_at;
+    dep_sync();                                           // nothing before this reads or writes global memory
 
     const int tiles = a.m_tiles * a.n_tiles * a.splits;
     uint32_t issued = 0;                                  // copy warp: K blocks whose copies were started
@@ -492,13 +493,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LX_THREADS, 1) lx_ge
 }
 
 // ------------------------------------------------------------------ around the products
-// fp32 inputs: the largest finite magnitude of a tensor, as the bits of a float (which compare like integers).  x is looked
-// at where its token has a target (S and D describe its layout; the table passes no targets).
-__global__ void __launch_bounds__(256) lx_largest_kernel(uint32_t *most, const float *__restrict__ p, size_t n, const void *__restrict__ targets, int id_u16, int V, int D, int S) {
+// fp32 inputs: the largest finite magnitude that each block finds in x (blockIdx.y = 0; where a token has a target) and in the
+// table (1), as the bits of a float, which compare like integers.
+constexpr int LX_LARGEST_BLOCKS = 592;
+__global__ void __launch_bounds__(256) lx_largest_kernel(uint32_t *most, const float *__restrict__ x, size_t nx, const float *__restrict__ table, size_t ne,
+                                                         const void *__restrict__ targets, int id_u16, int V, int D, int S) {
+    dep_sync();
+    const bool of_x = blockIdx.y == 0;
+    const float *p = of_x ? x : table;
+    const size_t n = of_x ? nx : ne;
     uint32_t top = 0;
     auto look = [&](float f, size_t i) {
         const uint32_t u = __float_as_uint(f) & 0x7fffffffu;
-        if (u > top && u < 0x7f800000u && (!targets || lx_target(targets, id_u16, V, (int)(i / ((size_t)D * S) * S + i % S)) >= 0)) top = u;
+        if (u > top && u < 0x7f800000u && (!of_x || lx_target(targets, id_u16, V, (int)(i / ((size_t)D * S) * S + i % S)) >= 0)) top = u;
     };
     const size_t step = (size_t)gridDim.x * 256, at = (size_t)blockIdx.x * 256 + threadIdx.x, quads = aligned16(p) ? n / 4 : 0;
     for (size_t i = at; i < quads; i += 4 * step) {
@@ -512,27 +519,41 @@ __global__ void __launch_bounds__(256) lx_largest_kernel(uint32_t *most, const f
         }
     }
     for (size_t i = 4 * quads + at; i < n; i += step) look(p[i], i);
+    __shared__ uint32_t sh[8];
     top = __reduce_max_sync(0xffffffffu, top);
-    if ((threadIdx.x & 31) == 0 && top) atomicMax(most, top);      // a maximum does not depend on the order
+    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = top;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int i = 1; i < 8; i++) top = sh[i] > top ? sh[i] : top;
+        most[blockIdx.y * LX_LARGEST_BLOCKS + blockIdx.x] = top;
+    }
 }
-// -> scale (a power of two) in scales[0..1] as its inverse, the form the products need.
-__device__ __forceinline__ float lx_scale(uint32_t most) {
-    int e = 13 - ((int)(most >> 23) - 127);
-    e = e > 60 ? 60 : e < -60 ? -60 : e;
-    return most ? __uint_as_float((uint32_t)(127 + e) << 23) : 1.0f;
+// -> scales[0..1] = 1 / scale of x and of the table, scales[2..3] the scales: powers of two that put the largest at 2^13.
+__global__ void __launch_bounds__(64) lx_scales_kernel(float *scales, const uint32_t *most, int blocks) {
+    dep_sync();
+    const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint32_t top = 0;
+    for (int i = lane; i < blocks; i += 32) { const uint32_t u = most[w * LX_LARGEST_BLOCKS + i]; top = u > top ? u : top; }
+    top = __reduce_max_sync(0xffffffffu, top);
+    int e = 13 - ((int)(top >> 23) - 127);
+    e = top == 0 ? 0 : e > 60 ? 60 : e < -60 ? -60 : e;
+    if (lane == 0) {
+        scales[w] = __uint_as_float((uint32_t)(127 - e) << 23);
+        scales[2 + w] = __uint_as_float((uint32_t)(127 + e) << 23);
+    }
 }
-__global__ void lx_scales_kernel(float *scales, const uint32_t *most) { if (threadIdx.x < 2) scales[threadIdx.x] = 1.0f / lx_scale(most[threadIdx.x]); }
 
 // x of tokens [t0, t0 + tokens) -> [token][ldx] 16-bit rows, zeros for tokens without a target; fp32 scaled, as two parts.
 template <typename T, typename H>
-__global__ void __launch_bounds__(256) lx_pack_x_kernel(H *hi, H *lo, const T *__restrict__ x, const uint32_t *most, const void *__restrict__ targets, int id_u16, int V, int t0,
+__global__ void __launch_bounds__(256) lx_pack_x_kernel(H *hi, H *lo, const T *__restrict__ x, const float *scales, const void *__restrict__ targets, int id_u16, int V, int t0,
                                                         int tokens, int D, int S, size_t ldx) {
     __shared__ float tile[32][33];
+    dep_sync();
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
     const int t = blockIdx.x * 32 + tx, d0 = blockIdx.y * 32;
     const bool live = t < tokens && lx_target(targets, id_u16, V, t0 + t) >= 0;
     const int b = (t0 + t) / S, s = (t0 + t) % S;
-    const float scale = most ? lx_scale(*most) : 1.0f;
+    const float scale = scales ? scales[2] : 1.0f;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const int d = d0 + ty + 8 * i;
@@ -554,8 +575,9 @@ __global__ void __launch_bounds__(256) lx_pack_x_kernel(H *hi, H *lo, const T *_
 
 // Rows of the table -> [row][lde] 16-bit rows with aligned ends; fp32 scaled, as two parts.
 template <typename T, typename H>
-__global__ void __launch_bounds__(256) lx_pack_rows_kernel(H *hi, H *lo, const T *__restrict__ src, const uint32_t *most, int rows, int D, size_t lde) {
-    const float scale = most ? lx_scale(*most) : 1.0f;
+__global__ void __launch_bounds__(256) lx_pack_rows_kernel(H *hi, H *lo, const T *__restrict__ src, const float *scales, int rows, int D, size_t lde) {
+    dep_sync();
+    const float scale = scales ? scales[3] : 1.0f;
     for (int r = blockIdx.x; r < rows; r += gridDim.x)
         for (int d = threadIdx.x; d < (int)lde; d += 256) {
             const float v = d < D ? Elt<T>::to_f(src[(size_t)r * D + d]) * scale : 0.0f;
@@ -565,22 +587,23 @@ __global__ void __launch_bounds__(256) lx_pack_rows_kernel(H *hi, H *lo, const T
         }
 }
 
-// (max, sum) pairs of the vocabulary tiles -> lse and loss of 32 tokens per block: 32 warps with every 32nd tile each, joined
-// in a fixed order.
+// (max, sum) pairs of the vocabulary tiles -> lse and loss of TOK tokens per block: 1024 / TOK threads take turns at the tiles
+// of a token and are joined in a fixed order.
+template <int TOK>
 __global__ void __launch_bounds__(1024) lx_join_kernel(float *__restrict__ lse2, float *__restrict__ loss_tok, const float2 *__restrict__ part, const float *__restrict__ hit,
                                                        const void *__restrict__ targets, int id_u16, int V, int tiles, int tokens, size_t ldt, ane_cuda_status *status) {
-    __shared__ float2 sh[32][33];
-    const int cl = threadIdx.x & 31, sl = threadIdx.x >> 5;
-    const int t = blockIdx.x * 32 + cl;
+    constexpr int SL = 1024 / TOK;
+    __shared__ float2 sh[SL][TOK + 1];
+    dep_sync();
+    const int cl = threadIdx.x % TOK, sl = threadIdx.x / TOK;
+    const int t = blockIdx.x * TOK + cl;
     float m = -INFINITY, s = 0.0f;
     if (t < tokens)
-        for (int i = sl; i < tiles; i += 128) {
+        for (int i = sl; i < tiles; i += 4 * SL) {
             float2 p[4];
             float mn = m;
 #pragma unroll
-            for (int u = 0; u < 4; u++) {
-                p[u] = i + 32 * u < tiles ? part[(size_t)(i + 32 * u) * ldt + t] : make_float2(-INFINITY, 0.0f);
-            }
+            for (int u = 0; u < 4; u++) p[u] = i + SL * u < tiles ? part[(size_t)(i + SL * u) * ldt + t] : make_float2(-INFINITY, 0.0f);
 #pragma unroll
             for (int u = 0; u < 4; u++) mn = fmaxf(mn, p[u].x);
             s *= lx_exp2(m - mn);
@@ -590,15 +613,22 @@ __global__ void __launch_bounds__(1024) lx_join_kernel(float *__restrict__ lse2,
         }
     sh[sl][cl] = make_float2(m, s);
     __syncthreads();
-    // warp w joins the 32 slices of token w: a lane each, by a fixed tree
-    float2 p = sh[cl][sl];
-    float top = p.x;
+    // warp w joins the slices of token w: SL / 32 per lane, then the lanes by a fixed tree
+    const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (w >= TOK) return;
+    float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < SL / 32; i++) top = fmaxf(top, sh[i * 32 + lane][w].x);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    float sum = p.y != 0.0f ? p.y * lx_exp2(p.x - top) : 0.0f;               // slices without a tile hold (-inf, 0)
+#pragma unroll
+    for (int i = 0; i < SL / 32; i++) {                                       // slices without a tile hold (-inf, 0)
+        const float2 p = sh[i * 32 + lane][w];
+        if (p.y != 0.0f) sum += p.y * lx_exp2(p.x - top);
+    }
     sum = warp_sum(sum);
-    const int token = blockIdx.x * 32 + sl;
-    if (cl != 0 || token >= tokens) return;
+    const int token = blockIdx.x * TOK + w;
+    if (lane != 0 || token >= tokens) return;
     const float l2 = top + log2f(sum);
     lse2[token] = l2;
     const int id = id_u16 ? (int)static_cast<const uint16_t *>(targets)[token] : static_cast<const int32_t *>(targets)[token];
@@ -615,6 +645,7 @@ __global__ void __launch_bounds__(1024) lx_join_kernel(float *__restrict__ lse2,
 // dx[b][d][s] = alpha * sum over the shares of K, in order.
 template <typename T>
 __global__ void __launch_bounds__(256) lx_finish_dx_kernel(T *__restrict__ dx, const float *__restrict__ sums, int splits, int t0, int tokens, int D, int S, size_t ldt, float alpha) {
+    dep_sync();
     const int t = blockIdx.x * 256 + threadIdx.x;
     if (t >= tokens) return;
     const int b = (t0 + t) / S, s = (t0 + t) % S;
@@ -628,6 +659,7 @@ __global__ void __launch_bounds__(256) lx_finish_dx_kernel(T *__restrict__ dx, c
 // loss_seq[b] = (sum_t loss_tok[b][t]) / S, fixed summation tree.
 __global__ void __launch_bounds__(256) lx_loss_kernel(float *__restrict__ loss_seq, const float *__restrict__ loss_tok, int S) {
     __shared__ float sh[8];
+    dep_sync();
     const float *p = loss_tok + (size_t)blockIdx.x * S;
     float acc = 0.0f;
     for (int t = threadIdx.x; t < S; t += 256) acc += p[t];
@@ -644,6 +676,20 @@ __global__ void __launch_bounds__(256) lx_loss_kernel(float *__restrict__ loss_s
 static inline int lx_div(long long a, long long b) { return (int)((a + b - 1) / b); }
 static inline int lx_pairs() { return ctx().sm_count / 2; }
 
+// Every kernel of the chain is a programmatic dependent launch: its blocks may be placed and set up their barriers and
+// accumulators while the kernel before drains, and stop in dep_sync() until that one has completed.  A call has 4 to 12 short
+// launches where the problem is small: 146 -> 120 us for one fp32 sequence over 9200 rows.
+template <typename... KArgs, typename... Args>
+static inline void lx_call(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args &&...args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid; cfg.blockDim = block; cfg.dynamicSmemBytes = smem; cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = tuning("linear_xent_dep", 1) != 0;
+    cfg.attrs = attr; cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);          // the error, if any, is picked up by ANE_LAUNCH_OK
+}
+
 template <int EPI, int MODE, bool HALF> static int lx_start_kernel(cudaStream_t st, const LxMaps &maps, const LxArgs &a) {
     static bool ready = false;
     if (!ready) {
@@ -652,7 +698,7 @@ template <int EPI, int MODE, bool HALF> static int lx_start_kernel(cudaStream_t 
     }
     const long long tiles = (long long)a.m_tiles * a.n_tiles * a.splits;
     const int pairs = tiles < lx_pairs() ? (int)tiles : lx_pairs();
-    lx_gemm_kernel<EPI, MODE, HALF><<<2 * pairs, LX_THREADS, LX_SMEM, st>>>(maps, a);
+    lx_call(lx_gemm_kernel<EPI, MODE, HALF>, dim3(2 * pairs), dim3(LX_THREADS), LX_SMEM, st, maps, a);
     ANE_LAUNCH_OK(1);
     return ANE_CUDA_OK;
 }
@@ -667,7 +713,7 @@ template <int EPI, int MODE> static int lx_start(cudaStream_t st, const LxMaps &
 constexpr double LX_WIDE_COST = 1.55;
 static double lx_cost(int m, int n, int splits, bool can_be_wide, bool *wide) {
     const double plain = lx_div((long long)m * n * splits, lx_pairs()), w = lx_div((long long)m * lx_div(n, 2) * splits, lx_pairs()) * LX_WIDE_COST;
-    const bool is = can_be_wide && w < plain;
+    const bool is = can_be_wide && tuning("linear_xent_wide", w < plain) != 0;
     if (wide) *wide = is;
     return is ? w : plain;
 }
@@ -756,7 +802,7 @@ template <typename T, typename H> static int lx_run(const LxCall &c) {
 
     size_t off = 0;
     auto take = [&](size_t bytes) { const size_t at = off; off += round_up(bytes, 1024); return at; };
-    const size_t o_most = take(16), o_scales = take(16);
+    const size_t o_most = take(split ? 2 * LX_LARGEST_BLOCKS * 4 : 0), o_scales = take(16);
     const size_t o_tok = take(c.loss_tok ? 0 : (size_t)T_all * 4), o_lse = take(ldt * 4), o_hit = take(ldt * 4), o_part = take((size_t)halves * ldt * 8);
     const size_t o_xh = take((size_t)chunk * ldd * 2), o_xl = take(split ? (size_t)chunk * ldd * 2 : 0);
     const size_t o_eh = take((size_t)vk * ldd * 2), o_el = take(split ? (size_t)vk * ldd * 2 : 0);
@@ -776,13 +822,12 @@ template <typename T, typename H> static int lx_run(const LxCall &c) {
     ane_cuda_status *status = ctx().status;
 
     if (split) {
-        ANE_CUDA_TRY(cudaMemsetAsync(most, 0, 8, c.st));
         const size_t nx = (size_t)T_all * D, ne = (size_t)V * D;
-        auto blocks = [&](size_t n) { const size_t b = (n + 4095) / 4096; return (unsigned)(b < 1184 ? b : 1184); };
-        lx_largest_kernel<<<blocks(nx), 256, 0, c.st>>>(most, static_cast<const float *>(c.x), nx, c.targets, c.id_u16, V, D, c.S);
-        lx_largest_kernel<<<blocks(ne), 256, 0, c.st>>>(most + 1, static_cast<const float *>(c.table), ne, nullptr, 0, 0, 1, 1);
-        lx_scales_kernel<<<1, 32, 0, c.st>>>(scales, most);
-        ANE_LAUNCH_OK(3);
+        const size_t want = ((nx > ne ? nx : ne) + 4095) / 4096;
+        const int blocks = want < LX_LARGEST_BLOCKS ? (int)want : LX_LARGEST_BLOCKS;
+        lx_call(lx_largest_kernel, dim3(blocks, 2), dim3(256), 0, c.st, most, static_cast<const float *>(c.x), nx, static_cast<const float *>(c.table), ne, c.targets, c.id_u16, V, D, c.S);
+        lx_call(lx_scales_kernel, dim3(1), dim3(64), 0, c.st, scales, most, blocks);
+        ANE_LAUNCH_OK(2);
     }
     // Rows [v0, v0 + nv) of the table as 16-bit rows with `ld` elements between them; packs them where that is needed.
     int packed = 0;                                          // rows from 0 that stay packed
@@ -796,7 +841,7 @@ template <typename T, typename H> static int lx_run(const LxCall &c) {
         }
         if (vk < V || packed < V) {
             const int lo = vk < V ? v0 : 0, n = vk < V ? nv : V;
-            lx_pack_rows_kernel<T, H><<<n < 4096 ? n : 4096, 256, 0, c.st>>>(eh, el, static_cast<const T *>(c.table) + (size_t)lo * D, split ? most + 1 : nullptr, n, D, ldd);
+            lx_call(lx_pack_rows_kernel<T, H>, dim3(n < 4096 ? n : 4096), dim3(256), 0, c.st, eh, el, static_cast<const T *>(c.table) + (size_t)lo * D, scales, n, D, ldd);
             ANE_LAUNCH_OK(1);
             if (vk == V) packed = V;
         }
@@ -818,7 +863,8 @@ template <typename T, typename H> static int lx_run(const LxCall &c) {
     for (int t0 = 0; t0 < T_all; t0 += chunk) {
         const int n_tok = T_all - t0 < chunk ? T_all - t0 : chunk;
         const void *tg = static_cast<const char *>(c.targets) + (size_t)t0 * idb;
-        lx_pack_x_kernel<T, H><<<dim3(lx_div(n_tok, 32), lx_div(D, 32)), 256, 0, c.st>>>(xh, xl, static_cast<const T *>(c.x), most, c.targets, c.id_u16, V, t0, n_tok, D, c.S, ldd);
+        lx_call(lx_pack_x_kernel<T, H>, dim3(lx_div(n_tok, 32), lx_div(D, 32)), dim3(256), 0, c.st, xh, xl, static_cast<const T *>(c.x), scales, c.targets, c.id_u16, V, t0, n_tok, D,
+                c.S, ldd);
         ANE_LAUNCH_OK(1);
 
         LxArgs a = {};
@@ -840,7 +886,9 @@ template <typename T, typename H> static int lx_run(const LxCall &c) {
             a.n_tiles = lx_div(nv, LX_BN); a.n = nv; a.v0 = v0; a.tile0 = v0 / LX_COLS;
             if (int rc = lx_launch<LX_STATS>(c.st, m, a)) return rc;
         }
-        lx_join_kernel<<<lx_div(n_tok, 32), 1024, 0, c.st>>>(lse2, loss_tok + t0, parts, hit, tg, c.id_u16, V, halves, n_tok, ldt, status);
+        // few tokens: more threads for each
+        if (n_tok <= 1024) lx_call(lx_join_kernel<4>, dim3(lx_div(n_tok, 4)), dim3(1024), 0, c.st, lse2, loss_tok + t0, parts, hit, tg, c.id_u16, V, halves, n_tok, ldt, status);
+        else lx_call(lx_join_kernel<32>, dim3(lx_div(n_tok, 32)), dim3(1024), 0, c.st, lse2, loss_tok + t0, parts, hit, tg, c.id_u16, V, halves, n_tok, ldt, status);
         ANE_LAUNCH_OK(1);
         if (!grad) continue;
 
@@ -883,11 +931,11 @@ template <typename T, typename H> static int lx_run(const LxCall &c) {
         }
         if (c.dx) {
             const int by = D < 1024 ? D : 1024;
-            lx_finish_dx_kernel<T><<<dim3(lx_div(n_tok, 256), by), 256, 0, c.st>>>(static_cast<T *>(c.dx), dxs, splits, t0, n_tok, D, c.S, ldt, alpha);
+            lx_call(lx_finish_dx_kernel<T>, dim3(lx_div(n_tok, 256), by), dim3(256), 0, c.st, static_cast<T *>(c.dx), dxs, splits, t0, n_tok, D, c.S, ldt, alpha);
             ANE_LAUNCH_OK(1);
         }
     }
-    lx_loss_kernel<<<c.B, 256, 0, c.st>>>(c.loss_seq, loss_tok, c.S);
+    lx_call(lx_loss_kernel, dim3(c.B), dim3(256), 0, c.st, c.loss_seq, loss_tok, c.S);
     ANE_LAUNCH_OK(1);
     return ANE_CUDA_OK;
 }
