@@ -234,50 +234,238 @@ block_norm_bwd_kernel(T *dx, T *df, float *__restrict__ partial, const T *dy, co
     }
 }
 
-// Sums of the rows of partials of one group (a sequence, or everything), in a fixed order: 32 channels x 8 slices of rows per
-// block.  One group: the gradients are added to their buffers.  Several (gate per sequence): the sums stay in `sums`
-// [group][2][C] for the kernel below, and dgate of the sequence is finished here.
+// ------------------------------------------------------------------ clusters
+// The channels of a token tile are shared out over a cluster of up to eight blocks, each of which keeps its part of the tile
+// on the SM (forward in registers, backward in shared memory) between the sweeps, so that every tensor crosses HBM once.  The
+// per-token sums of the blocks meet in distributed shared memory and are added in block order.  Rows of 16-byte vectors; LG
+// lanes per row, NV rows per thread.
+__device__ __forceinline__ uint32_t bn_rank() { uint32_t r; asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ uint32_t bn_size() { uint32_t r; asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ void bn_cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void bn_cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ float bn_peer(const float *p, uint32_t rank) {
+    uint32_t at;
+    float v;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
+
+// NS per-token sums over the cluster, the warps' parts three sums at a time (`red` holds [3][warps][TW]: three blocks fit an SM
+// then).  `mine` [NS][TW] is read by the other blocks until the next cluster barrier behind this call, so it is not reused
+// before that.
+template <int NS, int N, int LG> __device__ __forceinline__ void bn_cluster_sums(V<N> (&v)[NS], float *red, float *mine, float *tot) {
+    constexpr int TW = N * LG, PER = NS < 3 ? NS : 3;
+    const int lg = threadIdx.x % LG, warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+#pragma unroll
+    for (int s0 = 0; s0 < NS; s0 += PER) {
+        if (s0) __syncthreads();
+#pragma unroll
+        for (int s = 0; s < PER; s++) {
+            v[s0 + s] = bn_warp_sum<N, LG>(v[s0 + s]);
+            if (lane < LG) lanes_to_smem<N>(red + (s * BN_WARPS + warp) * TW + lg * N, v[s0 + s]);
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < PER * TW; i += BN_THREADS) {
+            const int s = i / TW, t = i % TW;
+            float a = 0.0f;
+#pragma unroll
+            for (int w = 0; w < BN_WARPS; w++) a += red[(s * BN_WARPS + w) * TW + t];
+            mine[s0 * TW + i] = a;
+        }
+    }
+    bn_cluster_arrive();
+    bn_cluster_wait();
+    const uint32_t blocks = bn_size();
+    for (int i = threadIdx.x; i < NS * TW; i += BN_THREADS) {
+        float p[8], a = 0.0f;
+#pragma unroll
+        for (uint32_t r = 0; r < 8; r++) p[r] = r < blocks ? bn_peer(mine + i, r) : 0.0f;
+#pragma unroll
+        for (uint32_t r = 0; r < 8; r++) a += p[r];
+        tot[i] = a;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int s = 0; s < NS; s++) v[s] = lanes_from_smem<N>(tot + s * TW + lg * N);
+}
+
+template <typename T, int LG, int NV>
+__global__ void __launch_bounds__(BN_THREADS, NV <= 4 ? 4 : 2)
+block_norm_cluster_kernel(T *x2, T *y, const T *x, const T *f, const float *__restrict__ w_post, const float *__restrict__ gate,
+                          const float *__restrict__ w_pre, BnShape sh, int rows) {
+    constexpr int VEC = Elt<T>::VEC, R = BN_THREADS / LG, TW = LG * VEC;
+    __shared__ __align__(16) float red[BN_WARPS * TW], mine[2][TW], tot[TW];
+    const int tile = blockIdx.x / bn_size(), c0 = (int)bn_rank() * rows;
+    const int b = tile / sh.tiles_per_seq;
+    const int lg = threadIdx.x % LG, c = c0 + threadIdx.x / LG;
+    const int end = c0 + rows < sh.C ? c0 + rows : sh.C;
+    const int t = (tile % sh.tiles_per_seq) * TW + lg * VEC;
+    const bool active = t < sh.S;
+    const size_t base = ((size_t)b * sh.C + c) * sh.S + t, step = (size_t)R * sh.S;
+    const float inv_c = 1.0f / (float)sh.C;
+    if (gate) gate += (size_t)b * sh.gate_stride;
+
+    Raw<T, VEC> rf[NV], rx[NV];
+    dep_sync();
+#pragma unroll
+    for (int k = 0; k < NV; k++) if (active && c + k * R < end) { rf[k].load_stream(f + base + k * step); rx[k].load_stream(x + base + k * step); }
+    V<VEC> ss[1] = {V<VEC>::splat(0.0f)}, r = V<VEC>::splat(1.0f);
+    if (w_post) {
+#pragma unroll
+        for (int k = 0; k < NV; k++) if (active && c + k * R < end) { const V<VEC> v = rf[k].get(); ss[0] = vfma(v, v, ss[0]); }
+        bn_cluster_sums<1, VEC, LG>(ss, red, mine[0], tot);
+        r = bn_rms(ss[0], inv_c, sh.eps);
+        ss[0] = V<VEC>::splat(0.0f);
+    }
+#pragma unroll
+    for (int k = 0; k < NV; k++)
+        if (active && c + k * R < end) {
+            const int ch = c + k * R;
+            const float s = sh.alpha * (gate ? __ldg(gate + ch) : 1.0f) * (w_post ? __ldg(w_post + ch) : 1.0f);
+            rx[k].put(vfma_s(vmul(rf[k].get(), r), s, rx[k].get()));
+            rx[k].store_stream(x2 + base + k * step);
+            const V<VEC> v = rx[k].get();
+            ss[0] = vfma(v, v, ss[0]);
+        }
+    bn_cluster_sums<1, VEC, LG>(ss, red, mine[1], tot);
+    bn_cluster_arrive();                              // this block has read its peers' sums
+    r = bn_rms(ss[0], inv_c, sh.eps);
+#pragma unroll
+    for (int k = 0; k < NV; k++)
+        if (active && c + k * R < end) {
+            rx[k].put(vscale(vmul(rx[k].get(), r), __ldg(w_pre + c + k * R)));
+            rx[k].store_stream(y + base + k * step);
+        }
+    bn_cluster_wait();                                // no block leaves while a peer may still read its sums
+}
+
+__device__ __forceinline__ void bn_copy16(void *dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
+}
+
+template <typename T, int LG, int NV>
+__global__ void __launch_bounds__(BN_THREADS, NV <= 4 ? 3 : 1)
+block_norm_bwd_cluster_kernel(T *dx, T *df, float *__restrict__ partial, const T *dy, const T *dx2, const T *x2, const T *f,
+                              const float *__restrict__ w_post, const float *__restrict__ gate, const float *__restrict__ w_pre, BnShape sh, int rows) {
+    constexpr int VEC = Elt<T>::VEC, R = BN_THREADS / LG, TW = LG * VEC;
+    extern __shared__ __align__(16) uint4 strip[];       // [4 tensors][NV][threads]: each thread's own vectors
+    __shared__ __align__(16) float red[3 * BN_WARPS * TW], mine[6 * TW], tot[6 * TW];
+    const int tile = blockIdx.x / bn_size(), c0 = (int)bn_rank() * rows;
+    const int b = tile / sh.tiles_per_seq;
+    const int lg = threadIdx.x % LG, c = c0 + threadIdx.x / LG;
+    const int end = c0 + rows < sh.C ? c0 + rows : sh.C;
+    const int t = (tile % sh.tiles_per_seq) * TW + lg * VEC;
+    const bool active = t < sh.S, want_p = w_post || gate;
+    const size_t base = ((size_t)b * sh.C + c) * sh.S + t, step = (size_t)R * sh.S;
+    const float inv_c = 1.0f / (float)sh.C;
+    if (gate) gate += (size_t)b * sh.gate_stride;
+    auto entry = [&](int tensor, int k) { return strip + (tensor * NV + k) * BN_THREADS + threadIdx.x; };
+    auto get = [&](int tensor, int k) { Raw<T, VEC> r; r.v = *entry(tensor, k); return r.get(); };
+
+    dep_sync();
+#pragma unroll
+    for (int k = 0; k < NV; k++)
+        if (active && c + k * R < end) {
+            const size_t at = base + k * step;
+            bn_copy16(entry(0, k), x2 + at);
+            bn_copy16(entry(1, k), dy + at);
+            bn_copy16(entry(2, k), f + at);
+            if (dx2) bn_copy16(entry(3, k), dx2 + at);
+        }
+    asm volatile("cp.async.wait_all;" ::: "memory");      // a thread reads back what it copied itself
+    V<VEC> s[6];
+#pragma unroll
+    for (int i = 0; i < 6; i++) s[i] = V<VEC>::splat(0.0f);
+#pragma unroll
+    for (int k = 0; k < NV; k++)
+        if (active && c + k * R < end) {
+            const int ch = c + k * R;
+            const V<VEC> vx = get(0, k), va = vscale(get(1, k), __ldg(w_pre + ch));
+            s[0] = vfma(vx, vx, s[0]);
+            s[1] = vfma(va, vx, s[1]);
+            if (w_post) {
+                const V<VEC> vf = get(2, k), vq = vscale(vf, (gate ? __ldg(gate + ch) : 1.0f) * __ldg(w_post + ch));
+                s[2] = vfma(vf, vf, s[2]);
+                if (dx2) s[3] = vfma(vq, get(3, k), s[3]);
+                s[4] = vfma(vq, va, s[4]);
+                s[5] = vfma(vq, vx, s[5]);
+            }
+        }
+    bn_cluster_sums<6, VEC, LG>(s, red, mine, tot);
+    bn_cluster_arrive();
+    const BnFactors<VEC> o = bn_factors<VEC>(s, w_post != nullptr, inv_c, sh.alpha, sh.eps);
+    const V<VEC> nk = vscale(o.k, -1.0f), nj = vscale(o.j, -1.0f);
+    float2 *prow = reinterpret_cast<float2 *>(partial) + (size_t)tile * sh.C;
+#pragma unroll
+    for (int k = 0; k < NV; k++) {
+        const int ch = c + k * R;
+        float sum_q = 0.0f, sum_p = 0.0f;
+        if (active && ch < end) {
+            const V<VEC> vx = get(0, k), vy = get(1, k), vf = get(2, k);
+            V<VEC> G = vfma(vscale(vy, __ldg(w_pre + ch)), o.r2, vmul(nk, vx));
+            if (dx2) G = vadd(G, get(3, k));
+            sum_q = vmul(vy, vmul(vx, o.r2)).hsum();
+            sum_p = vmul(vmul(vf, o.rf), G).hsum();
+            Raw<T, VEC> out;
+            out.put(G);
+            out.store_stream(dx + base + k * step);
+            const float gw = (gate ? __ldg(gate + ch) : 1.0f) * (w_post ? __ldg(w_post + ch) : 1.0f);
+            out.put(vfma(vscale(G, sh.alpha * gw), o.rf, vmul(nj, vf)));
+            out.store_stream(df + base + k * step);
+        }
+        sum_q = bn_row_sum<LG>(sum_q);
+        if (want_p) sum_p = bn_row_sum<LG>(sum_p);
+        if (lg == 0 && ch < end) prow[ch] = make_float2(sum_q, sum_p);
+    }
+    bn_cluster_wait();
+}
+
+// ------------------------------------------------------------------ parameter gradients
+// Sums of the rows of partials [row][C] of one group, in a fixed order: 32 channels x 8 slices of rows per block.  The sums
+// stay in `sums` [group][C] for the kernel below; where a group is a sequence with a gate of its own, its dgate is finished
+// here.  Rows of a group are consecutive; the last group may be shorter.
 __global__ void __launch_bounds__(256)
-block_norm_grad_kernel(const float *__restrict__ partial, int rows, float *__restrict__ sums, float *__restrict__ dw_post, float *__restrict__ dgate,
-                       float *__restrict__ dw_pre, const float *__restrict__ w_post, const float *__restrict__ gate, int C, float alpha) {
+block_norm_grad_kernel(const float2 *__restrict__ partial, long long all_rows, int rows, float2 *__restrict__ sums, float *__restrict__ dgate,
+                       const float *__restrict__ w_post, int C, float alpha) {
     __shared__ float2 acc[8][32];
+    dep_sync();
     const int cl = threadIdx.x & 31, sl = threadIdx.x >> 5;
-    const int c = blockIdx.x * 32 + cl, group = blockIdx.y;
-    const int per = (rows + 7) / 8;
-    const int r0 = sl * per, r1 = r0 + per < rows ? r0 + per : rows;
-    const float2 *p = reinterpret_cast<const float2 *>(partial) + (size_t)group * rows * C;
+    const int c = blockIdx.x * 32 + cl;
+    const size_t group = blockIdx.y;
+    const long long left = all_rows - (long long)group * rows;
+    const int have = left < rows ? (int)left : rows, per = (have + 7) / 8;
+    const int r0 = sl * per, r1 = r0 + per < have ? r0 + per : have;
+    const float2 *p = partial + group * rows * C;
     float2 s = make_float2(0.0f, 0.0f);
     if (c < C) {
         int r = r0;
-        for (; r + 8 <= r1; r += 8) {
-            float2 v[8];
+        for (; r + 4 <= r1; r += 4) {
+            float2 v[4];
 #pragma unroll
-            for (int u = 0; u < 8; u++) v[u] = p[(size_t)(r + u) * C + c];
+            for (int u = 0; u < 4; u++) v[u] = p[(size_t)(r + u) * C + c];
 #pragma unroll
-            for (int u = 0; u < 8; u++) { s.x += v[u].x; s.y += v[u].y; }
+            for (int u = 0; u < 4; u++) { s.x += v[u].x; s.y += v[u].y; }
         }
         for (; r < r1; r++) { const float2 v = p[(size_t)r * C + c]; s.x += v.x; s.y += v.y; }
     }
     acc[sl][cl] = s;
     __syncthreads();
     if (sl != 0 || c >= C) return;
-    float q = 0.0f, a = 0.0f;
+    s = make_float2(0.0f, 0.0f);
 #pragma unroll
-    for (int i = 0; i < 8; i++) { q += acc[i][cl].x; a += acc[i][cl].y; }
-    a *= alpha;
-    if (dgate) dgate[(sums ? (size_t)group * C : 0) + c] += w_post ? w_post[c] * a : a;
-    if (sums) {
-        sums[((size_t)group * 2) * C + c] = q;
-        sums[((size_t)group * 2 + 1) * C + c] = a * gate[(size_t)group * C + c];
-    } else {
-        if (dw_pre) dw_pre[c] += q;
-        if (dw_post) dw_post[c] += gate ? gate[c] * a : a;
-    }
+    for (int i = 0; i < 8; i++) { s.x += acc[i][cl].x; s.y += acc[i][cl].y; }
+    s.y *= alpha;
+    if (dgate) dgate[group * C + c] += w_post ? w_post[c] * s.y : s.y;
+    sums[group * C + c] = s;
 }
 
+// The groups' sums, in order, into the parameter gradients.  A gate per sequence weighs each group's share of dw_post.
 __global__ void __launch_bounds__(256)
-block_norm_grad_join_kernel(const float *__restrict__ sums, int groups, float *__restrict__ dw_post, float *__restrict__ dw_pre, int C) {
+block_norm_grad_join_kernel(const float2 *__restrict__ sums, int groups, float *__restrict__ dw_post, float *__restrict__ dgate, float *__restrict__ dw_pre,
+                            const float *__restrict__ w_post, const float *__restrict__ gate, int gate_stride, int C) {
     __shared__ float2 acc[8][32];
+    dep_sync();
     const int cl = threadIdx.x & 31, sl = threadIdx.x >> 5;
     const int c = blockIdx.x * 32 + cl;
     const int per = (groups + 7) / 8;
@@ -285,15 +473,48 @@ block_norm_grad_join_kernel(const float *__restrict__ sums, int groups, float *_
     float2 s = make_float2(0.0f, 0.0f);
     if (c < C)
 #pragma unroll 4
-        for (int g = g0; g < g1; g++) { s.x += sums[((size_t)g * 2) * C + c]; s.y += sums[((size_t)g * 2 + 1) * C + c]; }
+        for (int g = g0; g < g1; g++) {
+            const float2 v = sums[(size_t)g * C + c];
+            s.x += v.x;
+            s.y += gate_stride ? v.y * gate[(size_t)g * gate_stride + c] : v.y;
+        }
     acc[sl][cl] = s;
     __syncthreads();
     if (sl != 0 || c >= C) return;
-    float q = 0.0f, a = 0.0f;
+    s = make_float2(0.0f, 0.0f);
 #pragma unroll
-    for (int i = 0; i < 8; i++) { q += acc[i][cl].x; a += acc[i][cl].y; }
-    if (dw_pre) dw_pre[c] += q;
-    if (dw_post) dw_post[c] += a;
+    for (int i = 0; i < 8; i++) { s.x += acc[i][cl].x; s.y += acc[i][cl].y; }
+    if (dw_pre) dw_pre[c] += s.x;
+    if (dw_post) dw_post[c] += gate && !gate_stride ? gate[c] * s.y : s.y;
+    if (dgate && !gate_stride) dgate[c] += w_post ? w_post[c] * s.y : s.y;
+}
+
+// Blocks of a cluster and channels of each; 0 blocks: no cluster form for this many channels.
+struct BnSplit { int blocks, rows; };
+static BnSplit bn_split(int C, int rows_most) {
+    const int blocks = (C + rows_most - 1) / rows_most;
+    if (blocks > 8) return {0, 0};
+    return {blocks, (C + blocks - 1) / blocks};
+}
+template <typename... KArgs, typename... Args>
+static inline void bn_call(void (*kernel)(KArgs...), dim3 grid, int cluster, size_t smem, cudaStream_t st, Args &&...args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid; cfg.blockDim = dim3(BN_THREADS); cfg.dynamicSmemBytes = smem; cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)cluster; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr; cfg.numAttrs = cluster ? 2 : 1;
+    cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);      // the error, if any, is picked up by ANE_LAUNCH_OK
+}
+// Picks lanes per row and rows per thread: 128-byte rows where eight blocks hold the channels, else 64-byte rows.
+template <typename Fn> static int bn_pick_cluster(int C, Fn &&go) {
+    using I4 = std::integral_constant<int, 4>;
+    using I8 = std::integral_constant<int, 8>;
+    if (C <= 1024) return go(I8(), I4(), bn_split(C, BN_THREADS / 8 * 4));
+    if (C <= 2048) return go(I4(), I4(), bn_split(C, BN_THREADS / 4 * 4));
+    return go(I4(), I8(), bn_split(C, BN_THREADS / 4 * 8));
 }
 
 // LG lanes of VEC tokens per row of a tile for the kernels above.
@@ -326,6 +547,17 @@ int ane_cuda_block_norm_dev(void *stream, ane_dtype dtype, int B, int C, int S, 
     BnShape sh = {B, C, S, 0, 0, gate_per_seq ? C : 0, alpha, eps};
     ANE_DISPATCH_DTYPE(dtype, T, {
         const bool vec = S % Elt<T>::VEC == 0 && aligned16(x2) && aligned16(y) && aligned16(x) && aligned16(f);
+        if (vec && C <= 4096 && tuning("block_norm_cluster", 1)) {
+            bn_pick_cluster(C, [&](auto lg, auto nv, BnSplit sp) {
+                constexpr int LG = decltype(lg)::value, NV = decltype(nv)::value;
+                sh.tiles_per_seq = (S + LG * Elt<T>::VEC - 1) / (LG * Elt<T>::VEC);
+                bn_call(block_norm_cluster_kernel<T, LG, NV>, dim3((unsigned)B * (unsigned)sh.tiles_per_seq * (unsigned)sp.blocks), sp.blocks, 0, st, (T *)x2, (T *)y, (const T *)x,
+                        (const T *)f, w_post, gate, w_pre, sh, sp.rows);
+                return 0;
+            });
+            ANE_LAUNCH_OK(1);
+            return ANE_CUDA_OK;
+        }
         bn_pick<T>(vec, S, [&](auto v, auto lg) {
             constexpr int VEC = decltype(v)::value, LG = decltype(lg)::value;
             sh.tiles_per_seq = (S + VEC * LG - 1) / (VEC * LG);
@@ -354,46 +586,67 @@ int ane_cuda_block_norm_bwd_dev(void *stream, ane_dtype dtype, int B, int C, int
     ANE_CHECK_EXTENT(dw_pre, (size_t)C * 4); ANE_CHECK_EXTENT(gate, gb); ANE_CHECK_EXTENT(dgate, gb);
     cudaStream_t st = (cudaStream_t)stream;
     BnShape sh = {B, C, S, 0, 0, gate_per_seq ? C : 0, alpha, eps};
-    const int groups = gate_per_seq ? B : 1;
-    int rows = 1;
-    float *partial = nullptr, *sums = nullptr;
+    float2 *partial = nullptr, *sums = nullptr;
+    long long all_rows = 0;          // of partial sums, and how many make a group
+    int rows = 1, groups = 1;
+    // Scratch for the partial rows and the groups' sums.  A group is a sequence where the gate is per sequence, else 64 rows.
+    auto scratch = [&](long long n, int per_seq) -> int {
+        all_rows = n;
+        rows = per_seq ? per_seq : 64;
+        groups = (int)((n + rows - 1) / rows);
+        const size_t pbytes = round_up((size_t)n * C * sizeof(float2), 256);
+        char *ws = static_cast<char *>(workspace(pbytes + (size_t)groups * C * sizeof(float2)));
+        if (!ws) return fail(ANE_CUDA_ERR_NOMEM, "ane_cuda_block_norm_bwd_dev: no scratch");
+        partial = reinterpret_cast<float2 *>(ws);
+        sums = reinterpret_cast<float2 *>(ws + pbytes);
+        return ANE_CUDA_OK;
+    };
     ANE_DISPATCH_DTYPE(dtype, T, {
         const bool vec = S % Elt<T>::VEC == 0 && aligned16(dx) && aligned16(df) && aligned16(dy) && aligned16(dx2) && aligned16(x2) && aligned16(f);
-        const int rc = bn_pick<T>(vec, S, [&](auto v, auto lg) {
-            constexpr int VEC = decltype(v)::value, LG = decltype(lg)::value;
-            sh.tiles_per_seq = (S + VEC * LG - 1) / (VEC * LG);
-            // up to eight blocks per SM, each with a row of partial sums
-            const long long most = 8LL * ctx().sm_count;
-            if (gate_per_seq) {
-                const long long want = (most + B - 1) / B;
-                rows = sh.rows_per_seq = (int)(want < sh.tiles_per_seq ? want : sh.tiles_per_seq);
-            } else {
+        int rc;
+        if (vec && C <= 4096 && tuning("block_norm_cluster", 1)) {
+            rc = bn_pick_cluster(C, [&](auto lg, auto nv, BnSplit sp) -> int {
+                constexpr int LG = decltype(lg)::value, NV = decltype(nv)::value;
+                constexpr size_t smem = (size_t)4 * NV * BN_THREADS * 16;
+                static bool ready = false;
+                if (!ready) {
+                    ANE_CUDA_TRY(cudaFuncSetAttribute(block_norm_bwd_cluster_kernel<T, LG, NV>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+                    ready = true;
+                }
+                sh.tiles_per_seq = (S + LG * Elt<T>::VEC - 1) / (LG * Elt<T>::VEC);
                 const long long tiles = (long long)B * sh.tiles_per_seq;
-                rows = (int)(tiles < most ? tiles : most);
-            }
-            const size_t blocks = (size_t)rows * groups;
-            const size_t pbytes = round_up(blocks * 2 * C * sizeof(float), 256);
-            char *ws = static_cast<char *>(workspace(pbytes + (gate_per_seq ? (size_t)B * 2 * C * sizeof(float) : 0)));
-            if (!ws) return fail(ANE_CUDA_ERR_NOMEM, "ane_cuda_block_norm_bwd_dev: no scratch");
-            partial = reinterpret_cast<float *>(ws);
-            sums = gate_per_seq ? reinterpret_cast<float *>(ws + pbytes) : nullptr;
-            block_norm_bwd_kernel<T, VEC, LG><<<(unsigned)blocks, BN_THREADS, 0, st>>>((T *)dx, (T *)df, partial, (const T *)dy, (const T *)dx2, (const T *)x2,
-                                                                                     (const T *)f, w_post, gate, w_pre, sh);
-            return (int)ANE_CUDA_OK;
-        });
+                if (int e = scratch(tiles, gate_per_seq ? sh.tiles_per_seq : 0)) return e;
+                bn_call(block_norm_bwd_cluster_kernel<T, LG, NV>, dim3((unsigned)tiles * (unsigned)sp.blocks), sp.blocks, smem, st, (T *)dx, (T *)df, reinterpret_cast<float *>(partial),
+                        (const T *)dy, (const T *)dx2, (const T *)x2, (const T *)f, w_post, gate, w_pre, sh, sp.rows);
+                return ANE_CUDA_OK;
+            });
+        } else {
+            rc = bn_pick<T>(vec, S, [&](auto v, auto lg) -> int {
+                constexpr int VEC = decltype(v)::value, LG = decltype(lg)::value;
+                sh.tiles_per_seq = (S + VEC * LG - 1) / (VEC * LG);
+                // up to eight blocks per SM, each with a row of partial sums
+                const long long most = 8LL * ctx().sm_count, tiles = (long long)B * sh.tiles_per_seq, want = (most + B - 1) / B;
+                sh.rows_per_seq = !gate_per_seq ? 0 : (int)(want < sh.tiles_per_seq ? want : sh.tiles_per_seq);
+                const long long blocks = gate_per_seq ? (long long)B * sh.rows_per_seq : tiles < most ? tiles : most;
+                if (int e = scratch(blocks, sh.rows_per_seq)) return e;
+                block_norm_bwd_kernel<T, VEC, LG><<<(unsigned)blocks, BN_THREADS, 0, st>>>((T *)dx, (T *)df, reinterpret_cast<float *>(partial), (const T *)dy, (const T *)dx2,
+                                                                                         (const T *)x2, (const T *)f, w_post, gate, w_pre, sh);
+                return ANE_CUDA_OK;
+            });
+        }
         if (rc != ANE_CUDA_OK) return rc;
     });
     ANE_LAUNCH_OK(1);
     if (dw_pre || dw_post || dgate) {
-        // gridDim.y holds 65535 groups: more sequences than that take further launches
+        // gridDim.y holds 65535 groups: more than that take further launches
         for (int g0 = 0; g0 < groups; g0 += 65535) {
             const int n = groups - g0 < 65535 ? groups - g0 : 65535;
-            block_norm_grad_kernel<<<dim3((C + 31) / 32, n), 256, 0, st>>>(partial + (size_t)g0 * rows * 2 * C, rows, sums ? sums + (size_t)g0 * 2 * C : nullptr, dw_post,
-                                                                          dgate ? dgate + (size_t)g0 * C : nullptr, dw_pre, w_post, gate ? gate + (size_t)g0 * C : nullptr, C, alpha);
+            bn_call(block_norm_grad_kernel, dim3((C + 31) / 32, n), 0, 0, st, partial + (size_t)g0 * rows * C, all_rows - (long long)g0 * rows, rows, sums + (size_t)g0 * C,
+                    gate_per_seq && dgate ? dgate + (size_t)g0 * C : nullptr, w_post, C, alpha);
             ANE_LAUNCH_OK(1);
         }
-        if (sums && (dw_pre || dw_post)) {
-            block_norm_grad_join_kernel<<<(C + 31) / 32, 256, 0, st>>>(sums, groups, dw_post, dw_pre, C);
+        if (dw_pre || dw_post || (dgate && !gate_per_seq)) {
+            bn_call(block_norm_grad_join_kernel, dim3((C + 31) / 32), 0, 0, st, sums, groups, dw_post, dgate, dw_pre, w_post, gate, sh.gate_stride, C);
             ANE_LAUNCH_OK(1);
         }
     }
