@@ -50,9 +50,34 @@ template <int LG> __device__ __forceinline__ float bn_row_sum(float v) {
     return v;
 }
 
-// NS per-token sums over the block: each warp's total goes to shared memory, the warps are added in order.  `red` holds
-// [NS][warps][TW] floats, `tot` [NS][TW].  Ends with the totals in registers and the arrays free for reuse.
-template <int NS, int N, int LG> __device__ __forceinline__ void bn_block_sums(V<N> (&v)[NS], float *red, float *tot) {
+// Per-token factors out of per-token sums, once per token and not once per thread (a root and a division are 25
+// instructions): `tot` points at a token's sums, TW apart; the factors replace the first of them.
+template <int TW> struct BnRms {                         // sum of squares -> 1 / rms
+    static constexpr int FACTORS = 1;
+    float inv_c, eps;
+    __device__ __forceinline__ void operator()(float *tot) const { tot[0] = 1.0f / sqrtf(fmaf(tot[0], inv_c, eps)); }
+};
+// The six sums of the backward pass -> r_2, -k, r_f, -j.
+template <int TW> struct BnBwd {
+    static constexpr int FACTORS = 4;
+    float inv_c, eps, alpha;
+    bool post;
+    __device__ __forceinline__ void operator()(float *tot) const {
+        const float r2 = 1.0f / sqrtf(fmaf(tot[0], inv_c, eps));
+        const float rf = post ? 1.0f / sqrtf(fmaf(tot[2 * TW], inv_c, eps)) : 1.0f;
+        const float k = r2 * r2 * r2 * (tot[TW] * inv_c);
+        const float j = post ? alpha * rf * rf * rf * (inv_c * (tot[3 * TW] + r2 * tot[4 * TW] - k * tot[5 * TW])) : 0.0f;
+        tot[0] = r2;
+        tot[TW] = -k;
+        tot[2 * TW] = rf;
+        tot[3 * TW] = -j;
+    }
+};
+
+// NS per-token sums over the block, then their factors: each warp's total goes to shared memory, the warps are added in order.
+// `red` holds [NS][warps][TW] floats, `tot` [NS][TW].  Ends with the factors in registers; `tot` is read until the next
+// barrier.
+template <int NS, int N, int LG, typename F> __device__ __forceinline__ void bn_block_sums(V<N> (&v)[NS], float *red, float *tot, F finish) {
     constexpr int TW = N * LG;
     const int lg = threadIdx.x % LG, warp = threadIdx.x / 32, lane = threadIdx.x & 31;
 #pragma unroll
@@ -69,15 +94,10 @@ template <int NS, int N, int LG> __device__ __forceinline__ void bn_block_sums(V
         tot[i] = a;
     }
     __syncthreads();
+    if (threadIdx.x < TW) finish(tot + threadIdx.x);
+    __syncthreads();
 #pragma unroll
-    for (int s = 0; s < NS; s++) v[s] = lanes_from_smem<N>(tot + s * TW + lg * N);
-}
-
-template <int N> __device__ __forceinline__ V<N> bn_rms(const V<N> &sumsq, float inv_c, float eps) {
-    V<N> r;
-#pragma unroll
-    for (int j = 0; j < N; j++) r.set(j, 1.0f / sqrtf(fmaf(sumsq.get(j), inv_c, eps)));
-    return r;
+    for (int s = 0; s < F::FACTORS; s++) v[s] = lanes_from_smem<N>(tot + s * TW + lg * N);
 }
 
 // Any shape.  A block owns a [C x LG*VEC] token tile and sweeps the channels up to three times; what one sweep read the
@@ -98,6 +118,7 @@ block_norm_kernel(T *x2, T *y, const T *x, const T *f, const float *__restrict__
     const float inv_c = 1.0f / (float)sh.C;
     if (gate) gate += (size_t)b * sh.gate_stride;
 
+    const BnRms<TW> rms = {inv_c, sh.eps};
     V<VEC> rf = V<VEC>::splat(1.0f);
     if (w_post) {
         V<VEC> ss[1] = {V<VEC>::splat(0.0f)};
@@ -108,8 +129,8 @@ block_norm_kernel(T *x2, T *y, const T *x, const T *f, const float *__restrict__
                 r.load(f + base + (size_t)c * sh.S);
                 ss[0] = vfma(r.get(), r.get(), ss[0]);
             }
-        bn_block_sums<1, VEC, LG>(ss, red, tot);
-        rf = bn_rms(ss[0], inv_c, sh.eps);
+        bn_block_sums<1, VEC, LG>(ss, red, tot, rms);
+        rf = ss[0];
     }
     V<VEC> ss[1] = {V<VEC>::splat(0.0f)};
     if (active)
@@ -124,8 +145,8 @@ block_norm_kernel(T *x2, T *y, const T *x, const T *f, const float *__restrict__
             q.store(x2 + at);
             ss[0] = vfma(q.get(), q.get(), ss[0]);
         }
-    bn_block_sums<1, VEC, LG>(ss, red, tot);
-    const V<VEC> r2 = bn_rms(ss[0], inv_c, sh.eps);
+    bn_block_sums<1, VEC, LG>(ss, red, tot, rms);
+    const V<VEC> r2 = ss[0];
     if (active)
 #pragma unroll 4
         for (int c = rg; c < sh.C; c += R) {
@@ -135,22 +156,6 @@ block_norm_kernel(T *x2, T *y, const T *x, const T *f, const float *__restrict__
             q.put(vscale(vmul(q.get(), r2), __ldg(w_pre + c)));
             q.store(y + at);
         }
-}
-
-// The six per-token sums of the backward pass -> the five per-token factors of the sweep that writes.
-template <int N> struct BnFactors { V<N> r2, k, rf, j; };
-template <int N> __device__ __forceinline__ BnFactors<N> bn_factors(const V<N> (&s)[6], bool post, float inv_c, float alpha, float eps) {
-    BnFactors<N> o;
-    o.r2 = bn_rms(s[0], inv_c, eps);
-    o.rf = post ? bn_rms(s[2], inv_c, eps) : V<N>::splat(1.0f);
-#pragma unroll
-    for (int i = 0; i < N; i++) {
-        const float r2 = o.r2.get(i), rf = o.rf.get(i);
-        const float k = r2 * r2 * r2 * (s[1].get(i) * inv_c);
-        o.k.set(i, k);
-        o.j.set(i, post ? alpha * rf * rf * rf * (inv_c * (s[3].get(i) + r2 * s[4].get(i) - k * s[5].get(i))) : 0.0f);
-    }
-    return o;
 }
 
 template <typename T, int VEC, int LG>
@@ -197,9 +202,8 @@ block_norm_bwd_kernel(T *dx, T *df, float *__restrict__ partial, const T *dy, co
                     s[5] = vfma(vq, vx, s[5]);
                 }
             }
-        bn_block_sums<6, VEC, LG>(s, red, tot);
-        const BnFactors<VEC> o = bn_factors<VEC>(s, w_post != nullptr, inv_c, sh.alpha, sh.eps);
-        const V<VEC> nk = vscale(o.k, -1.0f), nj = vscale(o.j, -1.0f);
+        bn_block_sums<6, VEC, LG>(s, red, tot, BnBwd<TW>{inv_c, sh.eps, sh.alpha, w_post != nullptr});
+        const V<VEC> r2 = s[0], nk = s[1], rms_f = s[2], nj = s[3];
         for (int c = rg; c < (sh.C + R - 1) / R * R; c += R) {     // whole warps stay together for the row sums
             float sum_q = 0.0f, sum_p = 0.0f;
             if (active && c < sh.C) {
@@ -210,16 +214,16 @@ block_norm_bwd_kernel(T *dx, T *df, float *__restrict__ partial, const T *dy, co
                 if (dx2) rd.load(dx2 + at);
                 rf.load(f + at);
                 const V<VEC> vx = rx.get(), vy = ry.get(), vf = rf.get();
-                const V<VEC> z = vmul(vx, o.r2);
-                V<VEC> G = vfma(vscale(vy, __ldg(w_pre + c)), o.r2, vmul(nk, vx));
+                const V<VEC> z = vmul(vx, r2);
+                V<VEC> G = vfma(vscale(vy, __ldg(w_pre + c)), r2, vmul(nk, vx));
                 if (dx2) G = vadd(G, rd.get());
                 sum_q = vmul(vy, z).hsum();
                 const float gw = (g ? __ldg(g + c) : 1.0f) * (w_post ? __ldg(w_post + c) : 1.0f);
-                const V<VEC> u = vmul(vf, o.rf);
+                const V<VEC> u = vmul(vf, rms_f);
                 sum_p = vmul(u, G).hsum();
                 rx.put(G);
                 rx.store(dx + at);
-                rf.put(vfma(vscale(G, sh.alpha * gw), o.rf, vmul(nj, vf)));
+                rf.put(vfma(vscale(G, sh.alpha * gw), rms_f, vmul(nj, vf)));
                 rf.store(df + at);
             }
             sum_q = bn_row_sum<LG>(sum_q);
@@ -243,6 +247,8 @@ __device__ __forceinline__ uint32_t bn_rank() { uint32_t r; asm("mov.u32 %0, %%c
 __device__ __forceinline__ uint32_t bn_size() { uint32_t r; asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r)); return r; }
 __device__ __forceinline__ void bn_cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void bn_cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// An arrival that publishes nothing (a release would wait for this thread's stores to global memory).
+__device__ __forceinline__ void bn_cluster_leave() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
 __device__ __forceinline__ float bn_peer(const float *p, uint32_t rank) {
     uint32_t at;
     float v;
@@ -251,19 +257,59 @@ __device__ __forceinline__ float bn_peer(const float *p, uint32_t rank) {
     return v;
 }
 
+// Sums of N values a lane over the lanes that differ in the bits OFF, 2*OFF, ... 16.  As long as the count allows it a step
+// exchanges halves: the lane with the bit set goes on with the upper half, so each step halves the work.  `first` is the index
+// of the values that a lane ends up with; lanes that only hold copies drop out as writers.  -> number of values held.
+template <int N, int OFF> struct BnFold {
+    static constexpr bool HALVE = N % 8 == 0;
+    static constexpr int LEFT = BnFold<HALVE ? N / 2 : N, 2 * OFF>::LEFT;
+    __device__ __forceinline__ static void run(float *a, int lane, int &first, bool &writer) {
+        const bool up = lane & OFF;
+        if constexpr (HALVE) {
+#pragma unroll
+            for (int i = 0; i < N / 2; i++) {
+                const float other = __shfl_xor_sync(0xffffffffu, up ? a[i] : a[i + N / 2], OFF);
+                a[i] = (up ? a[i + N / 2] : a[i]) + other;
+            }
+            first += up ? N / 2 : 0;
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; i++) a[i] += __shfl_xor_sync(0xffffffffu, a[i], OFF);
+            writer = writer && !up;
+        }
+        BnFold<HALVE ? N / 2 : N, 2 * OFF>::run(a, lane, first, writer);
+    }
+};
+template <int N> struct BnFold<N, 32> {
+    static constexpr int LEFT = N;
+    __device__ __forceinline__ static void run(float *, int, int &, bool &) {}
+};
+
 // NS per-token sums over the cluster, the warps' parts three sums at a time (`red` holds [3][warps][TW]: three blocks fit an SM
 // then).  `mine` [NS][TW] is read by the other blocks until the next cluster barrier behind this call, so it is not reused
 // before that.
-template <int NS, int N, int LG> __device__ __forceinline__ void bn_cluster_sums(V<N> (&v)[NS], float *red, float *mine, float *tot) {
+template <int NS, int N, int LG, typename F> __device__ __forceinline__ void bn_cluster_sums(V<N> (&v)[NS], float *red, float *mine, float *tot, F finish) {
     constexpr int TW = N * LG, PER = NS < 3 ? NS : 3;
     const int lg = threadIdx.x % LG, warp = threadIdx.x / 32, lane = threadIdx.x & 31;
 #pragma unroll
     for (int s0 = 0; s0 < NS; s0 += PER) {
-        if (s0) __syncthreads();
+        float a[PER * N];
 #pragma unroll
-        for (int s = 0; s < PER; s++) {
-            v[s0 + s] = bn_warp_sum<N, LG>(v[s0 + s]);
-            if (lane < LG) lanes_to_smem<N>(red + (s * BN_WARPS + warp) * TW + lg * N, v[s0 + s]);
+        for (int s = 0; s < PER; s++)
+#pragma unroll
+            for (int j = 0; j < N; j++) a[s * N + j] = v[s0 + s].get(j);
+        int first = 0;
+        bool writer = true;
+        BnFold<PER * N, LG>::run(a, lane, first, writer);
+        if (s0) __syncthreads();
+        constexpr int LEFT = BnFold<PER * N, LG>::LEFT;
+        static_assert(LEFT % 4 == 0, "whole 16-byte words");
+        if (writer) {
+#pragma unroll
+            for (int i = 0; i < LEFT; i += 4) {
+                const int at = first + i;                         // value at % N of sum at / N
+                *reinterpret_cast<float4 *>(red + ((at / N) * BN_WARPS + warp) * TW + lg * N + at % N) = make_float4(a[i], a[i + 1], a[i + 2], a[i + 3]);
+            }
         }
         __syncthreads();
         for (int i = threadIdx.x; i < PER * TW; i += BN_THREADS) {
@@ -284,10 +330,15 @@ template <int NS, int N, int LG> __device__ __forceinline__ void bn_cluster_sums
 #pragma unroll
         for (uint32_t r = 0; r < 8; r++) a += p[r];
         tot[i] = a;
+        if (NS == 1) finish(tot + i);                  // the thread that holds the sum
     }
     __syncthreads();
+    if (NS > 1) {
+        if (threadIdx.x < TW) finish(tot + threadIdx.x);
+        __syncthreads();
+    }
 #pragma unroll
-    for (int s = 0; s < NS; s++) v[s] = lanes_from_smem<N>(tot + s * TW + lg * N);
+    for (int s = 0; s < F::FACTORS; s++) v[s] = lanes_from_smem<N>(tot + s * TW + lg * N);
 }
 
 template <typename T, int LG, int NV>
@@ -306,35 +357,44 @@ block_norm_cluster_kernel(T *x2, T *y, const T *x, const T *f, const float *__re
     const float inv_c = 1.0f / (float)sh.C;
     if (gate) gate += (size_t)b * sh.gate_stride;
 
+    // channels c, c + R, ... of this thread: n of them
+    const int n = !active || c >= end ? 0 : (end - c + R - 1) / R;
     Raw<T, VEC> rf[NV], rx[NV];
+    float k1[NV], k2[NV];                             // alpha * gate * w_post, w_pre
     dep_sync();
 #pragma unroll
-    for (int k = 0; k < NV; k++) if (active && c + k * R < end) { rf[k].load_stream(f + base + k * step); rx[k].load_stream(x + base + k * step); }
+    for (int k = 0; k < NV; k++) if (k < n) { rf[k].load_stream(f + base + k * step); rx[k].load_stream(x + base + k * step); }
+#pragma unroll
+    for (int k = 0; k < NV; k++)
+        if (k < n) {
+            k1[k] = sh.alpha * (gate ? __ldg(gate + c + k * R) : 1.0f) * (w_post ? __ldg(w_post + c + k * R) : 1.0f);
+            k2[k] = __ldg(w_pre + c + k * R);
+        }
+    const BnRms<TW> rms = {inv_c, sh.eps};
     V<VEC> ss[1] = {V<VEC>::splat(0.0f)}, r = V<VEC>::splat(1.0f);
     if (w_post) {
 #pragma unroll
-        for (int k = 0; k < NV; k++) if (active && c + k * R < end) { const V<VEC> v = rf[k].get(); ss[0] = vfma(v, v, ss[0]); }
-        bn_cluster_sums<1, VEC, LG>(ss, red, mine[0], tot);
-        r = bn_rms(ss[0], inv_c, sh.eps);
+        for (int k = 0; k < NV; k++) if (k < n) { const V<VEC> v = rf[k].get(); ss[0] = vfma(v, v, ss[0]); }
+        bn_cluster_sums<1, VEC, LG>(ss, red, mine[0], tot, rms);
+        r = ss[0];
         ss[0] = V<VEC>::splat(0.0f);
     }
 #pragma unroll
     for (int k = 0; k < NV; k++)
-        if (active && c + k * R < end) {
-            const int ch = c + k * R;
-            const float s = sh.alpha * (gate ? __ldg(gate + ch) : 1.0f) * (w_post ? __ldg(w_post + ch) : 1.0f);
-            rx[k].put(vfma_s(vmul(rf[k].get(), r), s, rx[k].get()));
-            rx[k].store_stream(x2 + base + k * step);
-            const V<VEC> v = rx[k].get();
+        if (k < n) {
+            rx[k].put(vfma_s(vmul(rf[k].get(), r), k1[k], rx[k].get()));
+            const V<VEC> v = rx[k].get();             // as it is stored
             ss[0] = vfma(v, v, ss[0]);
         }
-    bn_cluster_sums<1, VEC, LG>(ss, red, mine[1], tot);
-    bn_cluster_arrive();                              // this block has read its peers' sums
-    r = bn_rms(ss[0], inv_c, sh.eps);
+    bn_cluster_sums<1, VEC, LG>(ss, red, mine[1], tot, rms);
+    bn_cluster_leave();                               // this block has read its peers' sums
+    r = ss[0];
+    // both results only now: a store before the exchange would have to land before its barrier opens
 #pragma unroll
     for (int k = 0; k < NV; k++)
-        if (active && c + k * R < end) {
-            rx[k].put(vscale(vmul(rx[k].get(), r), __ldg(w_pre + c + k * R)));
+        if (k < n) {
+            rx[k].store_stream(x2 + base + k * step);
+            rx[k].put(vscale(vmul(rx[k].get(), r), k2[k]));
             rx[k].store_stream(y + base + k * step);
         }
     bn_cluster_wait();                                // no block leaves while a peer may still read its sums
@@ -363,15 +423,24 @@ block_norm_bwd_cluster_kernel(T *dx, T *df, float *__restrict__ partial, const T
     auto entry = [&](int tensor, int k) { return strip + (tensor * NV + k) * BN_THREADS + threadIdx.x; };
     auto get = [&](int tensor, int k) { Raw<T, VEC> r; r.v = *entry(tensor, k); return r.get(); };
 
+    const int n = !active || c >= end ? 0 : (end - c + R - 1) / R;
+    float k1[NV], k2[NV];                                // gate * w_post, w_pre
     dep_sync();
 #pragma unroll
     for (int k = 0; k < NV; k++)
-        if (active && c + k * R < end) {
+        if (k < n) {
             const size_t at = base + k * step;
             bn_copy16(entry(0, k), x2 + at);
             bn_copy16(entry(1, k), dy + at);
             bn_copy16(entry(2, k), f + at);
             if (dx2) bn_copy16(entry(3, k), dx2 + at);
+            else *entry(3, k) = make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+    for (int k = 0; k < NV; k++)
+        if (k < n) {
+            k1[k] = (gate ? __ldg(gate + c + k * R) : 1.0f) * (w_post ? __ldg(w_post + c + k * R) : 1.0f);
+            k2[k] = __ldg(w_pre + c + k * R);
         }
     asm volatile("cp.async.wait_all;" ::: "memory");      // a thread reads back what it copied itself
     V<VEC> s[6];
@@ -379,44 +448,62 @@ block_norm_bwd_cluster_kernel(T *dx, T *df, float *__restrict__ partial, const T
     for (int i = 0; i < 6; i++) s[i] = V<VEC>::splat(0.0f);
 #pragma unroll
     for (int k = 0; k < NV; k++)
-        if (active && c + k * R < end) {
-            const int ch = c + k * R;
-            const V<VEC> vx = get(0, k), va = vscale(get(1, k), __ldg(w_pre + ch));
+        if (k < n) {
+            const V<VEC> vx = get(0, k), va = vscale(get(1, k), k2[k]);
             s[0] = vfma(vx, vx, s[0]);
             s[1] = vfma(va, vx, s[1]);
             if (w_post) {
-                const V<VEC> vf = get(2, k), vq = vscale(vf, (gate ? __ldg(gate + ch) : 1.0f) * __ldg(w_post + ch));
+                const V<VEC> vf = get(2, k), vq = vscale(vf, k1[k]);
                 s[2] = vfma(vf, vf, s[2]);
-                if (dx2) s[3] = vfma(vq, get(3, k), s[3]);
+                s[3] = vfma(vq, get(3, k), s[3]);
                 s[4] = vfma(vq, va, s[4]);
                 s[5] = vfma(vq, vx, s[5]);
             }
         }
-    bn_cluster_sums<6, VEC, LG>(s, red, mine, tot);
-    bn_cluster_arrive();
-    const BnFactors<VEC> o = bn_factors<VEC>(s, w_post != nullptr, inv_c, sh.alpha, sh.eps);
-    const V<VEC> nk = vscale(o.k, -1.0f), nj = vscale(o.j, -1.0f);
+    bn_cluster_sums<6, VEC, LG>(s, red, mine, tot, BnBwd<TW>{inv_c, sh.eps, sh.alpha, w_post != nullptr});
+    bn_cluster_leave();
+    const V<VEC> r2 = s[0], nk = s[1], rms_f = s[2], nj = s[3];
     float2 *prow = reinterpret_cast<float2 *>(partial) + (size_t)tile * sh.C;
+    float sums[2 * NV];                                   // per row: dy x2 r2, f r_f G, over the thread's tokens
 #pragma unroll
     for (int k = 0; k < NV; k++) {
-        const int ch = c + k * R;
-        float sum_q = 0.0f, sum_p = 0.0f;
-        if (active && ch < end) {
+        sums[2 * k] = sums[2 * k + 1] = 0.0f;
+        if (k < n) {
             const V<VEC> vx = get(0, k), vy = get(1, k), vf = get(2, k);
-            V<VEC> G = vfma(vscale(vy, __ldg(w_pre + ch)), o.r2, vmul(nk, vx));
-            if (dx2) G = vadd(G, get(3, k));
-            sum_q = vmul(vy, vmul(vx, o.r2)).hsum();
-            sum_p = vmul(vmul(vf, o.rf), G).hsum();
+            const V<VEC> G = vfma(vscale(vy, k2[k]), r2, vfma(nk, vx, get(3, k)));
+            sums[2 * k] = vmul(vy, vmul(vx, r2)).hsum();
+            const V<VEC> u = vmul(vf, rms_f);
+            sums[2 * k + 1] = vmul(u, G).hsum();
             Raw<T, VEC> out;
             out.put(G);
             out.store_stream(dx + base + k * step);
-            const float gw = (gate ? __ldg(gate + ch) : 1.0f) * (w_post ? __ldg(w_post + ch) : 1.0f);
-            out.put(vfma(vscale(G, sh.alpha * gw), o.rf, vmul(nj, vf)));
+            out.put(vfma(vscale(G, sh.alpha * k1[k]), rms_f, vmul(nj, vf)));
             out.store_stream(df + base + k * step);
         }
-        sum_q = bn_row_sum<LG>(sum_q);
-        if (want_p) sum_p = bn_row_sum<LG>(sum_p);
-        if (lg == 0 && ch < end) prow[ch] = make_float2(sum_q, sum_p);
+    }
+    // over the lanes of a row: each of the first steps halves the values, a lane ends with one or two of them
+#pragma unroll
+    for (int off = LG / 2, left = 2 * NV; off > 0; off >>= 1) {
+        const bool up = lg & off;
+        if (left > 1) {
+            left >>= 1;
+#pragma unroll
+            for (int i = 0; i < NV; i++)
+                if (i < left) {
+                    const float other = __shfl_xor_sync(0xffffffffu, up ? sums[i] : sums[i + left], off);
+                    sums[i] = (up ? sums[i + left] : sums[i]) + other;
+                }
+        }
+    }
+    constexpr int HELD = 2 * NV / LG;                     // values first .. first + HELD - 1 in the order above
+    static_assert(HELD >= 1, "every step halves");
+    int first = 0;
+#pragma unroll
+    for (int off = LG / 2, half = NV; off > 0; off >>= 1, half >>= 1) first += lg & off ? half : 0;
+#pragma unroll
+    for (int i = 0; i < HELD; i++) {
+        const int row = (first + i) / 2, ch = c + row * R;
+        if (ch < end) reinterpret_cast<float *>(prow + ch)[(first + i) & 1] = sums[i];
     }
     bn_cluster_wait();
 }

@@ -15,7 +15,7 @@ _ID = {torch.int32: _l.ID_I32, torch.uint16: _l.ID_U16, torch.int16: _l.ID_U16}
 
 
 def _stream():
-    return torch.cuda.current_stream().cuda_stream
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())     # current_stream() builds an object first
 
 
 def _p(t):
@@ -38,16 +38,27 @@ def _bcs(t):
     raise ValueError("expected [B, C, S] or [C, S]")
 
 
-def _same_device(*tensors):
-    """Refuses tensors that are not on the current CUDA device (the stream of the call belongs to it)."""
+def _ptrs(*tensors):
+    """Addresses of contiguous tensors on the current CUDA device (the stream of the call belongs to it); None stays None."""
+    current, out = -1, []
     for t in tensors:
-        if t is not None and (not t.is_cuda or t.device.index != torch.cuda.current_device()):
+        if t is None:
+            out.append(None)
+            continue
+        at = t.get_device()                              # -1 on the CPU
+        if current < 0:
+            current = torch._C._cuda_getDevice() if at >= 0 else -2
+        if at != current:
             raise ValueError(f"expected a tensor on the current CUDA device, got one on {t.device}")
+        if not t.is_contiguous():
+            raise ValueError("expected a contiguous CUDA tensor")
+        out.append(t.data_ptr())
+    return out
 
 
 def _like(name, t, shape, dtype):
     """Checks an argument's shape and element type; None passes."""
-    if t is not None and (tuple(t.shape) != tuple(shape) or t.dtype != dtype):
+    if t is not None and (t.shape != shape or t.dtype != dtype):
         raise ValueError(f"{name}: expected {dtype} {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
 
 
@@ -106,9 +117,8 @@ def block_norm(x, f, w_pre, w_post=None, gate=None, alpha=1.0, eps=1e-5, x2=None
     B, Cn, S, per_seq = _block_norm_args(x, f, w_pre, w_post, gate)
     _like("x2", x2, x.shape, x.dtype)
     _like("y", y, x.shape, x.dtype)
-    _same_device(x, f, w_pre, w_post, gate, x2, y)
-    _l.check(_l.load().ane_cuda_block_norm_dev(_stream(), _dt(x), B, Cn, S, _p(x2), _p(y), _p(x), _p(f), _p(w_post), _p(gate), per_seq,
-                                              _p(w_pre), alpha, eps))
+    x2p, yp, xp, fp, wp, gp, vp = _ptrs(x2, y, x, f, w_post, gate, w_pre)
+    _l.check(_l.load().ane_cuda_block_norm_dev(_stream(), _dt(x), B, Cn, S, x2p, yp, xp, fp, wp, gp, per_seq, vp, alpha, eps))
     return x2, y
 
 
@@ -126,9 +136,8 @@ def block_norm_bwd(dy, x2, f, w_pre, dw_pre, w_post=None, dw_post=None, gate=Non
     if (dw_post is not None and w_post is None) or (dgate is not None and gate is None):
         raise ValueError("dw_post needs w_post and dgate needs gate")
     _like("dgate", dgate, () if gate is None else gate.shape, torch.float32)
-    _same_device(dy, x2, f, w_pre, dw_pre, w_post, dw_post, gate, dgate, dx2, dx, df)
-    _l.check(_l.load().ane_cuda_block_norm_bwd_dev(_stream(), _dt(x2), B, Cn, S, _p(dx), _p(df), _p(dw_post), _p(dgate), _p(dw_pre), _p(dy),
-                                                  _p(dx2), _p(x2), _p(f), _p(w_post), _p(gate), per_seq, _p(w_pre), alpha, eps))
+    *out, gp, vp = _ptrs(dx, df, dw_post, dgate, dw_pre, dy, dx2, x2, f, w_post, gate, w_pre)
+    _l.check(_l.load().ane_cuda_block_norm_bwd_dev(_stream(), _dt(x2), B, Cn, S, *out, gp, per_seq, vp, alpha, eps))
     return dx, df
 
 
@@ -258,12 +267,11 @@ def linear_cross_entropy(x, table, targets, d_table=None, grad_scale=1.0, dx=Non
     _like("d_table", d_table, (V, D), torch.float32)
     _like("loss_tok", loss_tok, targets.shape, torch.float32)
     _like("dx", dx, x.shape, x.dtype)
-    _same_device(x, table, targets, d_table, dx, loss_tok)
     if grad and dx is None:
         dx = torch.empty_like(x)
     loss = torch.empty(B, dtype=torch.float32, device=x.device)
-    _l.check(_l.load().ane_cuda_linear_cross_entropy_dev(_stream(), _dt(x), _ID[targets.dtype], B, D, V, S, _p(loss), _p(loss_tok), _p(dx), _p(d_table),
-                                                        _p(x), _p(table), _p(targets), grad_scale))
+    at = _ptrs(loss, loss_tok, dx, d_table, x, table, targets)
+    _l.check(_l.load().ane_cuda_linear_cross_entropy_dev(_stream(), _dt(x), _ID[targets.dtype], B, D, V, S, *at, grad_scale))
     return loss, dx
 
 
@@ -318,10 +326,8 @@ class AdamTensors:
         self.items = (_l.AdamItem * count)()
         self.count, self.wd = count, wd
         self.tensors = (list(w), list(g), list(m), list(v), m_scale and list(m_scale), v_scale and list(v_scale), copy and list(copy))
-        for ts in self.tensors:
-            _same_device(*(ts or ()))
         for k in range(count):
-            at = [None if ts is None else _p(ts[k]) for ts in self.tensors]
+            at = _ptrs(*(None if ts is None else ts[k] for ts in self.tensors))
             self.items[k] = _l.AdamItem(w[k].numel(), *at, wd[k], 0)
 
 
@@ -329,9 +335,9 @@ def adam_multi(tensors, t, lr, b1, b2, eps, gscale=1.0, clip=None, seed=0, dynam
     """One Adam / AdamW step over an ``AdamTensors`` list.  With 8-bit moments pass another ``seed`` every step: it decides
     which way each stored moment is rounded."""
     _like("clip", clip, (1,), torch.float32)
-    _same_device(clip)
+    clip, = _ptrs(clip)
     _l.check(_l.load().ane_cuda_adam_multi_dev(_stream(), _l.ADAM_STATE_Q8 if tensors.q8 else _l.ADAM_STATE_F32, tensors.g_dtype, tensors.copy_dtype,
-                                              tensors.count, tensors.items, t, lr, b1, b2, eps, gscale, _p(clip), seed & 0xFFFFFFFF,
+                                              tensors.count, tensors.items, t, lr, b1, b2, eps, gscale, clip, seed & 0xFFFFFFFF,
                                               _l.ADAM_DYNAMIC if dynamic else _l.ADAM_STORIES))
 
 
@@ -341,8 +347,8 @@ def adam_state_unpack(codes, scales, second=False, out=None):
     _like("codes", codes, codes.shape, torch.uint8)
     _like("scales", scales, (-(-codes.numel() // ADAM_BLOCK),), torch.float32)
     _like("out", out, codes.shape, torch.float32)
-    _same_device(codes, scales, out)
-    _l.check(_l.load().ane_cuda_adam_state_unpack_dev(_stream(), codes.numel(), _p(out), _p(codes), _p(scales), int(second)))
+    at = _ptrs(out, codes, scales)
+    _l.check(_l.load().ane_cuda_adam_state_unpack_dev(_stream(), codes.numel(), *at, int(second)))
     return out
 
 
@@ -354,8 +360,8 @@ def adam_state_pack(value, second=False, seed=0, codes=None, scales=None):
     _like("value", value, value.shape, torch.float32)
     _like("codes", codes, value.shape, torch.uint8)
     _like("scales", scales, blocks, torch.float32)
-    _same_device(value, codes, scales)
-    _l.check(_l.load().ane_cuda_adam_state_pack_dev(_stream(), value.numel(), _p(codes), _p(scales), _p(value), int(second), seed & 0xFFFFFFFF))
+    at = _ptrs(codes, scales, value)
+    _l.check(_l.load().ane_cuda_adam_state_pack_dev(_stream(), value.numel(), *at, int(second), seed & 0xFFFFFFFF))
     return codes, scales
 
 
