@@ -288,8 +288,8 @@ template <int N> struct BnFold<N, 32> {
 // NS per-token sums over the cluster, the warps' parts three sums at a time (`red` holds [3][warps][TW]: three blocks fit an SM
 // then).  `mine` [NS][TW] is read by the other blocks until the next cluster barrier behind this call, so it is not reused
 // before that.
-template <int NS, int N, int LG, typename F> __device__ __forceinline__ void bn_cluster_sums(V<N> (&v)[NS], float *red, float *mine, float *tot, F finish) {
-    constexpr int TW = N * LG, PER = NS < 3 ? NS : 3;
+template <int NS, int N, int LG, int THREADS, typename F> __device__ __forceinline__ void bn_cluster_sums(V<N> (&v)[NS], float *red, float *mine, float *tot, F finish) {
+    constexpr int TW = N * LG, PER = NS < 3 ? NS : 3, WARPS = THREADS / 32;
     const int lg = threadIdx.x % LG, warp = threadIdx.x / 32, lane = threadIdx.x & 31;
 #pragma unroll
     for (int s0 = 0; s0 < NS; s0 += PER) {
@@ -303,32 +303,45 @@ template <int NS, int N, int LG, typename F> __device__ __forceinline__ void bn_
         BnFold<PER * N, LG>::run(a, lane, first, writer);
         if (s0) __syncthreads();
         constexpr int LEFT = BnFold<PER * N, LG>::LEFT;
-        static_assert(LEFT % 4 == 0, "whole 16-byte words");
-        if (writer) {
+        static_assert(N == 1 || LEFT % 4 == 0, "whole 16-byte words");
+        if constexpr (N == 1) {
+#pragma unroll
+            for (int s = 0; s < PER; s++) red[(s * WARPS + warp) * TW + lg] = a[s];
+        } else if (writer) {
 #pragma unroll
             for (int i = 0; i < LEFT; i += 4) {
                 const int at = first + i;                         // value at % N of sum at / N
-                *reinterpret_cast<float4 *>(red + ((at / N) * BN_WARPS + warp) * TW + lg * N + at % N) = make_float4(a[i], a[i + 1], a[i + 2], a[i + 3]);
+                *reinterpret_cast<float4 *>(red + ((at / N) * WARPS + warp) * TW + lg * N + at % N) = make_float4(a[i], a[i + 1], a[i + 2], a[i + 3]);
             }
         }
         __syncthreads();
-        for (int i = threadIdx.x; i < PER * TW; i += BN_THREADS) {
+        for (int i = threadIdx.x; i < PER * TW; i += THREADS) {
             const int s = i / TW, t = i % TW;
             float a = 0.0f;
 #pragma unroll
-            for (int w = 0; w < BN_WARPS; w++) a += red[(s * BN_WARPS + w) * TW + t];
+            for (int w = 0; w < WARPS; w++) a += red[(s * WARPS + w) * TW + t];
             mine[s0 * TW + i] = a;
         }
     }
-    bn_cluster_arrive();
-    bn_cluster_wait();
     const uint32_t blocks = bn_size();
-    for (int i = threadIdx.x; i < NS * TW; i += BN_THREADS) {
-        float p[8], a = 0.0f;
+    if (blocks > 1) {
+        bn_cluster_arrive();
+        bn_cluster_wait();
+    } else if (NS > 1) {
+        __syncthreads();
+    }
+    for (int i = threadIdx.x; i < NS * TW; i += THREADS) {     // for one block a thread's own entries again
+        float a;
+        if (blocks > 1) {
+            float p[8];
 #pragma unroll
-        for (uint32_t r = 0; r < 8; r++) p[r] = r < blocks ? bn_peer(mine + i, r) : 0.0f;
+            for (uint32_t r = 0; r < 8; r++) p[r] = r < blocks ? bn_peer(mine + i, r) : 0.0f;
+            a = 0.0f;
 #pragma unroll
-        for (uint32_t r = 0; r < 8; r++) a += p[r];
+            for (uint32_t r = 0; r < 8; r++) a += p[r];
+        } else {
+            a = mine[i];
+        }
         tot[i] = a;
         if (NS == 1) finish(tot + i);                  // the thread that holds the sum
     }
@@ -341,139 +354,149 @@ template <int NS, int N, int LG, typename F> __device__ __forceinline__ void bn_
     for (int s = 0; s < F::FACTORS; s++) v[s] = lanes_from_smem<N>(tot + s * TW + lg * N);
 }
 
-template <typename T, int LG, int NV>
-__global__ void __launch_bounds__(BN_THREADS, NV <= 4 ? 4 : 2)
+__device__ __forceinline__ void bn_copy16(void *dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void bn_copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+// A thread's own vectors of NT tensors, NV rows each: the first SM tensors in shared memory, filled by asynchronous copies that
+// nobody else has to know of, the others in registers.
+template <typename T, int VEC, int NT, int SM, int NV, int THREADS> struct BnStrip {
+    static constexpr size_t BYTES = (size_t)SM * NV * THREADS * 16;
+    uint4 *at;                                            // this thread's first entry
+    Raw<T, VEC> r[NT - SM > 0 ? NT - SM : 1][NV];
+    __device__ __forceinline__ BnStrip(uint4 *strip) : at(strip + threadIdx.x) {}
+    __device__ __forceinline__ void fill(int tensor, int k, const T *p) {
+        if (tensor < SM) bn_copy16(at + (tensor * NV + k) * THREADS, p); else r[tensor - SM][k].load_stream(p);
+    }
+    __device__ __forceinline__ void zero(int tensor, int k) {
+        if (tensor < SM) at[(tensor * NV + k) * THREADS] = make_uint4(0, 0, 0, 0);
+        else { V<VEC> z = V<VEC>::splat(0.0f); r[tensor - SM][k].put(z); }
+    }
+    __device__ __forceinline__ void done() { if (SM) bn_copies_done(); }
+    __device__ __forceinline__ V<VEC> get(int tensor, int k) const {
+        if constexpr (SM > 0) {
+            if (tensor < SM) { Raw<T, VEC> q; q.v = at[(tensor * NV + k) * THREADS]; return q.get(); }
+        }
+        return r[tensor - SM][k].get();
+    }
+};
+
+// A cluster per token tile.  LG lanes of VEC tokens per row, NV rows per thread; x2 takes x's place in the strip.
+template <typename T, int VEC, int LG, int NV, int THREADS, int SM>
+__global__ void __launch_bounds__(THREADS, THREADS == 512 ? (NV <= 8 ? 2 : 1) : NV * VEC <= 32 ? 4 : 2)
 block_norm_cluster_kernel(T *x2, T *y, const T *x, const T *f, const float *__restrict__ w_post, const float *__restrict__ gate,
                           const float *__restrict__ w_pre, BnShape sh, int rows) {
-    constexpr int VEC = Elt<T>::VEC, R = BN_THREADS / LG, TW = LG * VEC;
-    __shared__ __align__(16) float red[BN_WARPS * TW], mine[2][TW], tot[TW];
-    const int tile = blockIdx.x / bn_size(), c0 = (int)bn_rank() * rows;
-    const int b = tile / sh.tiles_per_seq;
-    const int lg = threadIdx.x % LG, c = c0 + threadIdx.x / LG;
+    constexpr int R = THREADS / LG, TW = LG * VEC;
+    extern __shared__ __align__(16) uint4 strips[];
+    __shared__ __align__(16) float red[THREADS / 32 * TW], mine[2][TW], tot[TW];
+    const int tile = blockIdx.x / bn_size(), c0 = (int)bn_rank() * rows, c = c0 + threadIdx.x / LG;
     const int end = c0 + rows < sh.C ? c0 + rows : sh.C;
-    const int t = (tile % sh.tiles_per_seq) * TW + lg * VEC;
-    const bool active = t < sh.S;
+    const int b = tile / sh.tiles_per_seq, t = (tile - b * sh.tiles_per_seq) * TW + (int)(threadIdx.x % LG) * VEC;
+    const int n = t >= sh.S || c >= end ? 0 : (end - c + R - 1) / R;      // rows c, c + R, ... of this thread
     const size_t base = ((size_t)b * sh.C + c) * sh.S + t, step = (size_t)R * sh.S;
-    const float inv_c = 1.0f / (float)sh.C;
+    const BnRms<TW> rms = {1.0f / (float)sh.C, sh.eps};
+    BnStrip<T, VEC, 2, SM, NV, THREADS> strip(strips);    // x, f
     if (gate) gate += (size_t)b * sh.gate_stride;
-
-    // channels c, c + R, ... of this thread: n of them
-    const int n = !active || c >= end ? 0 : (end - c + R - 1) / R;
-    Raw<T, VEC> rf[NV], rx[NV];
-    float k1[NV], k2[NV];                             // alpha * gate * w_post, w_pre
     dep_sync();
 #pragma unroll
-    for (int k = 0; k < NV; k++) if (k < n) { rf[k].load_stream(f + base + k * step); rx[k].load_stream(x + base + k * step); }
+    for (int k = 0; k < NV; k++) if (k < n) strip.fill(1, k, f + base + k * step);
 #pragma unroll
-    for (int k = 0; k < NV; k++)
-        if (k < n) {
-            k1[k] = sh.alpha * (gate ? __ldg(gate + c + k * R) : 1.0f) * (w_post ? __ldg(w_post + c + k * R) : 1.0f);
-            k2[k] = __ldg(w_pre + c + k * R);
-        }
-    const BnRms<TW> rms = {inv_c, sh.eps};
+    for (int k = 0; k < NV; k++) if (k < n) strip.fill(0, k, x + base + k * step);
+    strip.done();
     V<VEC> ss[1] = {V<VEC>::splat(0.0f)}, r = V<VEC>::splat(1.0f);
     if (w_post) {
 #pragma unroll
-        for (int k = 0; k < NV; k++) if (k < n) { const V<VEC> v = rf[k].get(); ss[0] = vfma(v, v, ss[0]); }
-        bn_cluster_sums<1, VEC, LG>(ss, red, mine[0], tot, rms);
+        for (int k = 0; k < NV; k++) if (k < n) { const V<VEC> v = strip.get(1, k); ss[0] = vfma(v, v, ss[0]); }
+        bn_cluster_sums<1, VEC, LG, THREADS>(ss, red, mine[0], tot, rms);
         r = ss[0];
         ss[0] = V<VEC>::splat(0.0f);
     }
+    Raw<T, VEC> z[NV];                                    // x2 as it is stored
 #pragma unroll
     for (int k = 0; k < NV; k++)
         if (k < n) {
-            rx[k].put(vfma_s(vmul(rf[k].get(), r), k1[k], rx[k].get()));
-            const V<VEC> v = rx[k].get();             // as it is stored
+            const float k1 = sh.alpha * (gate ? __ldg(gate + c + k * R) : 1.0f) * (w_post ? __ldg(w_post + c + k * R) : 1.0f);
+            z[k].put(vfma_s(vmul(strip.get(1, k), r), k1, strip.get(0, k)));
+            const V<VEC> v = z[k].get();
             ss[0] = vfma(v, v, ss[0]);
         }
-    bn_cluster_sums<1, VEC, LG>(ss, red, mine[1], tot, rms);
-    bn_cluster_leave();                               // this block has read its peers' sums
-    r = ss[0];
+    bn_cluster_sums<1, VEC, LG, THREADS>(ss, red, mine[1], tot, rms);
+    bn_cluster_leave();                                   // this block has read its peers' sums
     // both results only now: a store before the exchange would have to land before its barrier opens
 #pragma unroll
     for (int k = 0; k < NV; k++)
         if (k < n) {
-            rx[k].store_stream(x2 + base + k * step);
-            rx[k].put(vscale(vmul(rx[k].get(), r), k2[k]));
-            rx[k].store_stream(y + base + k * step);
+            z[k].store_stream(x2 + base + k * step);
+            z[k].put(vscale(vmul(z[k].get(), ss[0]), __ldg(w_pre + c + k * R)));
+            z[k].store_stream(y + base + k * step);
         }
-    bn_cluster_wait();                                // no block leaves while a peer may still read its sums
+    bn_cluster_wait();                                    // no block leaves while a peer may still read its sums
 }
 
-__device__ __forceinline__ void bn_copy16(void *dst, const void *src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
-}
-
-template <typename T, int LG, int NV>
-__global__ void __launch_bounds__(BN_THREADS, NV <= 4 ? 3 : 1)
+template <typename T, int VEC, int LG, int NV, int THREADS, int SM>
+__global__ void __launch_bounds__(THREADS, THREADS == 512 ? 1 : VEC == 1 ? 2 : NV <= 4 ? 3 : 1)
 block_norm_bwd_cluster_kernel(T *dx, T *df, float *__restrict__ partial, const T *dy, const T *dx2, const T *x2, const T *f,
                               const float *__restrict__ w_post, const float *__restrict__ gate, const float *__restrict__ w_pre, BnShape sh, int rows) {
-    constexpr int VEC = Elt<T>::VEC, R = BN_THREADS / LG, TW = LG * VEC;
-    extern __shared__ __align__(16) uint4 strip[];       // [4 tensors][NV][threads]: each thread's own vectors
-    __shared__ __align__(16) float red[3 * BN_WARPS * TW], mine[6 * TW], tot[6 * TW];
-    const int tile = blockIdx.x / bn_size(), c0 = (int)bn_rank() * rows;
-    const int b = tile / sh.tiles_per_seq;
-    const int lg = threadIdx.x % LG, c = c0 + threadIdx.x / LG;
-    const int end = c0 + rows < sh.C ? c0 + rows : sh.C;
-    const int t = (tile % sh.tiles_per_seq) * TW + lg * VEC;
-    const bool active = t < sh.S, want_p = w_post || gate;
+    constexpr int R = THREADS / LG, TW = LG * VEC;
+    extern __shared__ __align__(16) uint4 strips[];
+    __shared__ __align__(16) float red[3 * (THREADS / 32) * TW], mine[6 * TW], tot[6 * TW];
+    const int tile = blockIdx.x / bn_size(), c0 = (int)bn_rank() * rows, c = c0 + threadIdx.x / LG;
+    const int end = c0 + rows < sh.C ? c0 + rows : sh.C, lg = threadIdx.x % LG;
+    const int b = tile / sh.tiles_per_seq, t = (tile - b * sh.tiles_per_seq) * TW + lg * VEC;
+    const int n = t >= sh.S || c >= end ? 0 : (end - c + R - 1) / R;
     const size_t base = ((size_t)b * sh.C + c) * sh.S + t, step = (size_t)R * sh.S;
-    const float inv_c = 1.0f / (float)sh.C;
+    const bool want_p = w_post || gate;
+    const BnBwd<TW> factors = {1.0f / (float)sh.C, sh.eps, sh.alpha, w_post != nullptr};
+    BnStrip<T, VEC, 4, SM, NV, THREADS> strip(strips);    // x2, dy, f, dx2
     if (gate) gate += (size_t)b * sh.gate_stride;
-    auto entry = [&](int tensor, int k) { return strip + (tensor * NV + k) * BN_THREADS + threadIdx.x; };
-    auto get = [&](int tensor, int k) { Raw<T, VEC> r; r.v = *entry(tensor, k); return r.get(); };
-
-    const int n = !active || c >= end ? 0 : (end - c + R - 1) / R;
-    float k1[NV], k2[NV];                                // gate * w_post, w_pre
     dep_sync();
 #pragma unroll
     for (int k = 0; k < NV; k++)
         if (k < n) {
-            const size_t at = base + k * step;
-            bn_copy16(entry(0, k), x2 + at);
-            bn_copy16(entry(1, k), dy + at);
-            bn_copy16(entry(2, k), f + at);
-            if (dx2) bn_copy16(entry(3, k), dx2 + at);
-            else *entry(3, k) = make_uint4(0, 0, 0, 0);
+            const size_t i = base + k * step;
+            if (dx2) strip.fill(3, k, dx2 + i); else strip.zero(3, k);
+            strip.fill(0, k, x2 + i);
+            strip.fill(1, k, dy + i);
+            strip.fill(2, k, f + i);
         }
+    float k1[NV], k2[NV];                                 // gate * w_post, w_pre
 #pragma unroll
     for (int k = 0; k < NV; k++)
         if (k < n) {
             k1[k] = (gate ? __ldg(gate + c + k * R) : 1.0f) * (w_post ? __ldg(w_post + c + k * R) : 1.0f);
             k2[k] = __ldg(w_pre + c + k * R);
         }
-    asm volatile("cp.async.wait_all;" ::: "memory");      // a thread reads back what it copied itself
+    strip.done();
     V<VEC> s[6];
 #pragma unroll
     for (int i = 0; i < 6; i++) s[i] = V<VEC>::splat(0.0f);
 #pragma unroll
     for (int k = 0; k < NV; k++)
         if (k < n) {
-            const V<VEC> vx = get(0, k), va = vscale(get(1, k), k2[k]);
+            const V<VEC> vx = strip.get(0, k), va = vscale(strip.get(1, k), k2[k]);
             s[0] = vfma(vx, vx, s[0]);
             s[1] = vfma(va, vx, s[1]);
             if (w_post) {
-                const V<VEC> vf = get(2, k), vq = vscale(vf, k1[k]);
+                const V<VEC> vf = strip.get(2, k), vq = vscale(vf, k1[k]);
                 s[2] = vfma(vf, vf, s[2]);
-                s[3] = vfma(vq, get(3, k), s[3]);
+                s[3] = vfma(vq, strip.get(3, k), s[3]);
                 s[4] = vfma(vq, va, s[4]);
                 s[5] = vfma(vq, vx, s[5]);
             }
         }
-    bn_cluster_sums<6, VEC, LG>(s, red, mine, tot, BnBwd<TW>{inv_c, sh.eps, sh.alpha, w_post != nullptr});
+    bn_cluster_sums<6, VEC, LG, THREADS>(s, red, mine, tot, factors);
     bn_cluster_leave();
     const V<VEC> r2 = s[0], nk = s[1], rms_f = s[2], nj = s[3];
-    float2 *prow = reinterpret_cast<float2 *>(partial) + (size_t)tile * sh.C;
     float sums[2 * NV];                                   // per row: dy x2 r2, f r_f G, over the thread's tokens
 #pragma unroll
     for (int k = 0; k < NV; k++) {
         sums[2 * k] = sums[2 * k + 1] = 0.0f;
         if (k < n) {
-            const V<VEC> vx = get(0, k), vy = get(1, k), vf = get(2, k);
-            const V<VEC> G = vfma(vscale(vy, k2[k]), r2, vfma(nk, vx, get(3, k)));
+            const V<VEC> vx = strip.get(0, k), vy = strip.get(1, k), vf = strip.get(2, k);
+            const V<VEC> G = vfma(vscale(vy, k2[k]), r2, vfma(nk, vx, strip.get(3, k)));
             sums[2 * k] = vmul(vy, vmul(vx, r2)).hsum();
-            const V<VEC> u = vmul(vf, rms_f);
-            sums[2 * k + 1] = vmul(u, G).hsum();
+            sums[2 * k + 1] = vmul(vmul(vf, rms_f), G).hsum();
             Raw<T, VEC> out;
             out.put(G);
             out.store_stream(dx + base + k * step);
@@ -481,29 +504,26 @@ block_norm_bwd_cluster_kernel(T *dx, T *df, float *__restrict__ partial, const T
             out.store_stream(df + base + k * step);
         }
     }
-    // over the lanes of a row: each of the first steps halves the values, a lane ends with one or two of them
-#pragma unroll
-    for (int off = LG / 2, left = 2 * NV; off > 0; off >>= 1) {
-        const bool up = lg & off;
-        if (left > 1) {
-            left >>= 1;
-#pragma unroll
-            for (int i = 0; i < NV; i++)
-                if (i < left) {
-                    const float other = __shfl_xor_sync(0xffffffffu, up ? sums[i] : sums[i + left], off);
-                    sums[i] = (up ? sums[i + left] : sums[i]) + other;
-                }
-        }
-    }
-    constexpr int HELD = 2 * NV / LG;                     // values first .. first + HELD - 1 in the order above
+    // over the lanes of a row: each step exchanges halves, a lane ends with HELD of the sums, the first of them `first`
+    constexpr int HELD = 2 * NV / LG;
     static_assert(HELD >= 1, "every step halves");
     int first = 0;
 #pragma unroll
-    for (int off = LG / 2, half = NV; off > 0; off >>= 1, half >>= 1) first += lg & off ? half : 0;
+    for (int off = LG / 2, left = NV; off > 0; off >>= 1, left >>= 1) {
+        const bool up = lg & off;
+#pragma unroll
+        for (int i = 0; i < NV; i++)
+            if (i < left) {
+                const float other = __shfl_xor_sync(0xffffffffu, up ? sums[i] : sums[i + left], off);
+                sums[i] = (up ? sums[i + left] : sums[i]) + other;
+            }
+        first += up ? left : 0;
+    }
+    float *prow = partial + (size_t)tile * sh.C * 2;
 #pragma unroll
     for (int i = 0; i < HELD; i++) {
-        const int row = (first + i) / 2, ch = c + row * R;
-        if (ch < end) reinterpret_cast<float *>(prow + ch)[(first + i) & 1] = sums[i];
+        const int ch = c + (first + i) / 2 * R, p = (first + i) & 1;
+        if (ch < end && (p == 0 || want_p)) prow[2 * (size_t)ch + p] = sums[i];
     }
     bn_cluster_wait();
 }
@@ -584,9 +604,9 @@ static BnSplit bn_split(int C, int rows_most) {
     return {blocks, (C + blocks - 1) / blocks};
 }
 template <typename... KArgs, typename... Args>
-static inline void bn_call(void (*kernel)(KArgs...), dim3 grid, int cluster, size_t smem, cudaStream_t st, Args &&...args) {
+static inline void bn_call(void (*kernel)(KArgs...), dim3 grid, int threads, int cluster, size_t smem, cudaStream_t st, Args &&...args) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid; cfg.blockDim = dim3(BN_THREADS); cfg.dynamicSmemBytes = smem; cfg.stream = st;
+    cfg.gridDim = grid; cfg.blockDim = dim3((unsigned)threads); cfg.dynamicSmemBytes = smem; cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -595,13 +615,37 @@ static inline void bn_call(void (*kernel)(KArgs...), dim3 grid, int cluster, siz
     cfg.attrs = attr; cfg.numAttrs = cluster ? 2 : 1;
     cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);      // the error, if any, is picked up by ANE_LAUNCH_OK
 }
-// Picks lanes per row and rows per thread: 128-byte rows where eight blocks hold the channels, else 64-byte rows.
-template <typename Fn> static int bn_pick_cluster(int C, Fn &&go) {
-    using I4 = std::integral_constant<int, 4>;
-    using I8 = std::integral_constant<int, 8>;
-    if (C <= 1024) return go(I8(), I4(), bn_split(C, BN_THREADS / 8 * 4));
-    if (C <= 2048) return go(I4(), I4(), bn_split(C, BN_THREADS / 4 * 4));
-    return go(I4(), I8(), bn_split(C, BN_THREADS / 4 * 8));
+// The cluster form for a shape, if there is one.
+//   many tiles   512 threads per block; 1024 channels to a block
+//   few tiles    256 threads, up to eight blocks per tile, so that more SMs take part
+//   rows that break 16-byte alignment: element by element, 32 tokens per row, eight blocks per tile
+// -> BN_NONE: none (channels beyond eight blocks, or unaligned sequences so short that most lanes of a row would idle).
+constexpr int BN_NONE = 1;
+template <int V_, int LG_, int NV_, int TH_> struct BnForm { static constexpr int VEC = V_, LG = LG_, NV = NV_, THREADS = TH_; };
+// BIG_LG: lanes per row of the large form (a thread has C / (512 / BIG_LG) rows); BIG_C: channels above which it is used.
+template <typename T, int BIG_LG, int BIG_C, typename Fn> static int bn_pick_cluster(bool vec, int B, int C, int S, Fn &&go) {
+    constexpr int N = Elt<T>::VEC, BR = 512 / BIG_LG;
+    const int knob = tuning("block_norm_cluster", 3);    // 0: none, 1: the small form only, 3: both
+    if (!knob) return BN_NONE;
+    const long long big_tiles = (long long)B * ((S + BIG_LG * N - 1) / (BIG_LG * N));
+    if (vec && C > BIG_C && C <= 4096 && (knob & 2) && big_tiles * ((C + 1023) / 1024) >= 2LL * ctx().sm_count) {
+        if constexpr (BIG_C < 512) {
+            if (C <= 256) return go(BnForm<N, BIG_LG, 256 / BR, 512>(), bn_split(C, 256));
+            if (C <= 512) return go(BnForm<N, BIG_LG, 512 / BR, 512>(), bn_split(C, 512));
+        }
+        return go(BnForm<N, BIG_LG, 1024 / BR, 512>(), bn_split(C, 1024));
+    }
+    if (vec && C <= 1024) return go(BnForm<N, 8, 4, 256>(), bn_split(C, 256 / 8 * 4));
+    if (vec && C <= 2048) return go(BnForm<N, 4, 4, 256>(), bn_split(C, 256 / 4 * 4));
+    if (vec && C <= 4096) return go(BnForm<N, 4, 8, 256>(), bn_split(C, 256 / 4 * 8));
+    if (!vec && S >= 16 && C <= 1024) return go(BnForm<1, 32, 16, 256>(), bn_split(C, 256 / 32 * 16));
+    return BN_NONE;
+}
+// Blocks with more than the default shared memory ask for it once.
+template <typename... KArgs> static int bn_allow(void (*kernel)(KArgs...), size_t smem, bool &ready) {
+    if (!ready && smem) ANE_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    ready = true;
+    return ANE_CUDA_OK;
 }
 
 // LG lanes of VEC tokens per row of a tile for the kernels above.
@@ -634,17 +678,20 @@ int ane_cuda_block_norm_dev(void *stream, ane_dtype dtype, int B, int C, int S, 
     BnShape sh = {B, C, S, 0, 0, gate_per_seq ? C : 0, alpha, eps};
     ANE_DISPATCH_DTYPE(dtype, T, {
         const bool vec = S % Elt<T>::VEC == 0 && aligned16(x2) && aligned16(y) && aligned16(x) && aligned16(f);
-        if (vec && C <= 4096 && tuning("block_norm_cluster", 1)) {
-            bn_pick_cluster(C, [&](auto lg, auto nv, BnSplit sp) {
-                constexpr int LG = decltype(lg)::value, NV = decltype(nv)::value;
-                sh.tiles_per_seq = (S + LG * Elt<T>::VEC - 1) / (LG * Elt<T>::VEC);
-                bn_call(block_norm_cluster_kernel<T, LG, NV>, dim3((unsigned)B * (unsigned)sh.tiles_per_seq * (unsigned)sp.blocks), sp.blocks, 0, st, (T *)x2, (T *)y, (const T *)x,
-                        (const T *)f, w_post, gate, w_pre, sh, sp.rows);
-                return 0;
-            });
-            ANE_LAUNCH_OK(1);
+        const int rc = bn_pick_cluster<T, 8, 0>(vec, B, C, S, [&](auto form, BnSplit sp) -> int {
+            using F = decltype(form);
+            constexpr int SM = F::VEC == 1 ? 0 : F::THREADS == 512 ? 1 : 2;      // 512 threads: x in shared memory, f in registers
+            constexpr size_t smem = BnStrip<T, F::VEC, 2, SM, F::NV, F::THREADS>::BYTES;
+            static bool ready = false;
+            const auto kernel = block_norm_cluster_kernel<T, F::VEC, F::LG, F::NV, F::THREADS, SM>;
+            if (int e = bn_allow(kernel, smem, ready)) return e;
+            sh.tiles_per_seq = (S + F::LG * F::VEC - 1) / (F::LG * F::VEC);
+            bn_call(kernel, dim3((unsigned)B * (unsigned)sh.tiles_per_seq * (unsigned)sp.blocks), F::THREADS, sp.blocks, smem, st, (T *)x2, (T *)y, (const T *)x, (const T *)f, w_post, gate,
+                    w_pre, sh, sp.rows);
             return ANE_CUDA_OK;
-        }
+        });
+        if (rc == ANE_CUDA_OK) { ANE_LAUNCH_OK(1); return ANE_CUDA_OK; }
+        if (rc != BN_NONE) return rc;
         bn_pick<T>(vec, S, [&](auto v, auto lg) {
             constexpr int VEC = decltype(v)::value, LG = decltype(lg)::value;
             sh.tiles_per_seq = (S + VEC * LG - 1) / (VEC * LG);
@@ -690,24 +737,20 @@ int ane_cuda_block_norm_bwd_dev(void *stream, ane_dtype dtype, int B, int C, int
     };
     ANE_DISPATCH_DTYPE(dtype, T, {
         const bool vec = S % Elt<T>::VEC == 0 && aligned16(dx) && aligned16(df) && aligned16(dy) && aligned16(dx2) && aligned16(x2) && aligned16(f);
-        int rc;
-        if (vec && C <= 4096 && tuning("block_norm_cluster", 1)) {
-            rc = bn_pick_cluster(C, [&](auto lg, auto nv, BnSplit sp) -> int {
-                constexpr int LG = decltype(lg)::value, NV = decltype(nv)::value;
-                constexpr size_t smem = (size_t)4 * NV * BN_THREADS * 16;
-                static bool ready = false;
-                if (!ready) {
-                    ANE_CUDA_TRY(cudaFuncSetAttribute(block_norm_bwd_cluster_kernel<T, LG, NV>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-                    ready = true;
-                }
-                sh.tiles_per_seq = (S + LG * Elt<T>::VEC - 1) / (LG * Elt<T>::VEC);
-                const long long tiles = (long long)B * sh.tiles_per_seq;
-                if (int e = scratch(tiles, gate_per_seq ? sh.tiles_per_seq : 0)) return e;
-                bn_call(block_norm_bwd_cluster_kernel<T, LG, NV>, dim3((unsigned)tiles * (unsigned)sp.blocks), sp.blocks, smem, st, (T *)dx, (T *)df, reinterpret_cast<float *>(partial),
-                        (const T *)dy, (const T *)dx2, (const T *)x2, (const T *)f, w_post, gate, w_pre, sh, sp.rows);
-                return ANE_CUDA_OK;
-            });
-        } else {
+        int rc = bn_pick_cluster<T, 4, 512>(vec, B, C, S, [&](auto form, BnSplit sp) -> int {
+            using F = decltype(form);
+            constexpr int SM = F::VEC == 1 ? 0 : F::THREADS == 512 ? 3 : 4;      // 512 threads: dx2 in registers
+            constexpr size_t smem = BnStrip<T, F::VEC, 4, SM, F::NV, F::THREADS>::BYTES;
+            static bool ready = false;
+            const auto kernel = block_norm_bwd_cluster_kernel<T, F::VEC, F::LG, F::NV, F::THREADS, SM>;
+            if (int e = bn_allow(kernel, smem, ready)) return e;
+            sh.tiles_per_seq = (S + F::LG * F::VEC - 1) / (F::LG * F::VEC);
+            if (int e = scratch((long long)B * sh.tiles_per_seq, gate_per_seq ? sh.tiles_per_seq : 0)) return e;
+            bn_call(kernel, dim3((unsigned)B * (unsigned)sh.tiles_per_seq * (unsigned)sp.blocks), F::THREADS, sp.blocks, smem, st, (T *)dx, (T *)df, reinterpret_cast<float *>(partial),
+                    (const T *)dy, (const T *)dx2, (const T *)x2, (const T *)f, w_post, gate, w_pre, sh, sp.rows);
+            return ANE_CUDA_OK;
+        });
+        if (rc == BN_NONE) {
             rc = bn_pick<T>(vec, S, [&](auto v, auto lg) -> int {
                 constexpr int VEC = decltype(v)::value, LG = decltype(lg)::value;
                 sh.tiles_per_seq = (S + VEC * LG - 1) / (VEC * LG);
@@ -728,12 +771,12 @@ int ane_cuda_block_norm_bwd_dev(void *stream, ane_dtype dtype, int B, int C, int
         // gridDim.y holds 65535 groups: more than that take further launches
         for (int g0 = 0; g0 < groups; g0 += 65535) {
             const int n = groups - g0 < 65535 ? groups - g0 : 65535;
-            bn_call(block_norm_grad_kernel, dim3((C + 31) / 32, n), 0, 0, st, partial + (size_t)g0 * rows * C, all_rows - (long long)g0 * rows, rows, sums + (size_t)g0 * C,
+            bn_call(block_norm_grad_kernel, dim3((C + 31) / 32, n), 256, 0, 0, st, partial + (size_t)g0 * rows * C, all_rows - (long long)g0 * rows, rows, sums + (size_t)g0 * C,
                     gate_per_seq && dgate ? dgate + (size_t)g0 * C : nullptr, w_post, C, alpha);
             ANE_LAUNCH_OK(1);
         }
         if (dw_pre || dw_post || (dgate && !gate_per_seq)) {
-            bn_call(block_norm_grad_join_kernel, dim3((C + 31) / 32), 0, 0, st, sums, groups, dw_post, dgate, dw_pre, w_post, gate, sh.gate_stride, C);
+            bn_call(block_norm_grad_join_kernel, dim3((C + 31) / 32), 256, 0, 0, st, sums, groups, dw_post, dgate, dw_pre, w_post, gate, sh.gate_stride, C);
             ANE_LAUNCH_OK(1);
         }
     }
