@@ -271,7 +271,8 @@ def test_many_tensors_in_several_launches(ops):
     ops.adam_multi(ops.AdamTensors(w, g, m, v), **HYPER)
     ops.adam_multi(ops.AdamTensors(w8, g, *q, *s), **HYPER, seed=11)
     for k in (0, 399, 400, 799, 800, 899):
-        assert torch.equal(w[k], w8[k]) and float(m[k][0]) != 0.0
+        # from zero weights the step itself: root and quotient within 2^-22 each beside 8-bit states, five roundings more
+        assert bool(((w[k] - w8[k]).abs() <= (2 * 2.0 ** -22 + 6 * 2.0 ** -24) * w[k].abs()).all()) and float(m[k][0]) != 0.0
         assert np.array_equal(q[1][k].cpu().numpy(), encode(np32(v[k]), 11, k, True)[0])
 
 
