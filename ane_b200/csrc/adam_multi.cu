@@ -42,7 +42,7 @@ template <int CAP> struct AmList {
     AmItem it[CAP];
 };
 struct AmScalars {
-    float b1, b2, omb1, omb2, bc1, bc2, ibc1, ibc2, lr, eps, gscale;
+    float b1, b2, omb1, omb2, bc1, bc2, ibc1, ibc2, lr, eps, gscale, one;
     const float *clip;
     unsigned variant;
     int use_gscale, copy_dtype;
@@ -54,79 +54,100 @@ __host__ __device__ __forceinline__ uint32_t am_mix(uint32_t h) {
     h ^= h >> 13; h *= 0xC2B2AE35u;
     return h ^ (h >> 16);
 }
-__device__ __forceinline__ uint32_t am_hash(size_t place, uint32_t key) { return am_mix((uint32_t)place * 0x9E3779B1u + key); }
+constexpr uint32_t AM_GOLD = 0x9E3779B1u;
+__device__ __forceinline__ float am_sqrt(float x) { float y; asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+__device__ __forceinline__ float am_rcp(float x) { float y; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+__device__ __forceinline__ float2 am_two(float x) { return make_float2(x, x); }
 
-__device__ __forceinline__ float am_sqrt(float x) {
-    float y;
-    asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
+// The step is bound by instruction issue beside 8-bit states (16 bytes an element, 50 instructions), so values go in pairs
+// through the packed fp32 operations -- which round each half like the scalar ones -- and codes four to a word.
 template <bool SECOND> struct Code8;
 template <> struct Code8<false> {
     static constexpr float TOP = 480.0f;
-    __device__ __forceinline__ static float decode(uint32_t c, float scale) {
-        const float v = __fmul_rn(__fmul_rn(__uint_as_float((c & 127u) << 20), 0x1p120f), scale);
-        return c & 128u ? -v : v;
+    static constexpr float UP = 0x1p120f, DOWN = 0x1p-120f;
+    // byte j of a word as a float's bits: the sign to bit 31, the code's seven bits to 26..20
+    __device__ __forceinline__ static float bits(uint32_t word, int j) {
+        return __uint_as_float((uint32_t)((int32_t)(word << (24 - 8 * j)) >> 4) & 0x87f00000u);
     }
-    __device__ __forceinline__ static uint32_t encode(float v, float inv, uint32_t r20) {
-        const uint32_t c = (__float_as_uint(__fmul_rn(__fmul_rn(fabsf(v), inv), 0x1p-120f)) + r20) >> 20;
+    // y = value * inverse * 2^-120
+    __device__ __forceinline__ static uint32_t encode(float v, float y, uint32_t r20) {
+        const uint32_t c = ((__float_as_uint(y) & 0x7fffffffu) + r20) >> 20;
         return (c < 127u ? c : 127u) | (v < 0.0f ? 128u : 0u);
     }
 };
 template <> struct Code8<true> {
     static constexpr float TOP = 122880.0f;
-    __device__ __forceinline__ static float decode(uint32_t c, float scale) {
-        return __fmul_rn(__fmul_rn(__uint_as_float(c << 20), 0x1p112f), scale);
+    static constexpr float UP = 0x1p112f, DOWN = 0x1p-112f;
+    __device__ __forceinline__ static float bits(uint32_t word, int j) {
+        return __uint_as_float((8 * j < 20 ? word << (20 - 8 * j) : word >> (8 * j - 20)) & 0x0ff00000u);
     }
     // A value above zero keeps a code above zero: m / sqrt(v) with v lost to rounding would be m / eps.
-    __device__ __forceinline__ static uint32_t encode(float v, float inv, uint32_t r20) {
-        const float y = __fmul_rn(__fmul_rn(fabsf(v), inv), 0x1p-112f);
-        uint32_t c = (__float_as_uint(y) + r20) >> 20;
-        c = c < 255u ? c : 255u;
-        return c == 0u && y > 0.0f ? 1u : c;
+    __device__ __forceinline__ static uint32_t encode(float, float y, uint32_t r20) {
+        const uint32_t u = __float_as_uint(y) & 0x7fffffffu, c = (u + r20) >> 20, least = u < 1u ? u : 1u;
+        return c < least ? least : c < 255u ? c : 255u;
     }
 };
+
+// Eight values of a lane.
+typedef float2 Am8[4];
+__device__ __forceinline__ float am_at(const Am8 &f, int j) { return j & 1 ? f[j >> 1].y : f[j >> 1].x; }
 
 // Scale of a block from its largest magnitude over the warp.  Magnitudes compare as unsigned integers, and NaN above all, so
 // a NaN or an infinity makes the whole block NaN instead of vanishing in a code.  A block below 2^-100 is zero: top / most
 // would leave fp32's range.  Scale and inverse come from reciprocals (most * (1 / top), (1 / most) * top): the code of a value
 // is defined by these roundings.
-template <bool SECOND> __device__ __forceinline__ float am_scale(const float *v, float &inv) {
+template <bool SECOND> __device__ __forceinline__ float am_scale(const Am8 &v, float &inv) {
     uint32_t most = 0;
 #pragma unroll
-    for (int i = 0; i < 8; i++) { const uint32_t a = __float_as_uint(v[i]) & 0x7fffffffu; most = a > most ? a : most; }
+    for (int j = 0; j < 8; j++) { const uint32_t a = __float_as_uint(am_at(v, j)) & 0x7fffffffu; most = a > most ? a : most; }
     float a = __uint_as_float(__reduce_max_sync(0xffffffffu, most));
     if (a < 0x1p-100f) a = 0.0f;
     inv = a > 0.0f ? __fmul_rn(__frcp_rn(a), Code8<SECOND>::TOP) : 0.0f;
     return a <= 3.402823466e38f ? __fmul_rn(a, 1.0f / Code8<SECOND>::TOP) : __uint_as_float(0x7fc00000u);
 }
-
-// Eight elements at p + i: whole when `full`, else those below n, the others 0.
-template <typename T> __device__ __forceinline__ void am_load8(const T *p, size_t i, size_t n, bool full, float *f) {
-    if (full) {
-        if constexpr (sizeof(T) == 4) {
-            Elt<T>::unpack(__ldcs(reinterpret_cast<const uint4 *>(p + i)), f);
-            Elt<T>::unpack(__ldcs(reinterpret_cast<const uint4 *>(p + i) + 1), f + 4);
-        } else {
-            Elt<T>::unpack(__ldcs(reinterpret_cast<const uint4 *>(p + i)), f);
-        }
-    } else {
+template <bool SECOND> __device__ __forceinline__ void am_decode8(uint2 c, float scale, Am8 &f) {
 #pragma unroll
-        for (int j = 0; j < 8; j++) f[j] = i + j < n ? Elt<T>::to_f(p[i + j]) : 0.0f;
+    for (int i = 0; i < 4; i++) {
+        const uint32_t w = i < 2 ? c.x : c.y;
+        const float2 q = make_float2(Code8<SECOND>::bits(w, 2 * i & 3), Code8<SECOND>::bits(w, (2 * i & 3) + 1));
+        f[i] = f2_mul(f2_mul(q, am_two(Code8<SECOND>::UP)), am_two(scale));
     }
 }
-template <typename T> __device__ __forceinline__ void am_store8(T *p, size_t i, size_t n, bool full, const float *f) {
+// The random bits of element j of a lane whose first element hashes to h0: the upper 20 for the first moment, the lower 20
+// for the second.
+__device__ __forceinline__ uint32_t am_noise(uint32_t h0, int j) { return am_mix(h0 + (uint32_t)j * AM_GOLD); }
+template <bool SECOND> __device__ __forceinline__ uint2 am_encode8(const Am8 &v, float inv, const uint32_t (&h)[8]) {
+    uint32_t c[8];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float2 y = f2_mul(f2_mul(v[i], am_two(inv)), am_two(Code8<SECOND>::DOWN));
+        c[2 * i] = Code8<SECOND>::encode(v[i].x, y.x, SECOND ? h[2 * i] & 0xfffffu : h[2 * i] >> 12);
+        c[2 * i + 1] = Code8<SECOND>::encode(v[i].y, y.y, SECOND ? h[2 * i + 1] & 0xfffffu : h[2 * i + 1] >> 12);
+    }
+    return make_uint2(__byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410),
+                      __byte_perm(__byte_perm(c[4], c[5], 0x0040), __byte_perm(c[6], c[7], 0x0040), 0x5410));
+}
+
+// Eight elements at p + i: whole when `full`, else those below n, the others 0.
+template <typename T> __device__ __forceinline__ void am_load8(const T *p, size_t i, size_t n, bool full, Am8 &f) {
     if (full) {
-        if constexpr (sizeof(T) == 4) {
-            __stcs(reinterpret_cast<uint4 *>(p + i), Elt<T>::pack(f));
-            __stcs(reinterpret_cast<uint4 *>(p + i) + 1, Elt<T>::pack(f + 4));
-        } else {
-            __stcs(reinterpret_cast<uint4 *>(p + i), Elt<T>::pack(f));
-        }
+        Elt<T>::unpack2(__ldcs(reinterpret_cast<const uint4 *>(p + i)), f);
+        if constexpr (sizeof(T) == 4) Elt<T>::unpack2(__ldcs(reinterpret_cast<const uint4 *>(p + i) + 1), f + 2);
+    } else {
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = i + j < n ? Elt<T>::to_f(p[i + j]) : 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; j++) f[j] = make_float2(v[2 * j], v[2 * j + 1]);
+    }
+}
+template <typename T> __device__ __forceinline__ void am_store8(T *p, size_t i, size_t n, bool full, const Am8 &f) {
+    if (full) {
+        __stcs(reinterpret_cast<uint4 *>(p + i), Elt<T>::pack2(f));
+        if constexpr (sizeof(T) == 4) __stcs(reinterpret_cast<uint4 *>(p + i) + 1, Elt<T>::pack2(f + 2));
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; j++) if (i + j < n) p[i + j] = Elt<T>::from_f(f[j]);
+        for (int j = 0; j < 8; j++) if (i + j < n) p[i + j] = Elt<T>::from_f(am_at(f, j));
     }
 }
 __device__ __forceinline__ uint2 am_load_codes(const uint8_t *p, size_t i, size_t n, bool full) {
@@ -141,11 +162,6 @@ __device__ __forceinline__ void am_store_codes(uint8_t *p, size_t i, size_t n, b
 #pragma unroll
     for (int j = 0; j < 8; j++) if (i + j < n) p[i + j] = (uint8_t)((j < 4 ? c.x : c.y) >> (8 * (j & 3)));
 }
-template <bool SECOND> __device__ __forceinline__ void am_decode8(uint2 c, float scale, float *f) {
-#pragma unroll
-    for (int j = 0; j < 8; j++) f[j] = Code8<SECOND>::decode(((j < 4 ? c.x : c.y) >> (8 * (j & 3))) & 255u, scale);
-}
-
 // A warp owns 256 consecutive elements of one tensor, a lane eight of them.  All loads of the lane are issued before the
 // first use; nothing is kept between elements, so the kernel is a stream.
 template <typename G, bool Q8, int CAP>
@@ -163,7 +179,7 @@ __global__ void __launch_bounds__(AM_THREADS) adam_multi_kernel(const __grid_con
     const size_t i = group * AM_GROUP + (threadIdx.x & 31) * 8;
     const bool full = it.vec && i + 8 <= n;
 
-    float w[8], g[8], m[8], v[8];
+    Am8 w, g, m, v;
     am_load8(it.w, i, n, full, w);
     am_load8(static_cast<const G *>(it.g), i, n, full, g);
     if constexpr (Q8) {
@@ -177,22 +193,29 @@ __global__ void __launch_bounds__(AM_THREADS) adam_multi_kernel(const __grid_con
     const float clip = s.clip ? __ldg(s.clip) : 1.0f;        // a product with 1 changes nothing
     const float gscale = s.use_gscale ? s.gscale : 1.0f;
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-        const float gj = __fmul_rn(__fmul_rn(g[j], gscale), clip);
-        m[j] = __fadd_rn(__fmul_rn(s.b1, m[j]), __fmul_rn(s.omb1, gj));
-        v[j] = __fadd_rn(__fmul_rn(s.b2, v[j]), __fmul_rn(__fmul_rn(s.omb2, gj), gj));
+    for (int j = 0; j < 4; j++) {
+        const float2 gj = f2_mul(f2_mul(g[j], am_two(gscale)), am_two(clip));
+        // A sum of two rounded products.  A packed product and a packed add would be contracted into one fma, with one rounding
+        // less; as a product with a 1 that the compiler does not know the add stays what it is.
+        m[j] = f2_fma(f2_mul(am_two(s.b1), m[j]), am_two(s.one), f2_mul(am_two(s.omb1), gj));
+        v[j] = f2_fma(f2_mul(am_two(s.b2), v[j]), am_two(s.one), f2_mul(f2_mul(am_two(s.omb2), gj), gj));
         if constexpr (Q8) {
-            // The moments are exact to the bit, because codes are made of them; the step is not: approximate root and quotient
-            // (2^-22) against 35 instructions an element more, where a byte-sized state leaves 60 in the time of its bytes.
-            const float den = am_sqrt(v[j] * s.ibc2) + s.eps;
-            const float step = __fdividef(m[j] * s.ibc1, den);
-            w[j] -= s.lr * (s.variant == ANE_ADAM_STORIES ? step : fmaf(it.wd, w[j], step));
-            continue;
+            // The moments are exact to the bit, because codes are made of them; the step is not: approximate root and reciprocal
+            // (2^-22 each) against 35 instructions an element more.
+            const float2 vh = f2_mul(v[j], am_two(s.ibc2));
+            const float2 den = f2_add(make_float2(am_sqrt(vh.x), am_sqrt(vh.y)), am_two(s.eps));
+            float2 step = f2_mul(f2_mul(m[j], am_two(s.ibc1)), make_float2(am_rcp(den.x), am_rcp(den.y)));
+            if (s.variant != ANE_ADAM_STORIES) step = f2_fma(am_two(it.wd), w[j], step);
+            w[j] = f2_fma(am_two(-s.lr), step, w[j]);
+        } else {
+            auto one = [&](float w, float m, float v) {
+                const float mh = __fdiv_rn(m, s.bc1), vh = __fdiv_rn(v, s.bc2);
+                const float den = __fadd_rn(__fsqrt_rn(vh), s.eps);
+                if (s.variant == ANE_ADAM_STORIES) return __fsub_rn(w, __fdiv_rn(__fmul_rn(s.lr, mh), den));
+                return __fsub_rn(w, __fmul_rn(s.lr, __fadd_rn(__fdiv_rn(mh, den), __fmul_rn(it.wd, w))));
+            };
+            w[j] = make_float2(one(w[j].x, m[j].x, v[j].x), one(w[j].y, m[j].y, v[j].y));
         }
-        const float mh = __fdiv_rn(m[j], s.bc1), vh = __fdiv_rn(v[j], s.bc2);
-        const float den = __fadd_rn(__fsqrt_rn(vh), s.eps);
-        if (s.variant == ANE_ADAM_STORIES) w[j] = __fsub_rn(w[j], __fdiv_rn(__fmul_rn(s.lr, mh), den));
-        else w[j] = __fsub_rn(w[j], __fmul_rn(s.lr, __fadd_rn(__fdiv_rn(mh, den), __fmul_rn(it.wd, w[j]))));
     }
     am_store8(it.w, i, n, full, w);
     if (it.copy) {
@@ -203,15 +226,12 @@ __global__ void __launch_bounds__(AM_THREADS) adam_multi_kernel(const __grid_con
         float im, iv;
         const float sm = am_scale<false>(m, im), sv = am_scale<true>(v, iv);
         if ((threadIdx.x & 31) == 0) { it.ms[group] = sm; it.vs[group] = sv; }
-        uint32_t cm[2] = {0, 0}, cv[2] = {0, 0};
+        uint32_t h[8];
+        const uint32_t h0 = (uint32_t)i * AM_GOLD + it.key;
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const uint32_t h = am_hash(i + j, it.key);
-            cm[j / 4] |= Code8<false>::encode(m[j], im, h >> 12) << (8 * (j & 3));
-            cv[j / 4] |= Code8<true>::encode(v[j], iv, h & 0xfffffu) << (8 * (j & 3));
-        }
-        am_store_codes(static_cast<uint8_t *>(it.m), i, n, full, make_uint2(cm[0], cm[1]));
-        am_store_codes(static_cast<uint8_t *>(it.v), i, n, full, make_uint2(cv[0], cv[1]));
+        for (int j = 0; j < 8; j++) h[j] = am_noise(h0, j);
+        am_store_codes(static_cast<uint8_t *>(it.m), i, n, full, am_encode8<false>(m, im, h));
+        am_store_codes(static_cast<uint8_t *>(it.v), i, n, full, am_encode8<true>(v, iv, h));
     } else {
         am_store8(static_cast<float *>(it.m), i, n, full, m);
         am_store8(static_cast<float *>(it.v), i, n, full, v);
@@ -224,7 +244,7 @@ __global__ void __launch_bounds__(AM_THREADS) adam_state_unpack_kernel(size_t n,
     const size_t i = group * AM_GROUP + (threadIdx.x & 31) * 8;
     if (i >= n) return;
     const bool full = vec && i + 8 <= n;
-    float f[8];
+    Am8 f;
     am_decode8<SECOND>(am_load_codes(codes, i, n, full), scales[group], f);
     am_store8(out, i, n, full, f);
 }
@@ -235,17 +255,16 @@ __global__ void __launch_bounds__(AM_THREADS) adam_state_pack_kernel(size_t n, u
     if (group * AM_GROUP >= n) return;
     const size_t i = group * AM_GROUP + (threadIdx.x & 31) * 8;
     const bool full = vec && i + 8 <= n;
-    float f[8], inv;
+    Am8 f;
+    float inv;
     am_load8(value, i, n, full, f);
     const float scale = am_scale<SECOND>(f, inv);
     if ((threadIdx.x & 31) == 0) scales[group] = scale;
-    uint32_t c[2] = {0, 0};
+    uint32_t h[8];
+    const uint32_t h0 = (uint32_t)i * AM_GOLD + key;
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-        const uint32_t h = am_hash(i + j, key);
-        c[j / 4] |= Code8<SECOND>::encode(f[j], inv, SECOND ? h & 0xfffffu : h >> 12) << (8 * (j & 3));
-    }
-    am_store_codes(codes, i, n, full, make_uint2(c[0], c[1]));
+    for (int j = 0; j < 8; j++) h[j] = am_noise(h0, j);
+    am_store_codes(codes, i, n, full, am_encode8<SECOND>(f, inv, h));
 }
 
 static inline bool aligned_to(const void *p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
@@ -338,6 +357,7 @@ int ane_cuda_adam_multi_dev(void *stream, ane_adam_state state, ane_dtype g_dtyp
     s.bc1 = 1.0f - powf(b1, t);           // on the host, as ane_cuda_adam_dev
     s.bc2 = 1.0f - powf(b2, t);
     s.ibc1 = 1.0f / s.bc1; s.ibc2 = 1.0f / s.bc2;
+    s.one = 1.0f;
     s.lr = lr; s.eps = eps; s.gscale = gscale;
     s.use_gscale = gscale != 1.0f;
     s.clip = clip_dev;
