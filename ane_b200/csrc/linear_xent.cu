@@ -573,11 +573,29 @@ __global__ void __launch_bounds__(256) lx_pack_x_kernel(H *hi, H *lo, const T *_
     }
 }
 
-// Rows of the table -> [row][lde] 16-bit rows with aligned ends; fp32 scaled, as two parts.
+// Rows of the table -> [row][lde] 16-bit rows with aligned ends; fp32 scaled, as two parts.  `flat`: rows without a gap on
+// both sides (lde == D), eight elements at a time.
 template <typename T, typename H>
-__global__ void __launch_bounds__(256) lx_pack_rows_kernel(H *hi, H *lo, const T *__restrict__ src, const float *scales, int rows, int D, size_t lde) {
+__global__ void __launch_bounds__(256) lx_pack_rows_kernel(H *hi, H *lo, const T *__restrict__ src, const float *scales, int rows, int D, size_t lde, int flat) {
     dep_sync();
     const float scale = scales ? scales[3] : 1.0f;
+    if (sizeof(T) == 4 && flat) {
+        const size_t n = (size_t)rows * D / 8, step = (size_t)gridDim.x * 256;
+        for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += step) {
+            float f[8], h[8];
+            Elt<float>::unpack(reinterpret_cast<const uint4 *>(src)[2 * i], f);
+            Elt<float>::unpack(reinterpret_cast<const uint4 *>(src)[2 * i + 1], f + 4);
+#pragma unroll
+            for (int j = 0; j < 8; j++) f[j] *= scale;
+            const uint4 q = Elt<H>::pack(f);
+            Elt<H>::unpack(q, h);
+            reinterpret_cast<uint4 *>(hi)[i] = q;
+#pragma unroll
+            for (int j = 0; j < 8; j++) f[j] -= h[j];
+            reinterpret_cast<uint4 *>(lo)[i] = Elt<H>::pack(f);
+        }
+        return;
+    }
     for (int r = blockIdx.x; r < rows; r += gridDim.x)
         for (int d = threadIdx.x; d < (int)lde; d += 256) {
             const float v = d < D ? Elt<T>::to_f(src[(size_t)r * D + d]) * scale : 0.0f;
@@ -841,7 +859,10 @@ template <typename T, typename H> static int lx_run(const LxCall &c) {
         }
         if (vk < V || packed < V) {
             const int lo = vk < V ? v0 : 0, n = vk < V ? nv : V;
-            lx_call(lx_pack_rows_kernel<T, H>, dim3(n < 4096 ? n : 4096), dim3(256), 0, c.st, eh, el, static_cast<const T *>(c.table) + (size_t)lo * D, scales, n, D, ldd);
+            const T *from = static_cast<const T *>(c.table) + (size_t)lo * D;
+            const int flat = split && D % 8 == 0 && aligned16(from);
+            const size_t want = flat ? ((size_t)n * D / 8 + 255) / 256 : (size_t)n;
+            lx_call(lx_pack_rows_kernel<T, H>, dim3((unsigned)(want < 4096 ? want : 4096)), dim3(256), 0, c.st, eh, el, from, scales, n, D, ldd, flat);
             ANE_LAUNCH_OK(1);
             if (vk == V) packed = V;
         }
