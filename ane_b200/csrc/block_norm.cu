@@ -528,6 +528,10 @@ block_norm_bwd_cluster_kernel(T *dx, T *df, float *__restrict__ partial, const T
     bn_cluster_wait();
 }
 
+}  // namespace ane
+#include "block_norm_ring.cuh"
+namespace ane {
+
 // ------------------------------------------------------------------ parameter gradients
 // Sums of the rows of partials [row][C] of one group, in a fixed order: 32 channels x 8 slices of rows per block.  The sums
 // stay in `sums` [group][C] for the kernel below; where a group is a sequence with a gate of its own, its dgate is finished
@@ -615,6 +619,18 @@ static inline void bn_call(void (*kernel)(KArgs...), dim3 grid, int threads, int
     cfg.attrs = attr; cfg.numAttrs = cluster ? 2 : 1;
     cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);      // the error, if any, is picked up by ANE_LAUNCH_OK
 }
+// Clusters of `blocks` blocks that the device holds at once.
+template <typename... KArgs> static int bn_resident(void (*kernel)(KArgs...), int threads, int blocks, size_t smem) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(blocks * ctx().sm_count)); cfg.blockDim = dim3((unsigned)threads); cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = (unsigned)blocks; at.val.clusterDim.y = 1; at.val.clusterDim.z = 1;
+    cfg.attrs = &at; cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) { cudaGetLastError(); n = ctx().sm_count / (2 * blocks); }
+    return n < 1 ? 1 : n;
+}
 // The cluster form for a shape, if there is one.
 //   many tiles   512 threads per block; 1024 channels to a block
 //   few tiles    256 threads, up to eight blocks per tile, so that more SMs take part
@@ -625,8 +641,8 @@ template <int V_, int LG_, int NV_, int TH_> struct BnForm { static constexpr in
 // BIG_LG: lanes per row of the large form (a thread has C / (512 / BIG_LG) rows); BIG_C: channels above which it is used.
 template <typename T, int BIG_LG, int BIG_C, typename Fn> static int bn_pick_cluster(bool vec, int B, int C, int S, Fn &&go) {
     constexpr int N = Elt<T>::VEC, BR = 512 / BIG_LG;
-    const int knob = tuning("block_norm_cluster", 3);    // 0: none, 1: the small form only, 3: both
-    if (!knob) return BN_NONE;
+    const int knob = tuning("block_norm_cluster", 7);    // bits: 1 small form, 2 large form, 4 backward ring; 0: none
+    if (!(knob & 3)) return BN_NONE;
     const long long big_tiles = (long long)B * ((S + BIG_LG * N - 1) / (BIG_LG * N));
     if (vec && C > BIG_C && C <= 4096 && (knob & 2) && big_tiles * ((C + 1023) / 1024) >= 2LL * ctx().sm_count) {
         if constexpr (BIG_C < 512) {
@@ -737,7 +753,35 @@ int ane_cuda_block_norm_bwd_dev(void *stream, ane_dtype dtype, int B, int C, int
     };
     ANE_DISPATCH_DTYPE(dtype, T, {
         const bool vec = S % Elt<T>::VEC == 0 && aligned16(dx) && aligned16(df) && aligned16(dy) && aligned16(dx2) && aligned16(x2) && aligned16(f);
-        int rc = bn_pick_cluster<T, 4, 512>(vec, B, C, S, [&](auto form, BnSplit sp) -> int {
+        int rc = BN_NONE;
+        constexpr int RTW = 32 * BrWord<T>::W;
+        const BnSplit rsp = bn_split(C, BR_ROWS);
+        const long long rtiles = (long long)B * ((S + RTW - 1) / RTW);
+        if (vec && rsp.blocks && (tuning("block_norm_cluster", 7) & 4) && rtiles * rsp.blocks >= 4LL * ctx().sm_count) {
+            BrMaps maps;
+            const void *from[4] = {x2, dy, f, dx2};
+            for (int i = 0; i < (dx2 ? 4 : 3); i++)
+                if (int e = make_bcs_tensor_map(&maps.t[i], dtype, from[i], B, C, S, RTW, rsp.rows)) return e;
+            sh.tiles_per_seq = (S + RTW - 1) / RTW;
+            if (int e = scratch(rtiles, gate_per_seq ? sh.tiles_per_seq : 0)) return e;
+            auto go = [&](auto post, auto has, auto full) -> int {
+                const auto kernel = block_norm_bwd_ring_kernel<T, decltype(post)::value, decltype(has)::value, decltype(full)::value>;
+                static int fit[9] = {};
+                if (!fit[rsp.blocks]) {
+                    ANE_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)BR_SMEM));
+                    fit[rsp.blocks] = bn_resident(kernel, BR_THREADS, rsp.blocks, BR_SMEM);
+                }
+                const int clusters = rtiles < fit[rsp.blocks] ? (int)rtiles : fit[rsp.blocks];
+                bn_call(kernel, dim3((unsigned)(clusters * rsp.blocks)), BR_THREADS, rsp.blocks, BR_SMEM, st, maps, (T *)dx, (T *)df, reinterpret_cast<float *>(partial), w_post, gate, w_pre,
+                        sh, rsp.rows, (int)rtiles, ctx().status);
+                return ANE_CUDA_OK;
+            };
+            auto pick = [&](auto post, auto has) { return C == rsp.blocks * BR_ROWS ? go(post, has, std::true_type()) : go(post, has, std::false_type()); };
+            rc = w_post ? (dx2 ? pick(std::true_type(), std::true_type()) : pick(std::true_type(), std::false_type()))
+                        : (dx2 ? pick(std::false_type(), std::true_type()) : pick(std::false_type(), std::false_type()));
+            if (rc != ANE_CUDA_OK) return rc;
+        }
+        if (rc == BN_NONE) rc = bn_pick_cluster<T, 4, 512>(vec, B, C, S, [&](auto form, BnSplit sp) -> int {
             using F = decltype(form);
             constexpr int SM = F::VEC == 1 ? 0 : F::THREADS == 512 ? 3 : 4;      // 512 threads: dx2 in registers
             constexpr size_t smem = BnStrip<T, F::VEC, 4, SM, F::NV, F::THREADS>::BYTES;

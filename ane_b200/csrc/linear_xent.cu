@@ -766,7 +766,9 @@ struct LxPlan { int chunk, piece_tiles, splits; };
 
 // A round has at most 8192 tokens.  A piece has as many vocabulary tiles as fill whole waves of the SM pairs best, counted in
 // waves of K blocks over all pieces and products (with four K blocks for the start of a launch), while the two parts of dl
-// stay within 384 MiB.  dx has few tiles and a long K: where its tiles leave pairs idle, K is cut into shares.
+// stay within 768 MiB (128, 192, 384, 768 MiB: 12.0, 11.4, 10.8, 10.3 ms for 8192 tokens x 151936 rows x 1024
+// channels under the power cap: a launch of dx has one tile per pair and nothing to hide its end behind).  dx has few tiles
+// and a long K: where its tiles leave pairs idle, K is cut into shares.
 static LxPlan lx_plan(int T_all, int D, int V, int segs, bool dx, bool d_table, bool two_parts) {
     LxPlan p;
     const int rounds = lx_div(T_all, 8192), pairs = lx_pairs();
@@ -774,7 +776,7 @@ static LxPlan lx_plan(int T_all, int D, int V, int segs, bool dx, bool d_table, 
     if (p.chunk > T_all) p.chunk = T_all;
     const int mt = lx_div(p.chunk, LX_BM), dt = lx_div(D, LX_BN), vt = lx_div(V, LX_BN);
     const int kd = lx_div(D, LX_BK), kt = lx_div(p.chunk, LX_BK);
-    long long most = (384ll << 20) / ((long long)p.chunk * LX_BN * (two_parts ? 4 : 2));
+    long long most = (768ll << 20) / ((long long)p.chunk * LX_BN * (two_parts ? 4 : 2));
     if (most < 1) most = 1;
     if (most > vt) most = vt;
     double best = 1e300;

@@ -329,7 +329,8 @@ int ane_cuda_cross_entropy_dev(void *stream, ane_idtype idtype, int B, int V, in
  * column in dx, nothing added to d_table, whatever its x holds -- unlike ane_cuda_cross_entropy_dev, which keeps the
  * reference's plain-softmax gradient there.  Ids >= V are counted in the status words, negative ones are not.  The products
  * run on the tensor cores with fp32 sums; fp32 inputs enter as two bf16 parts each, dl as two 16-bit parts in d_table and as
- * one in a 16-bit dx.  Bit-stable from call to call.  Scratch: about 100 to 250 MiB of the library's range. */
+ * one in a 16-bit dx.  Bit-stable from call to call.  Scratch: up to about 1 GiB of the library's range, however large the
+ * vocabulary. */
 int ane_cuda_linear_cross_entropy_dev(void *stream, ane_dtype dtype, ane_idtype idtype, int B, int D, int V, int S,
                                       float *loss_seq, float *loss_tok, void *dx, float *d_table, const void *x,
                                       const void *table, const void *targets, float grad_scale);

@@ -107,7 +107,8 @@ def inputs(shape, dt, post, gate, seed=0):
 
 
 SHAPES = [(1, 1, 1), (2, 7, 3), (3, 33, 5), (1, 768, 256), (2, 128, 257), (3, 100, 333), (4, 64, 1), (1, 4096, 64), (2, 1024, 48), (70, 16, 2),
-          (1, 300, 8), (1, 129, 64), (1, 4099, 8), (3, 2048, 72), (2, 1024, 1032), (1, 6000, 16)]
+          (1, 300, 8), (1, 129, 64), (1, 4099, 8), (3, 2048, 72), (2, 1024, 1032), (1, 6000, 16),
+          (32, 1024, 512), (40, 96, 1000), (20, 1000, 264), (24, 700, 520)]      # many tiles: the pipelined forms
 
 
 @pytest.mark.gpu
@@ -118,12 +119,13 @@ SHAPES = [(1, 1, 1), (2, 7, 3), (3, 33, 5), (1, 768, 256), (2, 128, 257), (3, 10
 def test_forward(ops, shape, dt, post, gate):
     s, _ = inputs(shape, DT[dt], post, gate)
     x2, y = ops.block_norm(s["x"], s["f"], s["w_pre"], w_post=s["w_post"], gate=s["gate"], alpha=0.35, eps=EPS)
-    assert within(x2, forward64(s["x"], s["f"], s["w_post"], s["gate"], 0.35), DT[dt]) [0]
+    assert within(x2, forward64(s["x"], s["f"], s["w_post"], s["gate"], 0.35), DT[dt])[0]
     assert within(y, norm64(x2, s["w_pre"]), DT[dt])[0]
     # in place, the same bits
     x = s["x"].clone()
     a, b = ops.block_norm(x, s["f"], s["w_pre"], w_post=s["w_post"], gate=s["gate"], alpha=0.35, eps=EPS, x2=x)
     assert torch.equal(a, x2) and torch.equal(b, y)
+    assert lib.poll_status().wait_giveups == 0
 
 
 @pytest.mark.gpu
@@ -171,6 +173,7 @@ def test_backward(ops, shape, dt, post, gate, with_dx2):
     f, kw["dx2"] = s["f"].clone(), None if dx2 is None else dx2.clone()
     dx_, df_ = ops.block_norm_bwd(dy, s["x"], f, s["w_pre"], None, **kw, dx=kw["dx2"], df=f)
     assert torch.equal(dx, dx_) and torch.equal(df, df_) and df_ is f
+    assert lib.poll_status().wait_giveups == 0
 
 
 @pytest.mark.gpu
