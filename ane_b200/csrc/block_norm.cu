@@ -631,6 +631,11 @@ template <typename... KArgs> static int bn_resident(void (*kernel)(KArgs...), in
     if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) { cudaGetLastError(); n = ctx().sm_count / (2 * blocks); }
     return n < 1 ? 1 : n;
 }
+// The pipelined backward form: up to eight blocks of 128 channels, and at least four tiles for every SM's block to walk (with
+// fewer the pipeline is mostly filling and draining).
+static bool bn_ring(int C, const BnSplit &sp, long long tiles) {
+    return sp.blocks && C % 128 == 0 && (tuning("block_norm_cluster", 7) & 4) && tiles * sp.blocks >= 4LL * ctx().sm_count;
+}
 // The cluster form for a shape, if there is one.
 //   many tiles   512 threads per block; 1024 channels to a block
 //   few tiles    256 threads, up to eight blocks per tile, so that more SMs take part
@@ -694,7 +699,7 @@ int ane_cuda_block_norm_dev(void *stream, ane_dtype dtype, int B, int C, int S, 
     BnShape sh = {B, C, S, 0, 0, gate_per_seq ? C : 0, alpha, eps};
     ANE_DISPATCH_DTYPE(dtype, T, {
         const bool vec = S % Elt<T>::VEC == 0 && aligned16(x2) && aligned16(y) && aligned16(x) && aligned16(f);
-        const int rc = bn_pick_cluster<T, 8, 0>(vec, B, C, S, [&](auto form, BnSplit sp) -> int {
+        const int rc = bn_pick_cluster<T, 4, 0>(vec, B, C, S, [&](auto form, BnSplit sp) -> int {
             using F = decltype(form);
             constexpr int SM = F::VEC == 1 ? 0 : F::THREADS == 512 ? 1 : 2;      // 512 threads: x in shared memory, f in registers
             constexpr size_t smem = BnStrip<T, F::VEC, 2, SM, F::NV, F::THREADS>::BYTES;
@@ -757,15 +762,15 @@ int ane_cuda_block_norm_bwd_dev(void *stream, ane_dtype dtype, int B, int C, int
         constexpr int RTW = 32 * BrWord<T>::W;
         const BnSplit rsp = bn_split(C, BR_ROWS);
         const long long rtiles = (long long)B * ((S + RTW - 1) / RTW);
-        if (vec && rsp.blocks && (tuning("block_norm_cluster", 7) & 4) && rtiles * rsp.blocks >= 4LL * ctx().sm_count) {
+        if (vec && bn_ring(C, rsp, rtiles)) {
             BrMaps maps;
             const void *from[4] = {x2, dy, f, dx2};
             for (int i = 0; i < (dx2 ? 4 : 3); i++)
-                if (int e = make_bcs_tensor_map(&maps.t[i], dtype, from[i], B, C, S, RTW, rsp.rows)) return e;
+                if (int e = make_bcs_tensor_map(&maps.t[i], dtype, from[i], B, C, S, RTW, BR_ROWS)) return e;
             sh.tiles_per_seq = (S + RTW - 1) / RTW;
             if (int e = scratch(rtiles, gate_per_seq ? sh.tiles_per_seq : 0)) return e;
-            auto go = [&](auto post, auto has, auto full) -> int {
-                const auto kernel = block_norm_bwd_ring_kernel<T, decltype(post)::value, decltype(has)::value, decltype(full)::value>;
+            auto go = [&](auto post, auto has) -> int {
+                const auto kernel = block_norm_bwd_ring_kernel<T, decltype(post)::value, decltype(has)::value>;
                 static int fit[9] = {};
                 if (!fit[rsp.blocks]) {
                     ANE_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)BR_SMEM));
@@ -773,12 +778,11 @@ int ane_cuda_block_norm_bwd_dev(void *stream, ane_dtype dtype, int B, int C, int
                 }
                 const int clusters = rtiles < fit[rsp.blocks] ? (int)rtiles : fit[rsp.blocks];
                 bn_call(kernel, dim3((unsigned)(clusters * rsp.blocks)), BR_THREADS, rsp.blocks, BR_SMEM, st, maps, (T *)dx, (T *)df, reinterpret_cast<float *>(partial), w_post, gate, w_pre,
-                        sh, rsp.rows, (int)rtiles, ctx().status);
+                        sh, (int)rtiles, ctx().status);
                 return ANE_CUDA_OK;
             };
-            auto pick = [&](auto post, auto has) { return C == rsp.blocks * BR_ROWS ? go(post, has, std::true_type()) : go(post, has, std::false_type()); };
-            rc = w_post ? (dx2 ? pick(std::true_type(), std::true_type()) : pick(std::true_type(), std::false_type()))
-                        : (dx2 ? pick(std::false_type(), std::true_type()) : pick(std::false_type(), std::false_type()));
+            rc = w_post ? (dx2 ? go(std::true_type(), std::true_type()) : go(std::true_type(), std::false_type()))
+                        : (dx2 ? go(std::false_type(), std::true_type()) : go(std::false_type(), std::false_type()));
             if (rc != ANE_CUDA_OK) return rc;
         }
         if (rc == BN_NONE) rc = bn_pick_cluster<T, 4, 512>(vec, B, C, S, [&](auto form, BnSplit sp) -> int {

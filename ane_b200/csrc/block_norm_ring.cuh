@@ -1,9 +1,9 @@
-// block_norm_ring.cuh -- backward pass of the norms around a block as a pipeline, for aligned rows, up to 1024 channels and many
-// tokens.
+// block_norm_ring.cuh -- backward pass of the norms around a block as a pipeline, for aligned rows, channels in multiples of
+// 128 up to 1024, and many tokens.
 //
-// One block per SM, clusters of up to eight blocks that share the channels of a tile (128 bytes of tokens per row, up to 128
-// rows per block) and walk the tiles.  The copy engine fills a ring of three stages (x2, dy, f, dx2 of one tile).  While the
-// per-token sums of tile j travel, the rows of tile j-1 are finished, so neither the copies nor the exchange stand in the way:
+// One block per SM, clusters of up to eight blocks that share the channels of a tile (128 bytes of tokens per row, 128 rows per
+// block) and walk the tiles.  The copy engine fills a ring of three stages (x2, dy, f, dx2 of one tile).  While the per-token
+// sums of tile j travel, the rows of tile j-1 are finished, so neither the copies nor the exchange stand in the way:
 //
 //   16 warps        sums of tile j | factors of tile j-1 arrive | sums of j on their way | rows of tile j-1 read again, written
 //   exchange warp   sums of the tokens that this block owns, from all blocks of the cluster -> factors -> to all of them
@@ -84,12 +84,14 @@ struct BrLayout {                            // shared memory behind the ring
 };
 constexpr size_t BR_SMEM = 1024 + (size_t)BR_STAGES * 4 * BR_BOX + sizeof(BrLayout);
 
-// POST: there is a norm behind the block; DX2: a gradient arrives at x2; FULL: 128 channels in every block.  (As conditions at
-// run time inside the unrolled rows they cost a quarter of the instructions.)
-template <typename T, bool POST, bool DX2, bool FULL>
+// POST: there is a norm behind the block; DX2: a gradient arrives at x2.  (As conditions at run time inside the unrolled rows
+// they cost a quarter of the instructions.)  Every block has all of its 128 rows: a condition per row, for a number of channels
+// that is no multiple of 128, keeps the loads of the rows from being started together (198 -> 340 us; the cluster form takes
+// 245).
+template <typename T, bool POST, bool DX2>
 __global__ void __launch_bounds__(BR_THREADS, 1)
 block_norm_bwd_ring_kernel(const __grid_constant__ BrMaps maps, T *__restrict__ dx, T *__restrict__ df, float *__restrict__ partial, const float *__restrict__ w_post,
-                           const float *__restrict__ gate, const float *__restrict__ w_pre, BnShape sh, int rows, int tiles, ane_cuda_status *status) {
+                           const float *__restrict__ gate, const float *__restrict__ w_pre, BnShape sh, int tiles, ane_cuda_status *status) {
     using Word = BrWord<T>;
     constexpr int W = Word::W, TW = 32 * W;
     extern __shared__ uint8_t raw[];
@@ -100,11 +102,9 @@ block_norm_bwd_ring_kernel(const __grid_constant__ BrMaps maps, T *__restrict__ 
     const uint32_t blocks = bn_size(), rank = bn_rank();
     const int clusters = gridDim.x / blocks, first = blockIdx.x / blocks;
     const int n_items = first < tiles ? (tiles - first + clusters - 1) / clusters : 0;
-    const int c0 = (int)rank * rows;
-    const int mine = c0 >= sh.C ? 0 : sh.C - c0 < rows ? sh.C - c0 : rows;      // channels of this block
+    const int c0 = (int)rank * BR_ROWS;
     const int per_owner = (TW + (int)blocks - 1) / (int)blocks;
     const int own0 = (int)rank * per_owner, own = own0 >= TW ? 0 : TW - own0 < per_owner ? TW - own0 : per_owner;
-    const uint32_t box = (uint32_t)rows * 128;                            // bytes of one tensor's tile
     if (threadIdx.x == 0) {
         for (int i = 0; i < BR_STAGES; i++) { mbar_init(&L.full[i], 1); mbar_init(&L.empty[i], BR_WARPS); }
         mbar_init(&L.mail_bar, 1);
@@ -128,7 +128,7 @@ block_norm_bwd_ring_kernel(const __grid_constant__ BrMaps maps, T *__restrict__ 
                 if (*give_up) break;
                 const int b = tile / sh.tiles_per_seq, t0 = (tile - b * sh.tiles_per_seq) * TW;
                 uint8_t *to = ring + (size_t)st * 4 * BR_BOX;
-                mbar_arrive_expect_tx(&L.full[st], (DX2 ? 4 : 3) * box);
+                mbar_arrive_expect_tx(&L.full[st], (DX2 ? 4 : 3) * BR_BOX);
                 for (int i = 0; i < (DX2 ? 4 : 3); i++) tma_load_3d(to + i * BR_BOX, &maps.t[i], t0, c0, b, &L.full[st]);
                 issued = it + 1;
             }
@@ -137,7 +137,7 @@ block_norm_bwd_ring_kernel(const __grid_constant__ BrMaps maps, T *__restrict__ 
                 for (int it = issued > BR_STAGES ? issued - BR_STAGES : 0; it < issued; it++) mbar_wait_bounded(&L.full[it % BR_STAGES], (it / BR_STAGES) & 1);
         }
     } else if (warp == BR_WARPS) {
-        const BnBwd<64> factors = {1.0f / (float)sh.C, sh.eps, sh.alpha, POST};
+        const BnBwd<64> factors = {1.0f / (float)sh.C, sh.eps, 1.0f, POST};      // alpha is in the sums already
         for (int it = 0; it < n_items && own; it++) {
             br_wait(&L.mail_bar, it & 1, give_up);
             if (__any_sync(0xffffffffu, *give_up)) break;
@@ -161,47 +161,61 @@ block_norm_bwd_ring_kernel(const __grid_constant__ BrMaps maps, T *__restrict__ 
         }
     } else {
         const bool want_p = POST || gate;
-        const int nr = mine <= warp ? 0 : (mine - warp + BR_WARPS - 1) / BR_WARPS;     // rows warp, warp + 16, ... of this warp
-        float k2[BR_NR], kw[BR_NR], k1[BR_NR], k1_last[BR_NR];                        // w_pre, w_post, gate * w_post of this tile and the last
+        const int row0 = c0 + warp;                // rows row0, row0 + 16, ... of this warp
+        // w_pre, and alpha * gate * w_post.  A gate per sequence: of sequence k1_of, read again when another one is needed (two
+        // sets would not fit the registers).
+        V<W> k2[BR_NR], k1[BR_NR];
+        int k1_of = 0;
+        auto load_k1 = [&](int b) {
+            k1_of = b;
 #pragma unroll
-        for (int k = 0; k < BR_NR; k++) {
-            const int c = c0 + warp + k * BR_WARPS;
-            k2[k] = FULL || k < nr ? w_pre[c] : 0.0f;
-            kw[k] = (FULL || k < nr) && POST ? w_post[c] : 1.0f;
-            k1[k] = k1_last[k] = kw[k] * ((FULL || k < nr) && gate && !sh.gate_stride ? gate[c] : 1.0f);
-        }
+            for (int k = 0; k < BR_NR; k++) {
+                const int c = row0 + k * BR_WARPS;
+                float v = sh.alpha;
+                if constexpr (POST) v *= __ldg(w_post + c);
+                if (gate) v *= __ldg(gate + (size_t)b * sh.gate_stride + c);
+                k1[k] = V<W>::splat(v);
+            }
+        };
+#pragma unroll
+        for (int k = 0; k < BR_NR; k++) k2[k] = V<W>::splat(__ldg(w_pre + row0 + k * BR_WARPS));
+        load_k1(0);
+        // this thread's share of the exchange: one sum over the warps, and where it goes
+        static_assert(6 * TW <= BR_WARPS * 32, "one sum per thread");
+        const bool sends = threadIdx.x < 6 * TW;
+        const float *red_at = &L.red[0][sends ? threadIdx.x / TW : 0][threadIdx.x % TW];
+        const int owner = (int)(threadIdx.x % TW) / per_owner, at_owner = (int)(threadIdx.x % TW) - owner * per_owner;
+        const int own_there = TW - owner * per_owner < per_owner ? TW - owner * per_owner : per_owner;
+        const uint32_t send_at = sends ? br_at(smem_u32(&L.mail[((int)rank * 6 + threadIdx.x / TW) * own_there + at_owner]), owner) : 0;
+        const uint32_t send_bar = sends ? br_at(smem_u32(&L.mail_bar), owner) : 0;
+        const size_t step = (size_t)BR_WARPS * sh.S;
         size_t base_last = 0;
-        int tile_last = 0;
+        int tile_last = 0, b_last = 0;
         bool active_last = false;
         for (int it = 0; it <= n_items; it++) {
             const bool cur = it < n_items;
-            const int tile = first + it * clusters, b = cur ? tile / sh.tiles_per_seq : 0;
+            const int tile = first + it * clusters, b = cur ? tile / sh.tiles_per_seq : b_last;
             const int t = (tile - b * sh.tiles_per_seq) * TW + lane * W;
             V<W> s[6];
             if (cur) {
-                if (sh.gate_stride) {
-#pragma unroll
-                    for (int k = 0; k < BR_NR; k++)
-                        if (FULL || k < nr) k1[k] = kw[k] * __ldg(gate + (size_t)b * sh.gate_stride + c0 + warp + k * BR_WARPS);
-                }
+                if (sh.gate_stride && k1_of != b) load_k1(b);
                 br_wait(&L.full[it % BR_STAGES], (it / BR_STAGES) & 1, give_up);
                 const uint32_t *w = reinterpret_cast<const uint32_t *>(ring + (size_t)(it % BR_STAGES) * 4 * BR_BOX) + warp * 32 + lane;
 #pragma unroll
                 for (int i = 0; i < 6; i++) s[i] = V<W>::splat(0.0f);
 #pragma unroll
-                for (int k = 0; k < BR_NR; k++)
-                    if (FULL || k < nr) {
-                        const uint32_t *r = w + k * BR_WARPS * 32;
-                        const V<W> vx = Word::get(r[0]), va = vscale(Word::get(r[BR_BOX / 4]), k2[k]);
-                        s[0] = vfma(vx, vx, s[0]);
-                        s[1] = vfma(va, vx, s[1]);
-                        if constexpr (POST) {
-                            const V<W> vf = Word::get(r[2 * (BR_BOX / 4)]), vq = vscale(vf, k1[k]);
-                            s[2] = vfma(vf, vf, s[2]);
-                            if constexpr (DX2) s[3] = vfma(vq, Word::get(r[3 * (BR_BOX / 4)]), s[3]);
-                            s[4] = vfma(vq, va, s[4]);
-                            s[5] = vfma(vq, vx, s[5]);
-                        }
+                for (int k = 0; k < BR_NR; k++) {
+                    const uint32_t *r = w + k * BR_WARPS * 32;
+                    const V<W> vx = Word::get(r[0]), va = vmul(Word::get(r[BR_BOX / 4]), k2[k]);
+                    s[0] = vfma(vx, vx, s[0]);
+                    s[1] = vfma(va, vx, s[1]);
+                    if constexpr (POST) {
+                        const V<W> vf = Word::get(r[2 * (BR_BOX / 4)]), vq = vmul(vf, k1[k]);
+                        s[2] = vfma(vf, vf, s[2]);
+                        if constexpr (DX2) s[3] = vfma(vq, Word::get(r[3 * (BR_BOX / 4)]), s[3]);
+                        s[4] = vfma(vq, va, s[4]);
+                        s[5] = vfma(vq, vx, s[5]);
+                    }
                     }
             }
             V<W> r2, nk, rf, nj;
@@ -218,37 +232,35 @@ block_norm_bwd_ring_kernel(const __grid_constant__ BrMaps maps, T *__restrict__ 
                 for (int i = 0; i < 6; i++) br_store(&L.red[warp][i][lane * W], s[i]);
             }
             asm volatile("bar.sync 1, %0;" ::"n"(BR_WARPS * 32) : "memory");
-            if (cur) {
-                for (int i = threadIdx.x; i < 6 * TW; i += BR_WARPS * 32) {
-                    const int k = i / TW, j = i % TW;
-                    float a = 0.0f;
+            if (cur && sends) {
+                float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                    for (int x = 0; x < BR_WARPS; x++) a += L.red[x][k][j];
-                    const int owner = j / per_owner, at = j - owner * per_owner;
-                    const int own_there = TW - owner * per_owner < per_owner ? TW - owner * per_owner : per_owner;
-                    br_send(br_at(smem_u32(&L.mail[((int)rank * 6 + k) * own_there + at]), owner), br_at(smem_u32(&L.mail_bar), owner), a);
-                }
+                for (int i = 0; i < BR_WARPS; i++) x[i & 3] += red_at[i * 6 * 64];
+                br_send(send_at, send_bar, (x[0] + x[1]) + (x[2] + x[3]));
             }
             if (it > 0) {
+                if (sh.gate_stride && k1_of != b_last) load_k1(b_last);
                 const int st = (it - 1) % BR_STAGES;
                 const uint32_t *w = reinterpret_cast<const uint32_t *>(ring + (size_t)st * 4 * BR_BOX) + warp * 32 + lane;
                 float sums[2 * BR_NR];
+                T *px = dx + base_last, *pf = df + base_last;
 #pragma unroll
                 for (int k = 0; k < BR_NR; k++) {
-                    sums[2 * k] = sums[2 * k + 1] = 0.0f;
-                    if (FULL || k < nr) {
-                        const uint32_t *r = w + k * BR_WARPS * 32;
-                        const V<W> vx = Word::get(r[0]), vy = Word::get(r[BR_BOX / 4]), vf = Word::get(r[2 * (BR_BOX / 4)]);
-                        V<W> G = vfma(vscale(vy, k2[k]), r2, vmul(nk, vx));
-                        if constexpr (DX2) G = vadd(G, Word::get(r[3 * (BR_BOX / 4)]));
-                        sums[2 * k] = br_hsum(vmul(vy, vmul(vx, r2)));
-                        sums[2 * k + 1] = br_hsum(vmul(vmul(vf, rf), G));
-                        if (active_last) {
-                            const size_t at = base_last + (size_t)k * BR_WARPS * sh.S;
-                            __stcs(reinterpret_cast<unsigned int *>(dx + at), Word::put(G));
-                            __stcs(reinterpret_cast<unsigned int *>(df + at), Word::put(vfma(vscale(G, sh.alpha * k1_last[k]), rf, vmul(nj, vf))));
-                        }
+                    const uint32_t *r = w + k * BR_WARPS * 32;
+                    const V<W> vx = Word::get(r[0]), vf = Word::get(r[2 * (BR_BOX / 4)]);
+                    const V<W> u = vmul(Word::get(r[BR_BOX / 4]), r2);                     // dy * r_2
+                    V<W> G;
+                    if constexpr (DX2) G = vfma(u, k2[k], vfma(nk, vx, Word::get(r[3 * (BR_BOX / 4)])));
+                    else G = vfma(u, k2[k], vmul(nk, vx));
+                    const V<W> h = vmul(G, rf);
+                    sums[2 * k] = br_hsum(vmul(u, vx));
+                    sums[2 * k + 1] = br_hsum(vmul(h, vf));
+                    if (active_last) {
+                        __stcs(reinterpret_cast<unsigned int *>(px), Word::put(G));
+                        __stcs(reinterpret_cast<unsigned int *>(pf), Word::put(vfma(h, k1[k], vmul(nj, vf))));
                     }
+                    px += step;
+                    pf += step;
                 }
                 __syncwarp();
                 if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&L.empty[st])) : "memory");
@@ -266,15 +278,14 @@ block_norm_bwd_ring_kernel(const __grid_constant__ BrMaps maps, T *__restrict__ 
                     at += up ? left : 0;
                 }
                 sums[0] += __shfl_xor_sync(0xffffffffu, sums[0], 1);
-                if (!(lane & 1) && at / 2 < nr && ((at & 1) == 0 || want_p))
-                    partial[((size_t)tile_last * sh.C + c0 + warp + at / 2 * BR_WARPS) * 2 + (at & 1)] = sums[0];
+                if (!(lane & 1) && ((at & 1) == 0 || want_p))
+                    partial[((size_t)tile_last * sh.C + row0 + at / 2 * BR_WARPS) * 2 + (at & 1)] = sums[0];
             }
             if (cur) {
-                base_last = ((size_t)b * sh.C + c0 + warp) * sh.S + t;
+                base_last = ((size_t)b * sh.C + row0) * sh.S + t;
                 tile_last = tile;
+                b_last = b;
                 active_last = t < sh.S;
-#pragma unroll
-                for (int k = 0; k < BR_NR; k++) k1_last[k] = k1[k];
             }
         }
     }
