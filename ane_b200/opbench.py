@@ -23,10 +23,11 @@ SEQ, DIM, HIDDEN, QD, KVD, HD, VOCAB = 2048, 1024, 3072, 2048, 1024, 128, 151936
 DEFAULT_SETS = 4
 
 
-def _cases(torch, ops, device, M, shape=None):
+def _cases(torch, ops, device, M, shape=None, step_ops=False):
     """name -> (builder) ; builder() returns (fn(i), algorithmic bytes per launch, default iterations).
     shape: optional dict(dim=, hidden=, seq=, dtype=) for the norm / residual / SwiGLU rows (the reference-native
-    Stories110M shapes are dim 768, hidden 2048, seq 256, float32)."""
+    Stories110M shapes are dim 768, hidden 2048, seq 256, float32).  step_ops: also the norms around a block, the loss head and
+    the step over a list of tensors."""
     shape = shape or {}
     S, D, H = shape.get("seq", SEQ), shape.get("dim", DIM), shape.get("hidden", HIDDEN)
     bf = shape.get("dtype", torch.bfloat16)
@@ -194,7 +195,50 @@ def _cases(torch, ops, device, M, shape=None):
         out = [torch.empty((Vc, D), device=device) for _ in range(2)]
         return (lambda i: ops.vocab_compact_embed(full, c2f, cnt, Vc, out=out[i % 2])), 2 * Vc * D * 4 + Vc * 4, 20
 
-    return {
+    # the norms around a block (gate per sequence), the loss head without logits (an eighth of the sequences: bound by its
+    # products, its bytes are those of x, the table, the targets and the gradients) and AdamW over a list of tensors
+    def block_norm():
+        xs, fs, x2, y = mk(D), mk(D), mk(D), mk(D)
+        w, v, g = torch.ones(D, device=device), torch.ones(D, device=device), torch.ones((M, D), device=device)
+        return (lambda i: ops.block_norm(xs[i % NSET], fs[i % NSET], w, w_post=v, gate=g, alpha=0.13, x2=x2[i % NSET], y=y[i % NSET])), 4 * D * T * e, 20
+
+    def block_norm_bwd():
+        dy, dx2, xs, fs, dx, df = (mk(D, n=2) for _ in range(6))
+        w, v, g = torch.ones(D, device=device), torch.ones(D, device=device), torch.ones((M, D), device=device)
+        dw, dv, dg = torch.zeros(D, device=device), torch.zeros(D, device=device), torch.zeros((M, D), device=device)
+        return (lambda i: ops.block_norm_bwd(dy[i % 2], xs[i % 2], fs[i % 2], w, dw, w_post=v, dw_post=dv, gate=g, dgate=dg, dx2=dx2[i % 2], alpha=0.13, dx=dx[i % 2],
+                                             df=df[i % 2])), 6 * D * T * e, 20
+
+    def linear_cross_entropy(grad=True):
+        Bc = max(1, M // 8)
+        xs = mk(D, n=2, b=Bc)
+        table = (torch.randn((VOCAB, D), device=device) * D ** -0.5).to(bf)
+        tg = torch.randint(0, VOCAB, (Bc, S), device=device, dtype=torch.int32)
+        dE = torch.zeros((VOCAB, D), device=device) if grad else None
+        read = (VOCAB * D + Bc * S * D) * e + 4 * Bc * S
+        return (lambda i: ops.linear_cross_entropy(xs[i % 2], table, tg, d_table=dE, grad=grad)), read + (Bc * S * D * e + 8 * VOCAB * D if grad else 0), 5
+
+    def _tensors(q8):
+        n, wv, gv, mv, vv = _flat()
+        cut = [t.view(-1, 1 << 20) for t in (wv, gv)]
+        w, g = (list(t.unbind(0)) for t in cut)
+        if not q8:
+            return n, ops.AdamTensors(w, g, list(mv.view(-1, 1 << 20).unbind(0)), list(vv.view(-1, 1 << 20).unbind(0)), wd=0.1)
+        m, v = (torch.zeros((len(w), 1 << 20), dtype=torch.uint8, device=device) for _ in range(2))
+        ms, vs = (torch.zeros((len(w), 1 << 12), device=device) for _ in range(2))
+        return n, ops.AdamTensors(w, g, list(m.unbind(0)), list(v.unbind(0)), m_scale=list(ms.unbind(0)), v_scale=list(vs.unbind(0)), wd=0.1)
+
+    def adam_multi():
+        n, tensors = _tensors(False)
+        return (lambda i: ops.adam_multi(tensors, 1 + i, 3e-4, 0.9, 0.95, 1e-8)), 28 * n, 20
+
+    def adam_multi_8bit():
+        n, tensors = _tensors(True)
+        return (lambda i: ops.adam_multi(tensors, 1 + i, 3e-4, 0.9, 0.95, 1e-8, seed=i)), 16 * n, 20
+
+    step = {"block_norm": block_norm, "block_norm_bwd": block_norm_bwd, "linear_cross_entropy": linear_cross_entropy,
+            "linear_cross_entropy_loss": lambda: linear_cross_entropy(False), "adam_multi": adam_multi, "adam_multi_8bit": adam_multi_8bit}
+    return (step if step_ops else {}) | {
         "gqa_tile": gqa_tile, "gqa_reduce": gqa_reduce, "qknorm_rope_tiled(K)": qknorm_rope_tiled,
         "rope_qknorm_bwd_gqa(K)": rope_qknorm_bwd_gqa, "convert_f32_bf16": convert_f32_bf16,
         "vocab_compact_embed": vocab_compact_embed,
@@ -274,10 +318,10 @@ def sustain_op(torch, builder, peak_gbs, seconds):
             "power_w": round(watts), "sm_mhz": mhz, "pJ_per_byte": round(watts * ms * 1e-3 / nbytes * 1e12, 1), "launches": n, "bytes": nbytes}
 
 
-def per_op_table(torch, ops, device, peak_gbs, batch=32, only=None, iters=None, warmup=5, shape=None, sustain=0.0):
+def per_op_table(torch, ops, device, peak_gbs, batch=32, only=None, iters=None, warmup=5, shape=None, sustain=0.0, step_ops=False):
     """Achieved GB/s per operator on benchmark-sized bf16 tensors (algorithmic bytes / time)."""
     res = {}
-    for name, builder in _cases(torch, ops, device, batch, shape).items():
+    for name, builder in _cases(torch, ops, device, batch, shape, step_ops).items():
         if only and name not in only:
             continue
         res[name] = sustain_op(torch, builder, peak_gbs, sustain) if sustain > 0 else time_op(torch, builder, peak_gbs, iters, warmup)
@@ -337,7 +381,7 @@ def main(argv=None):
     shape = {k: v for k, v in (("dim", a.dim), ("hidden", a.hidden), ("seq", a.seq), ("sets", a.sets)) if v}
     if a.dtype:
         shape["dtype"] = getattr(torch, a.dtype)
-    table = per_op_table(torch, ops, torch.device("cuda:0"), peak, a.batch, a.op, a.iters, a.warmup, shape or None, a.sustain)
+    table = per_op_table(torch, ops, torch.device("cuda:0"), peak, a.batch, a.op, a.iters, a.warmup, shape or None, a.sustain, step_ops=True)
     print(json.dumps({"batch": a.batch, "peak_gbs": peak, "peak_kind": kind, "sustain_s": a.sustain, "ops": table}))
 
 
