@@ -674,6 +674,185 @@ __global__ void __launch_bounds__(256) lx_finish_dx_kernel(T *__restrict__ dx, c
     }
 }
 
+// ------------------------------------------------------------------ one to four tokens
+// For so few tokens the operator is the table read once (and once more, with its gradient read and written, for the gradients):
+// plain fp32 arithmetic on the elements as they are, bound by HBM.  A tile of the tensor cores would be 252 rows of nothing,
+// and fp32 tables would have to be packed first.  The few logits of a row are kept for the second pass, [V][T].
+// Against the tensor cores, 151936 rows x 1024 channels, losses / with gradients: fp32 1 token 126 / 435 against 516 / 1176 us,
+// 4 tokens 188 / 583 against 548 / 1228; bf16 1 token 63 / 445 against 76 / 494, 2 tokens 145 / 517 against 72 / 493.  Hence four
+// tokens in fp32 and one in 16 bits.
+constexpr int LF_TOKENS = 4;
+constexpr size_t LF_SMEM = 96 << 10;                     // of x as fp32
+
+template <typename T> __device__ __forceinline__ void lf_x_to_shared(float *xs, const T *x, const void *targets, int id_u16, int V, int tokens, int D, int S) {
+    for (int i = threadIdx.x; i < tokens * D; i += blockDim.x) {
+        const int t = i / D, d = i - t * D;
+        xs[i] = lx_target(targets, id_u16, V, t) >= 0 ? Elt<T>::to_f(x[((size_t)(t / S) * D + d) * S + t % S]) : 0.0f;
+    }
+}
+
+// A warp takes two rows at a time; per block a (max, sum) pair per token over its rows.
+template <typename T, int VEC, int TOK>
+__global__ void __launch_bounds__(256) lf_logits_kernel(float *__restrict__ logits, float2 *__restrict__ part, float *__restrict__ hit, const T *__restrict__ x,
+                                                        const T *__restrict__ table, const void *__restrict__ targets, int id_u16, int V, int D, int S, size_t ldt) {
+    extern __shared__ float xs[];
+    __shared__ float2 sh[8][TOK];
+    dep_sync();
+    lf_x_to_shared(xs, x, targets, id_u16, V, TOK, D, S);
+    __syncthreads();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int step = 2 * 8 * gridDim.x;
+    float m[TOK], s[TOK];
+#pragma unroll
+    for (int t = 0; t < TOK; t++) { m[t] = -INFINITY; s[t] = 0.0f; }
+    for (int v = 2 * (blockIdx.x * 8 + warp); v < V; v += step) {
+        const T *row = table + (size_t)v * D, *next = v + 1 < V ? row + D : row;
+        float a[2][TOK];
+#pragma unroll
+        for (int t = 0; t < TOK; t++) a[0][t] = a[1][t] = 0.0f;
+#pragma unroll 2
+        for (int d = lane * VEC; d < D; d += 32 * VEC) {
+            Raw<T, VEC> r[2];
+            r[0].load_stream(row + d);
+            r[1].load_stream(next + d);
+            float e[2][VEC];
+            r[0].unpack(e[0]);
+            r[1].unpack(e[1]);
+#pragma unroll
+            for (int t = 0; t < TOK; t++)
+#pragma unroll
+                for (int j = 0; j < VEC; j++) {
+                    const float q = xs[t * D + d + j];
+                    a[0][t] = fmaf(e[0][j], q, a[0][t]);
+                    a[1][t] = fmaf(e[1][j], q, a[1][t]);
+                }
+        }
+#pragma unroll
+        for (int r = 0; r < 2; r++)
+#pragma unroll
+            for (int t = 0; t < TOK; t++) a[r][t] = warp_sum(a[r][t]);
+#pragma unroll
+        for (int r = 0; r < 2; r++)
+            if (v + r < V) {
+#pragma unroll
+                for (int t = 0; t < TOK; t++) {
+                    const float l2 = a[r][t] * LX_LOG2E, mn = fmaxf(m[t], l2);
+                    s[t] = s[t] * lx_exp2(m[t] - mn) + lx_exp2(l2 - mn);
+                    m[t] = mn;
+                    if (lane == t) {
+                        if (logits) logits[(size_t)(v + r) * TOK + t] = a[r][t];
+                        if (lx_target(targets, id_u16, V, t) == v + r) hit[t] = a[r][t];
+                    }
+                }
+            }
+    }
+    if (lane == 0)
+#pragma unroll
+        for (int t = 0; t < TOK; t++) sh[warp][t] = make_float2(m[t], s[t]);
+    __syncthreads();
+    if (threadIdx.x < TOK) {
+        float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 8; w++) top = fmaxf(top, sh[w][threadIdx.x].x);
+#pragma unroll
+        for (int w = 0; w < 8; w++) if (sh[w][threadIdx.x].y != 0.0f) sum += sh[w][threadIdx.x].y * lx_exp2(sh[w][threadIdx.x].x - top);
+        part[(size_t)blockIdx.x * ldt + threadIdx.x] = make_float2(top, sum);
+    }
+}
+
+// Rows [v0, v1) of a block, columns of blockIdx.y: d_table += dl x^T, and the block's share of dx, [chunk][TOK][D].
+constexpr int LF_ROWS = 64;                              // dl of this many rows at a time
+template <typename T, int VEC, int TOK>
+__global__ void __launch_bounds__(256) lf_grads_kernel(float *__restrict__ dx_part, float *__restrict__ d_table, const float *__restrict__ logits, const float *__restrict__ lse2,
+                                                       const T *__restrict__ x, const T *__restrict__ table, const void *__restrict__ targets, int id_u16, int V, int D, int S,
+                                                       int chunk, float alpha) {
+    __shared__ float dl[LF_ROWS][TOK];
+    dep_sync();
+    const int d = (blockIdx.y * 256 + threadIdx.x) * VEC;
+    const bool live = d < D;
+    float q[TOK][VEC], acc[TOK][VEC];
+#pragma unroll
+    for (int t = 0; t < TOK; t++)
+#pragma unroll
+        for (int j = 0; j < VEC; j++) {
+            acc[t][j] = 0.0f;
+            q[t][j] = live && lx_target(targets, id_u16, V, t) >= 0 ? Elt<T>::to_f(x[((size_t)(t / S) * D + d + j) * S + t % S]) * alpha : 0.0f;
+        }
+    const int v0 = blockIdx.x * chunk, v1 = v0 + chunk < V ? v0 + chunk : V;
+    for (int r0 = v0; r0 < v1; r0 += LF_ROWS) {
+        const int rows = v1 - r0 < LF_ROWS ? v1 - r0 : LF_ROWS;
+        __syncthreads();
+        for (int i = threadIdx.x; i < rows * TOK; i += 256) {
+            const int t = i % TOK, v = r0 + i / TOK, id = lx_target(targets, id_u16, V, t);
+            const float p = lx_exp2(fmaf(logits[(size_t)r0 * TOK + i], LX_LOG2E, -lse2[t]));
+            dl[i / TOK][t] = id < 0 ? 0.0f : id == v ? p - 1.0f : p;
+        }
+        __syncthreads();
+        if (live) {
+#pragma unroll 4
+            for (int r = 0; r < rows; r++) {
+                float k[TOK];
+#pragma unroll
+                for (int t = 0; t < TOK; t++) k[t] = dl[r][t];
+                const size_t at = (size_t)(r0 + r) * D + d;
+                if (dx_part) {
+                    Raw<T, VEC> e;
+                    float f[VEC];
+                    e.load_stream(table + at);
+                    e.unpack(f);
+#pragma unroll
+                    for (int t = 0; t < TOK; t++)
+#pragma unroll
+                        for (int j = 0; j < VEC; j++) acc[t][j] = fmaf(k[t], f[j], acc[t][j]);
+                }
+                if (d_table) {
+                    if constexpr (VEC % 4 == 0) {
+#pragma unroll
+                        for (int h = 0; h < VEC; h += 4) {
+                            float4 g = __ldcs(reinterpret_cast<const float4 *>(d_table + at + h));
+#pragma unroll
+                            for (int t = 0; t < TOK; t++) {
+                                g.x = fmaf(k[t], q[t][h], g.x); g.y = fmaf(k[t], q[t][h + 1], g.y);
+                                g.z = fmaf(k[t], q[t][h + 2], g.z); g.w = fmaf(k[t], q[t][h + 3], g.w);
+                            }
+                            __stcs(reinterpret_cast<float4 *>(d_table + at + h), g);
+                        }
+                    } else {
+                        float g = d_table[at];
+#pragma unroll
+                        for (int t = 0; t < TOK; t++) g = fmaf(k[t], q[t][0], g);
+                        d_table[at] = g;
+                    }
+                }
+            }
+        }
+    }
+    if (dx_part && live)
+#pragma unroll
+        for (int t = 0; t < TOK; t++)
+#pragma unroll
+            for (int j = 0; j < VEC; j++) dx_part[((size_t)blockIdx.x * TOK + t) * D + d + j] = acc[t][j];
+}
+
+// dx[b][d][s] = alpha * sum over the chunks, in order: eight slices of them per column.
+template <typename T>
+__global__ void __launch_bounds__(256) lf_finish_dx_kernel(T *__restrict__ dx, const float *__restrict__ part, int chunks, int tokens, int D, int S, float alpha) {
+    __shared__ float sh[8][33];
+    dep_sync();
+    const int cl = threadIdx.x & 31, sl = threadIdx.x >> 5, d = blockIdx.x * 32 + cl, t = blockIdx.y;
+    float a = 0.0f;
+    if (d < D)
+#pragma unroll 4
+        for (int i = sl; i < chunks; i += 8) a += part[((size_t)i * tokens + t) * D + d];
+    sh[sl][cl] = a;
+    __syncthreads();
+    if (sl != 0 || d >= D) return;
+    a = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) a += sh[i][cl];
+    dx[((size_t)(t / S) * D + d) * S + t % S] = Elt<T>::from_f(a * alpha);
+}
+
 // loss_seq[b] = (sum_t loss_tok[b][t]) / S, fixed summation tree.
 __global__ void __launch_bounds__(256) lx_loss_kernel(float *__restrict__ loss_seq, const float *__restrict__ loss_tok, int S) {
     __shared__ float sh[8];
@@ -802,7 +981,57 @@ static LxPlan lx_plan(int T_all, int D, int V, int segs, bool dx, bool d_table, 
     return p;
 }
 
+template <typename T, int VEC, int TOK> static int lf_run(const LxCall &c) {
+    const bool grad = c.dx || c.d_table;
+    const int D = c.D, V = c.V;
+    const int blocks = lx_div(V, 16) < 4 * ctx().sm_count ? lx_div(V, 16) : 4 * ctx().sm_count;
+    const int cols = lx_div(D, 256 * VEC);
+    int chunks = lx_div(4 * ctx().sm_count, cols);
+    if (chunks > lx_div(V, 8)) chunks = lx_div(V, 8);
+    const int chunk = lx_div(V, chunks);
+    chunks = lx_div(V, chunk);
+    size_t off = 0;
+    auto take = [&](size_t bytes) { const size_t at = off; off += round_up(bytes, 1024); return at; };
+    const size_t o_tok = take(LF_TOKENS * 4), o_lse = take(LF_TOKENS * 4), o_hit = take(LF_TOKENS * 4), o_part = take((size_t)blocks * LF_TOKENS * 8);
+    const size_t o_logits = take(grad ? (size_t)V * TOK * 4 : 0), o_dx = take(c.dx ? (size_t)chunks * TOK * D * 4 : 0);
+    char *ws = static_cast<char *>(workspace(off));
+    if (!ws) return fail(ANE_CUDA_ERR_NOMEM, "ane_cuda_linear_cross_entropy_dev: no scratch (%zu bytes)", off);
+    float *loss_tok = c.loss_tok ? c.loss_tok : reinterpret_cast<float *>(ws + o_tok), *lse2 = reinterpret_cast<float *>(ws + o_lse), *hit = reinterpret_cast<float *>(ws + o_hit);
+    float *logits = grad ? reinterpret_cast<float *>(ws + o_logits) : nullptr, *dxs = c.dx ? reinterpret_cast<float *>(ws + o_dx) : nullptr;
+    float2 *part = reinterpret_cast<float2 *>(ws + o_part);
+    const T *x = static_cast<const T *>(c.x), *table = static_cast<const T *>(c.table);
+    static bool ready = false;
+    if (!ready) {
+        ANE_CUDA_TRY(cudaFuncSetAttribute(lf_logits_kernel<T, VEC, TOK>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)LF_SMEM));
+        ready = true;
+    }
+    lx_call(lf_logits_kernel<T, VEC, TOK>, dim3(blocks), dim3(256), (size_t)TOK * D * 4, c.st, logits, part, hit, x, table, c.targets, c.id_u16, V, D, c.S, (size_t)LF_TOKENS);
+    lx_call(lx_join_kernel<4>, dim3(1), dim3(1024), 0, c.st, lse2, loss_tok, part, hit, c.targets, c.id_u16, V, blocks, TOK, (size_t)LF_TOKENS, ctx().status);
+    ANE_LAUNCH_OK(2);
+    const float alpha = c.grad_scale / (float)c.S;
+    if (grad) {
+        lx_call(lf_grads_kernel<T, VEC, TOK>, dim3(chunks, cols), dim3(256), 0, c.st, dxs, c.d_table, logits, lse2, x, table, c.targets, c.id_u16, V, D, c.S, chunk, alpha);
+        ANE_LAUNCH_OK(1);
+    }
+    if (c.dx) {
+        lx_call(lf_finish_dx_kernel<T>, dim3(lx_div(D, 32), TOK), dim3(256), 0, c.st, static_cast<T *>(c.dx), dxs, chunks, TOK, D, c.S, alpha);
+        ANE_LAUNCH_OK(1);
+    }
+    lx_call(lx_loss_kernel, dim3(c.B), dim3(256), 0, c.st, c.loss_seq, loss_tok, c.S);
+    ANE_LAUNCH_OK(1);
+    return ANE_CUDA_OK;
+}
+
 template <typename T, typename H> static int lx_run(const LxCall &c) {
+    if (c.B * c.S <= (sizeof(T) == 4 ? LF_TOKENS : 1) && (size_t)c.B * c.S * c.D * 4 <= LF_SMEM && c.V < (1 << 29) && tuning("linear_xent_few", 1)) {
+        const bool vec = c.D % Elt<T>::VEC == 0 && aligned16(c.table) && aligned16(c.d_table);
+        switch (c.B * c.S) {
+            case 1: return vec ? lf_run<T, Elt<T>::VEC, 1>(c) : lf_run<T, 1, 1>(c);
+            case 2: return vec ? lf_run<T, Elt<T>::VEC, 2>(c) : lf_run<T, 1, 2>(c);
+            case 3: return vec ? lf_run<T, Elt<T>::VEC, 3>(c) : lf_run<T, 1, 3>(c);
+            default: return vec ? lf_run<T, Elt<T>::VEC, 4>(c) : lf_run<T, 1, 4>(c);
+        }
+    }
     const bool split = sizeof(T) == 4;                       // fp32 inputs as two parts
     const ane_dtype part = c.dtype == ANE_BF16 ? ANE_BF16 : ANE_F16;
     const int half_type = part == ANE_F16;

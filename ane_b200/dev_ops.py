@@ -305,30 +305,33 @@ class AdamTensors:
         if self.copy_dtype == _l.F32:
             raise ValueError("copy: bf16 or fp16 tensors")
         state = torch.uint8 if self.q8 else torch.float32
-        written = []
+        kinds = (torch.float32, g[0].dtype if count else None, state, state, torch.float32, torch.float32, copy[0].dtype if count and copy is not None else None)
+        names = ("w", "g", "m", "v", "m_scale", "v_scale", "copy")
+        self.tensors = (list(w), list(g), list(m), list(v), m_scale and list(m_scale), v_scale and list(v_scale), copy and list(copy))
+        self.items = (_l.AdamItem * count)()
+        self.count, self.wd = count, wd
+        written, rows = [], []
         for k in range(count):
-            shape, blocks = w[k].shape, (-(-w[k].numel() // ADAM_BLOCK),)
-            _like(f"w[{k}]", w[k], shape, torch.float32)
-            _like(f"g[{k}]", g[k], shape, g[0].dtype)
-            _like(f"m[{k}]", m[k], shape, state)
-            _like(f"v[{k}]", v[k], shape, state)
-            if self.q8:
-                _like(f"m_scale[{k}]", m_scale[k], blocks, torch.float32)
-                _like(f"v_scale[{k}]", v_scale[k], blocks, torch.float32)
-            if copy is not None:
-                _like(f"copy[{k}]", copy[k], shape, copy[0].dtype)
-            for ts in (w, m, v, m_scale, v_scale, copy):
-                if ts is not None and ts[k].numel():
-                    written.append((ts[k].data_ptr(), ts[k].data_ptr() + ts[k].numel() * ts[k].element_size()))
+            n, shape = w[k].numel(), w[k].shape
+            blocks = (-(-n // ADAM_BLOCK),)
+            for i, ts in enumerate(self.tensors):
+                want = blocks if i in (4, 5) else shape
+                if ts is not None and (ts[k].dtype != kinds[i] or ts[k].shape != want):
+                    _like(f"{names[i]}[{k}]", ts[k], want, kinds[i])
+            rows.append((n, [None if ts is None else ts[k] for ts in self.tensors]))
+            if n:
+                for i in (0, 2, 3, 4, 5, 6):
+                    t = rows[-1][1][i]
+                    if t is not None:
+                        at = t.data_ptr()
+                        written.append((at, at + t.numel() * t.element_size()))
         written.sort()
         if any(b[0] < a[1] for a, b in zip(written, written[1:])):
             raise ValueError("two tensors that the step writes share memory")
-        self.items = (_l.AdamItem * count)()
-        self.count, self.wd = count, wd
-        self.tensors = (list(w), list(g), list(m), list(v), m_scale and list(m_scale), v_scale and list(v_scale), copy and list(copy))
-        for k in range(count):
-            at = _ptrs(*(None if ts is None else ts[k] for ts in self.tensors))
-            self.items[k] = _l.AdamItem(w[k].numel(), *at, wd[k], 0)
+        for k, (n, ts) in enumerate(rows):
+            item = self.items[k]
+            item.n, item.wd = n, wd[k]
+            item.w, item.g, item.m, item.v, item.m_scale, item.v_scale, item.copy = _ptrs(*ts)
 
 
 def adam_multi(tensors, t, lr, b1, b2, eps, gscale=1.0, clip=None, seed=0, dynamic=True):

@@ -106,7 +106,8 @@ def inputs(B, D, V, S, dt, seed=0, scale=1.0, masked=0.1):
 
 # tiles of 128 tokens and 256 rows, K blocks of 64: one below, at and above them; rows that break alignment; several pieces
 SHAPES = [(1, 8, 1, 1), (1, 64, 256, 128), (2, 64, 255, 1), (1, 72, 257, 129), (3, 33, 100, 5), (1, 1, 2, 3), (2, 200, 1000, 77), (1, 768, 9200, 256),
-          (5, 130, 513, 200), (1, 256, 20000, 16), (2, 96, 5000, 1100)]
+          (5, 130, 513, 200), (1, 256, 20000, 16), (2, 96, 5000, 1100),
+          (1, 256, 777, 4), (2, 64, 1001, 2), (4, 136, 300, 1), (1, 1709, 478, 1), (1, 1032, 2000, 1), (1, 96, 5, 2)]      # one to four tokens
 
 
 @pytest.mark.gpu
@@ -131,6 +132,25 @@ def test_losses_and_gradients(ops, shape, dt):
                                              dE2.data_ptr(), x.data_ptr(), E.data_ptr(), t.data_ptr(), 0.7)
     assert rc == lib.OK and torch.equal(dE, dE2)
     assert torch.equal(ops.linear_cross_entropy(x, E, t, grad=False)[0], loss)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("knob", [("linear_xent_few", 0), ("linear_xent_wide", 0), ("linear_xent_wide", 1), ("linear_xent_dep", 0)])
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("shape", [(1, 64, 700, 1), (3, 33, 100, 1), (2, 200, 1300, 77), (1, 520, 600, 300)])
+def test_alternate_kernels(ops, shape, dt, knob):
+    B, D, V, S = shape
+    x, E, t = inputs(B, D, V, S, DT[dt], seed=10)
+    t[0, 0] = 0
+    dE = torch.zeros(V, D, device="cuda")
+    lib.set_tuning(*knob)
+    try:
+        loss, dx = ops.linear_cross_entropy(x, E, t, d_table=dE)
+    finally:
+        lib.clear_tuning(knob[0])
+    ref = reference(x, E, t)
+    assert max(off(loss, ref[0])) <= 1e-5
+    check_grads(DT[dt], dx, ref[2], dE, ref[3])
 
 
 @pytest.mark.gpu
