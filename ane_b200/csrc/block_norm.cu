@@ -291,6 +291,7 @@ template <int N> struct BnFold<N, 32> {
 template <int NS, int N, int LG, int THREADS, typename F> __device__ __forceinline__ void bn_cluster_sums(V<N> (&v)[NS], float *red, float *mine, float *tot, F finish) {
     constexpr int TW = N * LG, PER = NS < 3 ? NS : 3, WARPS = THREADS / 32;
     const int lg = threadIdx.x % LG, warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+    const uint32_t blocks = bn_size();
 #pragma unroll
     for (int s0 = 0; s0 < NS; s0 += PER) {
         float a[PER * N];
@@ -315,6 +316,21 @@ template <int NS, int N, int LG, int THREADS, typename F> __device__ __forceinli
             }
         }
         __syncthreads();
+        if constexpr (NS == 1 && N > 1 && TW <= 32) {
+            if (blocks == 1) {
+                // one block: every warp adds up the warps' parts itself, a lane per token, and no second barrier is needed (`red` is
+                // not used again by the next exchange)
+                float a = 0.0f;
+                if (lane < TW) {
+#pragma unroll
+                    for (int w = 0; w < WARPS; w++) a += red[w * TW + lane];
+                }
+                finish(&a);
+#pragma unroll
+                for (int j = 0; j < N; j++) v[0].set(j, __shfl_sync(0xffffffffu, a, lg * N + j));
+                return;
+            }
+        }
         for (int i = threadIdx.x; i < PER * TW; i += THREADS) {
             const int s = i / TW, t = i % TW;
             float a = 0.0f;
@@ -323,7 +339,6 @@ template <int NS, int N, int LG, int THREADS, typename F> __device__ __forceinli
             mine[s0 * TW + i] = a;
         }
     }
-    const uint32_t blocks = bn_size();
     if (blocks > 1) {
         bn_cluster_arrive();
         bn_cluster_wait();
@@ -389,7 +404,7 @@ block_norm_cluster_kernel(T *x2, T *y, const T *x, const T *f, const float *__re
                           const float *__restrict__ w_pre, BnShape sh, int rows) {
     constexpr int R = THREADS / LG, TW = LG * VEC;
     extern __shared__ __align__(16) uint4 strips[];
-    __shared__ __align__(16) float red[THREADS / 32 * TW], mine[2][TW], tot[TW];
+    __shared__ __align__(16) float red[2][THREADS / 32 * TW], mine[2][TW], tot[TW];
     const int tile = blockIdx.x / bn_size(), c0 = (int)bn_rank() * rows, c = c0 + threadIdx.x / LG;
     const int end = c0 + rows < sh.C ? c0 + rows : sh.C;
     const int b = tile / sh.tiles_per_seq, t = (tile - b * sh.tiles_per_seq) * TW + (int)(threadIdx.x % LG) * VEC;
@@ -408,7 +423,7 @@ block_norm_cluster_kernel(T *x2, T *y, const T *x, const T *f, const float *__re
     if (w_post) {
 #pragma unroll
         for (int k = 0; k < NV; k++) if (k < n) { const V<VEC> v = strip.get(1, k); ss[0] = vfma(v, v, ss[0]); }
-        bn_cluster_sums<1, VEC, LG, THREADS>(ss, red, mine[0], tot, rms);
+        bn_cluster_sums<1, VEC, LG, THREADS>(ss, red[0], mine[0], tot, rms);
         r = ss[0];
         ss[0] = V<VEC>::splat(0.0f);
     }
@@ -421,7 +436,7 @@ block_norm_cluster_kernel(T *x2, T *y, const T *x, const T *f, const float *__re
             const V<VEC> v = z[k].get();
             ss[0] = vfma(v, v, ss[0]);
         }
-    bn_cluster_sums<1, VEC, LG, THREADS>(ss, red, mine[1], tot, rms);
+    bn_cluster_sums<1, VEC, LG, THREADS>(ss, red[1], mine[1], tot, rms);
     bn_cluster_leave();                                   // this block has read its peers' sums
     // both results only now: a store before the exchange would have to land before its barrier opens
 #pragma unroll
