@@ -10,6 +10,10 @@
 // a shift and two products, and encoding is one addition on the bits: 20 random bits added below the kept mantissa bits,
 // then a shift.  That rounds up or down with the probability that keeps the mean.  Rounding to nearest would not do here:
 // with beta2 = 0.95 a gradient of zero takes 5 % from v and codes are 6 to 12 % apart, so v would never come down again.
+//
+// Measured, 110 M parameters in 110 tensors: fp32 moments 28 bytes a parameter, 450 us, the copy rate; 8-bit moments with bf16
+// gradients and copies 16 bytes a parameter, 340 us (5.2 TB/s): the arithmetic of the codes keeps the integer pipe busy 68 % of
+// the time and the issue slots 74 %.
 #include "common.cuh"
 
 #include <math.h>

@@ -17,7 +17,16 @@
 //   sum q G = sum q dx2 + r_2 sum q a - k sum q x2
 // -- six sums over the channels in one sweep, one exchange, then the sweep that writes.
 //
-// Both directions move each tensor once at best (4 and 6 tensor passes) and do a few operations per element: HBM-bound.
+// Both directions move each tensor once at best (4 and 6 tensor passes) and do a few operations per element, so HBM is the
+// floor; what they run into before it are the phases of a tile (loads, sums, exchange, stores), which a block goes through one
+// after the other.  Measured, 32 sequences x 2048 tokens x 1024 channels in bf16 (82 and 123 us at the copy rate):
+//   forward   115 us   one block of 512 threads per 32 tokens, two blocks per SM       (4.7 TB/s)
+//             138      clusters of eight blocks of 256 threads, 128-byte rows
+//             157      three sweeps through L2
+//   backward  199 us   pipeline over clusters (block_norm_ring.cuh), issue-bound at 15 clusters of eight  (4.0 TB/s)
+//             245      one block of 512 threads per 32 tokens; clusters of eight, 128-byte rows: 250
+//             380      two sweeps through L2
+// Rows that break 16-byte alignment (5 x 1000 x 333 in fp16): 24 us over clusters of eight against 125 us in one block per tile.
 #include "common.cuh"
 
 #include <type_traits>
@@ -652,8 +661,8 @@ static bool bn_ring(int C, const BnSplit &sp, long long tiles) {
     return sp.blocks && C % 128 == 0 && (tuning("block_norm_cluster", 7) & 4) && tiles * sp.blocks >= 4LL * ctx().sm_count;
 }
 // The cluster form for a shape, if there is one.
-//   many tiles   512 threads per block; 1024 channels to a block
-//   few tiles    256 threads, up to eight blocks per tile, so that more SMs take part
+//   many tiles   512 threads per block; 1024 channels to a block (forward 115 us against 138, backward 245 against 250, see above)
+//   few tiles    256 threads, up to eight blocks per tile, so that more SMs take part (5 us for 256 tokens x 768 channels)
 //   rows that break 16-byte alignment: element by element, 32 tokens per row, eight blocks per tile
 // -> BN_NONE: none (channels beyond eight blocks, or unaligned sequences so short that most lanes of a row would idle).
 constexpr int BN_NONE = 1;

@@ -14,6 +14,11 @@
 // Writing the logits and reading them back would take longer than the second product: 12 bytes per logit (write, read, write
 // dl) at 6.5 TB/s are 1.9 ps, 2 * 1024 operations at 1.5 PFLOP/s are 1.4 ps.
 //
+// Measured, 8192 tokens x 151936 rows x 1024 channels in bf16 (cuBLAS on this GPU: 1650 TFLOP/s in a burst, 1410 under the
+// power cap), one call at a time: stats 1.50 ms (1700 TFLOP/s), dlogits 2.27 (1120; it writes 5 GB of dl), dx 1.9 (1340), d_table
+// 3.0 for two products (1690).  Back to back under the power cap the whole call takes 10.1 ms, 1260 TFLOP/s over the five
+// products that it does and 756 over the three that the result cannot do without.
+//
 // Precision.  16-bit inputs enter the products as they are.  dl is rounded to 16 bits for dx, whose result is rounded to 16
 // bits as well; d_table is an fp32 sum, so dl enters it as two 16-bit numbers, the rounded value and what the rounding left
 // (17 bits and more), at the price of one more product.  fp32 inputs are split into two fp16 parts after scaling by a power of
@@ -208,9 +213,10 @@ struct LxRange {
 // operands.  In each block one thread copies operand boxes into a ring of stages; in the first block one thread issues the
 // matrix instructions; eight warps take the accumulators over.
 //
-// What bounds the products is the way from L2 to the SMs: with 64 bytes per SM and clock wanted by a 256 x 256 tile, the
-// tensor cores were busy 58 % of the time in all four products alike, at 8.8 TB/s of reads (8192 tokens would want 15).  So
-// the large products bring two boxes of B for each box of A (48 bytes per clock): LX_WIDE and LX_TWO.
+// A 256 x 256 tile wants 64 bytes per SM and clock from L2 and 256 x 512 wants 48, so the large products bring two boxes of B for
+// each box of A (LX_WIDE, LX_TWO): d_table went from 1137 to 1414 TFLOP/s with it.  The second half of the distance was the
+// matrix thread itself: with descriptors computed in vector registers a K block took 1450 clocks instead of the 1024 of its
+// instructions (stats 1350 -> 1590 TFLOP/s with uniform registers).
 template <int EPI, int MODE, bool HALF>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LX_THREADS, 1) lx_gemm_kernel(const __grid_constant__ LxMaps maps, const __grid_constant__ LxArgs a) {
     constexpr bool A_MN = EPI == LX_DTABLE, B_MN = EPI == LX_DX || EPI == LX_DTABLE;
@@ -875,7 +881,7 @@ static inline int lx_pairs() { return ctx().sm_count / 2; }
 
 // Every kernel of the chain is a programmatic dependent launch: its blocks may be placed and set up their barriers and
 // accumulators while the kernel before drains, and stop in dep_sync() until that one has completed.  A call has 4 to 12 short
-// launches where the problem is small: 146 -> 120 us for one fp32 sequence over 9200 rows.
+// launches where the problem is small: 130 -> 106 us for one fp32 sequence over 9200 rows.
 template <typename... KArgs, typename... Args>
 static inline void lx_call(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args &&...args) {
     cudaLaunchConfig_t cfg = {};
@@ -906,7 +912,8 @@ template <int EPI, int MODE> static int lx_start(cudaStream_t st, const LxMaps &
 }
 
 // Time of a product of `tiles` accumulators of 256 x 256 (m x n of them), in K blocks of one accumulator: waves over the SM
-// pairs.  A wide tile takes the time of 1.55 plain ones.
+// pairs.  A wide tile takes the time of 1.55 plain ones (clocks per K block, 512 for a plain accumulator's instructions: about
+// 850 plain, 1300 wide).  Losses of 16 tokens over 151936 rows: 84 us wide, 101 plain; all of 8192 tokens: 10.3 against 10.4 ms.
 constexpr double LX_WIDE_COST = 1.55;
 static double lx_cost(int m, int n, int splits, bool can_be_wide, bool *wide) {
     const double plain = lx_div((long long)m * n * splits, lx_pairs()), w = lx_div((long long)m * lx_div(n, 2) * splits, lx_pairs()) * LX_WIDE_COST;
