@@ -58,16 +58,17 @@ static int resolve_encode_tiled() {
     return ANE_CUDA_OK;
 }
 
-int make_matrix_map(CUtensorMap *map, ane_dtype dtype, const void *base, size_t rows, size_t cols, size_t ld, int box_rows) {
+int make_matrix_map(CUtensorMap *map, ane_dtype dtype, const void *base, size_t rows, size_t cols, size_t ld, int box_rows, int box_cols) {
     if (int rc = resolve_encode_tiled()) return rc;
-    if (!aligned16(base) || ld % 8 || ld < cols || rows < 1 || cols < 1 || rows > 0xffffffffull || cols > 0xffffffffull || box_rows < 1 || box_rows > 256 || dtype == ANE_F32)
+    if (!aligned16(base) || ld % 8 || ld < cols || rows < 1 || cols < 1 || rows > 0xffffffffull || cols > 0xffffffffull || box_rows < 1 || box_rows > 256 || (box_cols != 64 && box_cols != 32) ||
+        dtype == ANE_F32)
         return fail(ANE_CUDA_ERR_INVALID, "matrix map: unsupported alignment or size (%zu x %zu, ld %zu, box %d)", rows, cols, ld, box_rows);
     const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
     const cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
-    const cuuint32_t box[2] = {64u, (cuuint32_t)box_rows};
+    const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
     const cuuint32_t estr[2] = {1u, 1u};
     const CUresult r = g_encode_tiled(map, dtype == ANE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void *>(base), dims, strides,
-                                      box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                      box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                                       CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return fail(ANE_CUDA_ERR_CUDA, "cuTensorMapEncodeTiled failed with code %d", (int)r);
     return ANE_CUDA_OK;

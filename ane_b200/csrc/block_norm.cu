@@ -23,7 +23,7 @@
 //   forward   115 us   one block of 512 threads per 32 tokens, two blocks per SM       (4.7 TB/s)
 //             138      clusters of eight blocks of 256 threads, 128-byte rows
 //             157      three sweeps through L2
-//   backward  199 us   pipeline over clusters (block_norm_ring.cuh), issue-bound at 15 clusters of eight  (4.0 TB/s)
+//   backward  199 us   pipeline over clusters (block_norm_ring.cuh): 15 clusters of eight, 59 % of their issue slots busy  (4.0 TB/s)
 //             245      one block of 512 threads per 32 tokens; clusters of eight, 128-byte rows: 250
 //             380      two sweeps through L2
 // Rows that break 16-byte alignment (5 x 1000 x 333 in fp16): 24 us over clusters of eight against 125 us in one block per tile.

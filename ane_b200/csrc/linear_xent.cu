@@ -15,9 +15,9 @@
 // dl) at 6.5 TB/s are 1.9 ps, 2 * 1024 operations at 1.5 PFLOP/s are 1.4 ps.
 //
 // Measured, 8192 tokens x 151936 rows x 1024 channels in bf16 (cuBLAS on this GPU: 1650 TFLOP/s in a burst, 1410 under the
-// power cap), one call at a time: stats 1.50 ms (1700 TFLOP/s), dlogits 2.27 (1120; it writes 5 GB of dl), dx 1.9 (1340), d_table
-// 3.0 for two products (1690).  Back to back under the power cap the whole call takes 10.1 ms, 1260 TFLOP/s over the five
-// products that it does and 756 over the three that the result cannot do without.
+// power cap), without overlap of the launches: stats 1.49 ms (1710 TFLOP/s), dlogits 2.15 (1190; it writes 5 GB of dl), dx 1.72
+// (1490), d_table 3.13 for two products (1630).  Back to back under the power cap the whole call takes 9.6 to 10.1 ms, 1290
+// TFLOP/s over the five products that it does and 780 over the three that the result cannot do without.
 //
 // Precision.  16-bit inputs enter the products as they are.  dl is rounded to 16 bits for dx, whose result is rounded to 16
 // bits as well; d_table is an fp32 sum, so dl enters it as two 16-bit numbers, the rounded value and what the rounding left
@@ -56,12 +56,13 @@ constexpr int LX_EPI_WARPS = 8;                          // two for each 32 accu
 constexpr int LX_COLS = LX_BN / 2;                       // columns of an epilogue warp
 constexpr int LX_THREADS = 64 + 32 * LX_EPI_WARPS;       // copy warp, matrix warp, epilogue warps
 constexpr int LX_RING_BOXES = 12;                        // of operands
-constexpr size_t LX_SMEM = (size_t)LX_RING_BOXES * LX_BOX_BYTES + 1024;
+constexpr int LX_STAGING_BYTES = 2 * 32 * 64;            // dlogits: an epilogue warp's 32 rows x 32 columns of both parts
+constexpr size_t lx_smem(int epi) { return (size_t)LX_RING_BOXES * LX_BOX_BYTES + (epi == LX_DLOGITS ? LX_EPI_WARPS * LX_STAGING_BYTES : 0) + 1024; }
 constexpr int LX_STEPS = 32;                             // of 16 along K that stay in an accumulator where an fp32 result is wanted
 constexpr int LX_WAIT_LIMIT = 1 << 20;
 constexpr float LX_HALF_SCALE = 16384.0f;                // of dl where it is held in fp16
 
-struct LxMaps { CUtensorMap a[3], b[3]; };               // one pair per 16-bit product that is summed
+struct LxMaps { CUtensorMap a[3], b[3], hi, lo; };       // one pair per 16-bit product that is summed; dlogits: where dl goes
 struct LxArgs {
     int segments;              // pairs in use
     int kblocks;               // K blocks of one pair
@@ -77,7 +78,7 @@ struct LxArgs {
     float2 *part; int tile0;   // stats: [half vocabulary tile][ldt], this piece's first
     float *hit;                // stats: the target's logit per token
     const float *lse2;         // dlogits: lse * log2(e)
-    void *hi, *lo; size_t ldl; // dlogits: [token][ldl]; lo null: the low parts are not wanted
+    int two_parts;             // dlogits: the low parts of dl are wanted
     float dscale;
     // dx: [split][column][ldt] sums; d_table: [column][D]
     float *out; size_t ldt; int first;
@@ -178,10 +179,13 @@ template <bool HALF> __device__ __forceinline__ void lx_split2(float a, float b,
         lo = *reinterpret_cast<const uint32_t *>(&l);
     }
 }
-// 32 bytes at once: every sector of a row is written whole, although neighbouring lanes hold different rows.
-__device__ __forceinline__ void lx_store32(void *p, const uint32_t (&w)[8]) {
-    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
-                 ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
+__device__ __forceinline__ void lx_store_shared(uint32_t at, const uint32_t (&w)[4]) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+}
+// A box out of shared memory; columns and rows outside the matrix are left out.
+__device__ __forceinline__ void lx_store_box(const CUtensorMap *map, uint32_t src, int x, int y) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];"
+                 ::"l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(src) : "memory");
 }
 
 // The K blocks of one tile: the tile's share [k0, k1), in parts of `span`; within a part every operand pair in turn.
@@ -443,28 +447,41 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LX_THREADS, 1) lx_ge
                     const float shift = log2f(a.dscale) - lse2;          // a power of two: exp2 brings it in
                     const bool mine = __any_sync(0xffffffffu, tgt >= 0 && tgt < LX_COLS);
                     const int row0 = mt * LX_BM + rank * LX_CTA_M + quad * 32;
-                    const size_t at = (size_t)m * a.ldl + n0;
-                    // 16 columns at a time straight to memory, whole sectors of 32 bytes per lane.  Rows could be written together by
-                    // way of shared memory, but its bandwidth belongs to the operands (112 of 128 bytes per clock).
+                    const uint32_t stage = base + STAGES * STAGE_BYTES + (warp - 2) * LX_STAGING_BYTES;
+                    // 32 columns at a time through this warp's shared memory to the copy engine: 64-byte rows, swizzled as it
+                    // expects them.  Straight to memory a lane writes its own row, 32 lines per instruction: this product took
+                    // 22.2 us instead of 20.0 for one sequence over 9200 rows, 2.22 ms instead of 2.15 for 8192 tokens over
+                    // 151936 (the whole call there: the same within its spread, the power cap sets it).
 #pragma unroll
-                    for (int c = 0; c < LX_COLS; c += 16) {
+                    for (int c = 0; c < LX_COLS; c += 32) {
                         if (c >= cols || row0 >= a.m) break;
-                        uint32_t hi[8], lo[8];
-                        float e[16];
+                        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");     // the staging is free again
+                        __syncwarp();
 #pragma unroll
-                        for (int j = 0; j < 16; j++) e[j] = lx_exp2(fmaf(v[c + j], k2, shift));
-                        if (mine) {
+                        for (int q = 0; q < 4; q++) {
+                            uint32_t hi[4], lo[4];
+                            float e[8];
 #pragma unroll
-                            for (int j = 0; j < 16; j++) e[j] = tgt == c + j ? e[j] - a.dscale : e[j];
+                            for (int j = 0; j < 8; j++) e[j] = lx_exp2(fmaf(v[c + q * 8 + j], k2, shift));
+                            if (mine) {
+#pragma unroll
+                                for (int j = 0; j < 8; j++) e[j] = tgt == c + q * 8 + j ? e[j] - a.dscale : e[j];
+                            }
+#pragma unroll
+                            for (int j = 0; j < 4; j++) {
+                                lx_split2<HALF>(e[2 * j], e[2 * j + 1], hi[j], lo[j]);
+                                if (id < 0) hi[j] = lo[j] = 0;           // a masked token: zeros, whatever its logits are
+                            }
+                            const uint32_t at = stage + lane * 64 + ((q ^ ((lane >> 1) & 3)) << 4);
+                            lx_store_shared(at, hi);
+                            lx_store_shared(at + LX_STAGING_BYTES / 2, lo);
                         }
-#pragma unroll
-                        for (int j = 0; j < 8; j++) {
-                            lx_split2<HALF>(e[2 * j], e[2 * j + 1], hi[j], lo[j]);
-                            if (id < 0) hi[j] = lo[j] = 0;               // a masked token: zeros, whatever its logits are
-                        }
-                        if (live) {
-                            lx_store32(static_cast<uint16_t *>(a.hi) + at + c, hi);
-                            if (a.lo) lx_store32(static_cast<uint16_t *>(a.lo) + at + c, lo);
+                        fence_proxy_async();
+                        __syncwarp();
+                        if (lane == 0) {
+                            lx_store_box(&maps.hi, stage, n0 + c, row0);
+                            if (a.two_parts) lx_store_box(&maps.lo, stage + LX_STAGING_BYTES / 2, n0 + c, row0);
+                            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
                         }
                     }
                 } else if (live) {
@@ -483,6 +500,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LX_THREADS, 1) lx_ge
             }
         }
     }
+    if (EPI == LX_DLOGITS && warp >= 2 && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     __syncwarp();
     lx_fence_before();
     __syncthreads();
@@ -896,12 +914,12 @@ static inline void lx_call(void (*kernel)(KArgs...), dim3 grid, dim3 block, size
 template <int EPI, int MODE, bool HALF> static int lx_start_kernel(cudaStream_t st, const LxMaps &maps, const LxArgs &a) {
     static bool ready = false;
     if (!ready) {
-        ANE_CUDA_TRY(cudaFuncSetAttribute(lx_gemm_kernel<EPI, MODE, HALF>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)LX_SMEM));
+        ANE_CUDA_TRY(cudaFuncSetAttribute(lx_gemm_kernel<EPI, MODE, HALF>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)lx_smem(EPI)));
         ready = true;
     }
     const long long tiles = (long long)a.m_tiles * a.n_tiles * a.splits;
     const int pairs = tiles < lx_pairs() ? (int)tiles : lx_pairs();
-    lx_call(lx_gemm_kernel<EPI, MODE, HALF>, dim3(2 * pairs), dim3(LX_THREADS), LX_SMEM, st, maps, a);
+    lx_call(lx_gemm_kernel<EPI, MODE, HALF>, dim3(2 * pairs), dim3(LX_THREADS), lx_smem(EPI), st, maps, a);
     ANE_LAUNCH_OK(1);
     return ANE_CUDA_OK;
 }
@@ -1158,7 +1176,9 @@ template <typename T, typename H> static int lx_run(const LxCall &c) {
             if (int rc = table_rows(v0, nv)) return rc;
             if (int rc = maps_for(m, segs, xh, xl, rows_hi, rows_lo, n_tok, D, ldd, LX_CTA_M, nv, D, ld, LX_BN / 2)) return rc;
             a.n_tiles = lx_div(nv, LX_BN); a.n = nv; a.v0 = v0;
-            a.hi = lh; a.lo = ll; a.ldl = ldl;
+            if (int rc = make_matrix_map(&m.hi, part, lh, n_tok, nv, ldl, 32, 32)) return rc;
+            if (need_lo) if (int rc = make_matrix_map(&m.lo, part, ll, n_tok, nv, ldl, 32, 32)) return rc;
+            a.two_parts = need_lo;
             if (int rc = lx_launch<LX_DLOGITS>(c.st, m, a)) return rc;
             if (c.dx) {
                 LxArgs g = a;

@@ -22,8 +22,9 @@ int make_bcs_tensor_map(CUtensorMap *map, ane_dtype dtype, const void *base, int
                         int l2_promotion_bytes = 128);
 
 // Row-major matrix of 16-bit elements (bf16 or fp16), rows x cols with `ld` elements between rows, seen as a 2-D map with
-// 128-byte swizzled boxes of 64 columns x box_rows rows.  Rows and columns outside the matrix read as zeros.
-int make_matrix_map(CUtensorMap *map, ane_dtype dtype, const void *base, size_t rows, size_t cols, size_t ld, int box_rows);
+// swizzled boxes of box_cols (64: 128-byte rows, 32: 64-byte rows) columns x box_rows rows.  Rows and columns outside the
+// matrix read as zeros and are not written.
+int make_matrix_map(CUtensorMap *map, ane_dtype dtype, const void *base, size_t rows, size_t cols, size_t ld, int box_rows, int box_cols = 64);
 
 #ifdef __CUDACC__
 // ------------------------------------------------------------------ device primitives
