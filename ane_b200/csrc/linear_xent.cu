@@ -985,7 +985,7 @@ static LxPlan lx_plan(int T_all, int D, int V, int segs, bool dx, bool d_table, 
     if (most > vt) most = vt;
     double best = 1e300;
     p.piece_tiles = 1; p.splits = 1;
-    for (int n = (int)most; n >= 1 && n >= (int)most / 4; n--) {
+    for (int n = (int)most; n >= 1 && n >= (int)most / 4; n -= 1 + (int)most / 1024) {
         const int pieces = lx_div(vt, n);
         int splits = 1;
         if (dx) {
@@ -1232,7 +1232,8 @@ int ane_cuda_linear_cross_entropy_dev(void *stream, ane_dtype dtype, ane_idtype 
     ANE_REQUIRE(dtype_ok(dtype), "%s: bad dtype %d", __func__, (int)dtype);
     ANE_REQUIRE(idtype == ANE_ID_U16 || idtype == ANE_ID_I32, "%s: bad id type", __func__);
     ANE_REQUIRE(B >= 1 && D >= 1 && V >= 1 && S >= 1, "%s: bad shape B=%d D=%d V=%d S=%d", __func__, B, D, V, S);
-    ANE_REQUIRE((long long)B * S < 0x7fffff00LL && V < 0x7fffff00 && D <= 65536, "%s: too many tokens, or D above 65536", __func__);
+    // up to 2^30, the sum of an index and a step over tokens or rows fits an int
+    ANE_REQUIRE((long long)B * S <= 1 << 30 && V <= 1 << 30 && D <= 65536, "%s: more than 2^30 tokens or rows, or D above 65536", __func__);
     ANE_REQUIRE(!dx || dx != x, "%s: dx may not be x", __func__);
     const size_t e = dtype_size(dtype), xb = (size_t)B * D * S * e;
     ANE_CHECK_EXTENT(loss_seq, (size_t)B * 4); ANE_CHECK_EXTENT(loss_tok, (size_t)B * S * 4); ANE_CHECK_EXTENT(dx, xb); ANE_CHECK_EXTENT(x, xb);

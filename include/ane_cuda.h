@@ -328,9 +328,11 @@ int ane_cuda_cross_entropy_dev(void *stream, ane_idtype idtype, int B, int V, in
  * d_table only the losses are computed.  A target outside [0, V) marks a token without a target (padding): no loss, a zero
  * column in dx, nothing added to d_table, whatever its x holds -- unlike ane_cuda_cross_entropy_dev, which keeps the
  * reference's plain-softmax gradient there.  Ids >= V are counted in the status words, negative ones are not.  The products
- * run on the tensor cores with fp32 sums; fp32 inputs enter as two bf16 parts each, dl as two 16-bit parts in d_table and as
- * one in a 16-bit dx.  Bit-stable from call to call.  Scratch: up to about 1 GiB of the library's range, however large the
- * vocabulary. */
+ * run on the tensor cores with fp32 sums; fp32 inputs enter as two fp16 parts each (scaled by a power of two), dl as two
+ * 16-bit parts in d_table and as one in a 16-bit dx.  One token, or up to four in fp32, go without the tensor cores.
+ * Bit-stable from call to call.  B*S and V up to 2^30, D up to 65536.  Scratch of the library's range: up to 768 MiB for dl
+ * and 256 MiB for a table that has to be packed (fp32, or rows that break 16-byte alignment), and with N = min(B*S, 8192)
+ * about N*V/16 bytes for the statistics and 8*N*D for x and dx -- 1 GiB in all for V = 151936, D = 1024. */
 int ane_cuda_linear_cross_entropy_dev(void *stream, ane_dtype dtype, ane_idtype idtype, int B, int D, int V, int S,
                                       float *loss_seq, float *loss_tok, void *dx, float *d_table, const void *x,
                                       const void *table, const void *targets, float grad_scale);

@@ -3,8 +3,8 @@ differences and the operator over given logits.
 
 Tolerances, as the 2-norm of the difference over that of the result, and as the largest difference over the largest value.
 A logit is an fp32 sum of D products: its error is below about sqrt(D) * 2^-24 of the norm of its terms, 2e-6 for D = 1000;
-fp32 inputs enter as two bf16 parts, which drops low * low (2^-18 of a term at most) and rounds the low part (2^-18): 2^-17 =
-7.6e-6 of a term, random in sign, so of the norm of the terms.  Logits here are of order 1 (up to 6 where scaled up), so
+fp32 inputs enter as two 16-bit parts, which drops low * low and rounds the low part: 2^-17 = 7.6e-6 of a term at most (bf16
+parts; fp16 ones, scaled, 2^-21), random in sign, so of the norm of the terms.  Logits here are of order 1 (up to 6 where scaled up), so
 probabilities carry a relative error of at most about 1e-5, and the loss, a mean of numbers of order log V, less.
   loss                1e-5
   d_table, fp32       dl in two parts leaves 2^-16 of it (bf16) in the worst case, half a step of the second rounding of
@@ -283,7 +283,7 @@ def test_refusals(ops):
         return L.ane_cuda_linear_cross_entropy_dev(None, dt, idt, B, D, V, S, loss_p, None, dx, None, xp, E.data_ptr(), t.data_ptr(), 1.0)
     assert call() == lib.OK
     for bad in (dict(dt=3), dict(idt=2), dict(B=0), dict(D=0), dict(V=0), dict(S=0), dict(loss_p=None), dict(xp=None), dict(dx=x.data_ptr()), dict(D=70000),
-                dict(B=1 << 20, S=1 << 20)):
+                dict(B=1 << 20, S=1 << 20), dict(B=(1 << 30) + 1, S=1), dict(V=(1 << 30) + 1), dict(V=(1 << 31) - 257)):
         assert call(**bad) == lib.ERR_INVALID, bad
     lib.set_tuning("check_extents", 1)
     try:
