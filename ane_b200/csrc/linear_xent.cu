@@ -684,17 +684,19 @@ __global__ void __launch_bounds__(1024) lx_join_kernel(float *__restrict__ lse2,
     loss_tok[token] = loss;
 }
 
-// dx[b][d][s] = alpha * sum over the shares of K, in order.
+// dx[b][d][s] = alpha * sum over the shares of K, in order.  A token without a target has zeros, whatever the table holds.
 template <typename T>
-__global__ void __launch_bounds__(256) lx_finish_dx_kernel(T *__restrict__ dx, const float *__restrict__ sums, int splits, int t0, int tokens, int D, int S, size_t ldt, float alpha) {
+__global__ void __launch_bounds__(256) lx_finish_dx_kernel(T *__restrict__ dx, const float *__restrict__ sums, const void *__restrict__ targets, int id_u16, int V, int splits,
+                                                           int t0, int tokens, int D, int S, size_t ldt, float alpha) {
     dep_sync();
     const int t = blockIdx.x * 256 + threadIdx.x;
     if (t >= tokens) return;
+    const bool live = lx_target(targets, id_u16, V, t0 + t) >= 0;
     const int b = (t0 + t) / S, s = (t0 + t) % S;
     for (int d = blockIdx.y; d < D; d += gridDim.y) {
         float v = 0.0f;
         for (int k = 0; k < splits; k++) v += sums[((size_t)k * D + d) * ldt + t];
-        dx[((size_t)b * D + d) * S + s] = Elt<T>::from_f(v * alpha);
+        dx[((size_t)b * D + d) * S + s] = Elt<T>::from_f(live ? v * alpha : 0.0f);
     }
 }
 
@@ -860,7 +862,8 @@ __global__ void __launch_bounds__(256) lf_grads_kernel(float *__restrict__ dx_pa
 
 // dx[b][d][s] = alpha * sum over the chunks, in order: eight slices of them per column.
 template <typename T>
-__global__ void __launch_bounds__(256) lf_finish_dx_kernel(T *__restrict__ dx, const float *__restrict__ part, int chunks, int tokens, int D, int S, float alpha) {
+__global__ void __launch_bounds__(256) lf_finish_dx_kernel(T *__restrict__ dx, const float *__restrict__ part, const void *__restrict__ targets, int id_u16, int V, int chunks,
+                                                           int tokens, int D, int S, float alpha) {
     __shared__ float sh[8][33];
     dep_sync();
     const int cl = threadIdx.x & 31, sl = threadIdx.x >> 5, d = blockIdx.x * 32 + cl, t = blockIdx.y;
@@ -874,7 +877,7 @@ __global__ void __launch_bounds__(256) lf_finish_dx_kernel(T *__restrict__ dx, c
     a = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; i++) a += sh[i][cl];
-    dx[((size_t)(t / S) * D + d) * S + t % S] = Elt<T>::from_f(a * alpha);
+    dx[((size_t)(t / S) * D + d) * S + t % S] = Elt<T>::from_f(lx_target(targets, id_u16, V, t) >= 0 ? a * alpha : 0.0f);
 }
 
 // loss_seq[b] = (sum_t loss_tok[b][t]) / S, fixed summation tree.
@@ -1039,7 +1042,7 @@ template <typename T, int VEC, int TOK> static int lf_run(const LxCall &c) {
         ANE_LAUNCH_OK(1);
     }
     if (c.dx) {
-        lx_call(lf_finish_dx_kernel<T>, dim3(lx_div(D, 32), TOK), dim3(256), 0, c.st, static_cast<T *>(c.dx), dxs, chunks, TOK, D, c.S, alpha);
+        lx_call(lf_finish_dx_kernel<T>, dim3(lx_div(D, 32), TOK), dim3(256), 0, c.st, static_cast<T *>(c.dx), dxs, c.targets, c.id_u16, V, chunks, TOK, D, c.S, alpha);
         ANE_LAUNCH_OK(1);
     }
     lx_call(lx_loss_kernel, dim3(c.B), dim3(256), 0, c.st, c.loss_seq, loss_tok, c.S);
@@ -1210,7 +1213,7 @@ template <typename T, typename H> static int lx_run(const LxCall &c) {
         }
         if (c.dx) {
             const int by = D < 1024 ? D : 1024;
-            lx_call(lx_finish_dx_kernel<T>, dim3(lx_div(n_tok, 256), by), dim3(256), 0, c.st, static_cast<T *>(c.dx), dxs, splits, t0, n_tok, D, c.S, ldt, alpha);
+            lx_call(lx_finish_dx_kernel<T>, dim3(lx_div(n_tok, 256), by), dim3(256), 0, c.st, static_cast<T *>(c.dx), dxs, c.targets, c.id_u16, V, splits, t0, n_tok, D, c.S, ldt, alpha);
             ANE_LAUNCH_OK(1);
         }
     }

@@ -207,6 +207,19 @@ def test_masked_tokens_hide_what_they_hold(ops, dt):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(1, 40, 300, 1), (1, 40, 300, 3), (2, 40, 300, 50)])
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+def test_a_table_that_is_not_finite_leaves_masked_tokens_alone(ops, dt, shape):
+    x, E, t = inputs(*shape, DT[dt], 9, masked=0.0)
+    E[7, 3], E[90, 20] = float("inf"), float("nan")
+    t[0, 0] = -1
+    tok = torch.ones(t.shape, device="cuda")
+    _, dx = ops.linear_cross_entropy(x, E, t, loss_tok=tok)
+    assert float(tok[0, 0]) == 0 and not dx[0, :, 0].float().any()
+    lib.poll_status()
+
+
+@pytest.mark.gpu
 def test_a_token_that_is_not_finite_shows_and_is_counted(ops):
     x, E, t = inputs(1, 64, 700, 200, torch.bfloat16, seed=4, masked=0.0)
     x[0, 5, 9] = float("nan")
