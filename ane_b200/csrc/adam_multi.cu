@@ -321,7 +321,8 @@ int ane_cuda_adam_multi_dev(void *stream, ane_adam_state state, ane_dtype g_dtyp
     ANE_REQUIRE(flags == ANE_ADAM_STORIES || flags == ANE_ADAM_DYNAMIC, "%s: bad flags %u", __func__, flags);
     const bool q8 = state == ANE_ADAM_STATE_Q8;
     std::vector<AmItem> list;
-    std::vector<std::pair<uintptr_t, uintptr_t>> written;
+    struct Range { uintptr_t from, to; bool written; };
+    std::vector<Range> ranges;
     list.reserve((size_t)count);
     for (int k = 0; k < count; k++) {
         const ane_adam_item &a = items[k];
@@ -338,8 +339,9 @@ int ane_cuda_adam_multi_dev(void *stream, ane_adam_state state, ane_dtype g_dtyp
             ANE_CHECK_EXTENT(a.w, a.n * 4); ANE_CHECK_EXTENT(a.g, a.n * dtype_size(g_dtype));
             ANE_CHECK_EXTENT(a.m, sb); ANE_CHECK_EXTENT(a.v, sb); ANE_CHECK_EXTENT(a.copy, a.n * 2);
             if (q8) { ANE_CHECK_EXTENT(a.m_scale, cb); ANE_CHECK_EXTENT(a.v_scale, cb); }
-            auto range = [&](const void *p, size_t bytes) { if (p) written.emplace_back((uintptr_t)p, (uintptr_t)p + bytes); };
+            auto range = [&](const void *p, size_t bytes, bool written = true) { if (p) ranges.push_back({(uintptr_t)p, (uintptr_t)p + bytes, written}); };
             range(a.w, a.n * 4); range(a.m, sb); range(a.v, sb); range(a.copy, a.n * 2);
+            range(a.g, a.n * dtype_size(g_dtype), false);
             if (q8) { range(a.m_scale, cb); range(a.v_scale, cb); }
         }
         AmItem d = {};
@@ -349,10 +351,13 @@ int ane_cuda_adam_multi_dev(void *stream, ane_adam_state state, ane_dtype g_dtyp
         d.vec = aligned16(a.w) && aligned16(a.g) && aligned_to(a.m, sa) && aligned_to(a.v, sa) && aligned16(a.copy);
         list.push_back(d);
     }
-    if (!written.empty()) {       // debug mode: two tensors that share memory would race
-        std::sort(written.begin(), written.end());
-        for (size_t k = 1; k < written.size(); k++)
-            ANE_REQUIRE(written[k].first >= written[k - 1].second, "%s: two ranges that the step writes overlap", __func__);
+    // debug mode: a tensor that shares memory with one that the step writes would race; gradients may share with each other
+    std::sort(ranges.begin(), ranges.end(), [](const Range &a, const Range &b) { return a.from < b.from; });
+    uintptr_t written_to = 0, any_to = 0;
+    for (const Range &r : ranges) {
+        ANE_REQUIRE(r.from >= (r.written ? any_to : written_to), "%s: two tensors overlap and the step writes one of them", __func__);
+        any_to = std::max(any_to, r.to);
+        if (r.written) written_to = std::max(written_to, r.to);
     }
     if (list.empty()) return ANE_CUDA_OK;
     AmScalars s = {};

@@ -310,7 +310,7 @@ class AdamTensors:
         self.tensors = (list(w), list(g), list(m), list(v), m_scale and list(m_scale), v_scale and list(v_scale), copy and list(copy))
         self.items = (_l.AdamItem * count)()
         self.count, self.wd = count, wd
-        written, rows = [], []
+        ranges, rows = [], []
         for k in range(count):
             n, shape = w[k].numel(), w[k].shape
             blocks = (-(-n // ADAM_BLOCK),)
@@ -320,14 +320,17 @@ class AdamTensors:
                     _like(f"{names[i]}[{k}]", ts[k], want, kinds[i])
             rows.append((n, [None if ts is None else ts[k] for ts in self.tensors]))
             if n:
-                for i in (0, 2, 3, 4, 5, 6):
-                    t = rows[-1][1][i]
+                for i, t in enumerate(rows[-1][1]):
                     if t is not None:
                         at = t.data_ptr()
-                        written.append((at, at + t.numel() * t.element_size()))
-        written.sort()
-        if any(b[0] < a[1] for a, b in zip(written, written[1:])):
-            raise ValueError("two tensors that the step writes share memory")
+                        ranges.append((at, at + t.numel() * t.element_size(), i != 1))
+        ranges.sort()
+        written_to = any_to = 0
+        for at, end, written in ranges:
+            if at < (any_to if written else written_to):     # gradients may share memory with each other
+                raise ValueError("two tensors share memory and the step writes one of them")
+            any_to = max(any_to, end)
+            written_to = max(written_to, end) if written else written_to
         for k, (n, ts) in enumerate(rows):
             item = self.items[k]
             item.n, item.wd = n, wd[k]

@@ -119,6 +119,17 @@ def test_refusals_without_a_gpu():
         dev_ops.adam_state_unpack(torch.zeros(257, dtype=torch.uint8), torch.zeros(1), out=torch.zeros(257))
 
 
+def test_a_gradient_in_memory_that_the_step_writes_is_refused():
+    w, m, v = torch.zeros(1, 8).unbind(0), [torch.zeros(8)], [torch.zeros(8)]
+    for g in (w, m, [torch.empty(0).set_(v[0].untyped_storage(), 4, (4,))]):
+        a = 4 if g[0].numel() == 4 else 8
+        with pytest.raises(ValueError, match="share memory"):
+            dev_ops.AdamTensors([t[:a] for t in w], list(g), [t[:a] for t in m], [t[-a:] for t in v])
+    g = torch.zeros(8)                    # two weights with one gradient: only read, and so refused for being on the CPU alone
+    with pytest.raises(ValueError, match="current CUDA device"):
+        dev_ops.AdamTensors([torch.zeros(8), torch.zeros(8)], [g, g], *[[torch.zeros(8), torch.zeros(8)] for _ in range(2)])
+
+
 def test_the_library_refuses_before_init():
     if torch.cuda.is_available():
         return
@@ -317,6 +328,10 @@ def test_refusals(ops):
     try:
         item[0].w = t[2].data_ptr()                        # the same memory as m
         assert call() == lib.ERR_INVALID
+        item[0].w, item[0].g = t[0].data_ptr(), t[3].data_ptr()        # the gradient in the memory of v
+        assert call() == lib.ERR_INVALID
+        item[0].g = t[1].data_ptr()
+        assert call() == lib.OK
     finally:
         lib.clear_tuning("check_extents")
     assert L.ane_cuda_adam_state_unpack_dev(None, 8, None, None, None, 0) == lib.ERR_INVALID
