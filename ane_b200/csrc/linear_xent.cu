@@ -29,7 +29,8 @@
 //
 // The accumulators of the tensor cores cut off what does not fit instead of rounding: every step of 16 along K takes half a
 // unit of the last place from the sum on average, 3e-8 of it (measured: 1.2e-5 after 345 steps).  So fp32 results leave the
-// accumulator after 32 steps and are added up in registers with rounding.
+// accumulator after 32 steps and are added up in registers with rounding; the logits of fp32 inputs after 72 (leaving more often
+// lets the matrix thread run less far ahead of the epilogue: dlogits 125 us against 108 for 4096 tokens over 9200 rows).
 //
 // A token without a target (id outside [0, V)) has zeros in place of its x, so that nothing it holds -- infinities and NaN
 // included -- reaches d_table.
@@ -47,13 +48,15 @@ enum LxEpilogue { LX_STATS, LX_DLOGITS, LX_DX, LX_DTABLE };
 //   LX_PLAIN   A, B           one accumulator (the other one belongs to the next tile)
 //   LX_WIDE    A, B, B'       B' = the next 256 rows of the output's columns: both accumulators make one 256 x 512 tile
 //   LX_TWO     A, B, B'       B' = the low part of B: both products into one accumulator
-enum LxMode { LX_PLAIN, LX_WIDE, LX_TWO };
+//   LX_SPLIT   A, B, B', A'   fp32 inputs, A' and B' the low parts: A' B, A B' and A B into one accumulator
+//   LX_NARROW  the same with tiles of 256 x 128
+enum LxMode { LX_PLAIN, LX_WIDE, LX_TWO, LX_SPLIT, LX_NARROW };
 
 constexpr int LX_CTA_M = 128;                            // rows of the tile in each block of a pair
 constexpr int LX_BM = 2 * LX_CTA_M, LX_BN = 256, LX_BK = 64;      // one accumulator: M x N outputs of a pair; K elements per stage
 constexpr int LX_BOX_BYTES = LX_CTA_M * LX_BK * 2;                // a block's 128 rows of one operand
 constexpr int LX_EPI_WARPS = 8;                          // two for each 32 accumulator lanes, half of the columns each
-constexpr int LX_COLS = LX_BN / 2;                       // columns of an epilogue warp
+constexpr int lx_acc_n(int mode) { return mode == LX_NARROW ? LX_BN / 2 : LX_BN; }
 constexpr int LX_THREADS = 64 + 32 * LX_EPI_WARPS;       // copy warp, matrix warp, epilogue warps
 constexpr int LX_RING_BOXES = 12;                        // of operands
 constexpr int LX_STAGING_BYTES = 2 * 32 * 64;            // dlogits: an epilogue warp's 32 rows x 32 columns of both parts
@@ -62,10 +65,9 @@ constexpr int LX_STEPS = 32;                             // of 16 along K that s
 constexpr int LX_WAIT_LIMIT = 1 << 20;
 constexpr float LX_HALF_SCALE = 16384.0f;                // of dl where it is held in fp16
 
-struct LxMaps { CUtensorMap a[3], b[3], hi, lo; };       // one pair per 16-bit product that is summed; dlogits: where dl goes
+struct LxMaps { CUtensorMap a[2], b[2], hi, lo; };       // operands and their low parts; dlogits: where dl goes
 struct LxArgs {
-    int segments;              // pairs in use
-    int kblocks;               // K blocks of one pair
+    int kblocks;
     int splits;                // shares of the K blocks, each with its own sums (dx only)
     int span;                  // K blocks that one accumulator sums before its values move to registers
     int m_tiles, n_tiles;
@@ -188,26 +190,20 @@ __device__ __forceinline__ void lx_store_box(const CUtensorMap *map, uint32_t sr
                  ::"l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(src) : "memory");
 }
 
-// The K blocks of one tile: the tile's share [k0, k1), in parts of `span`; within a part every operand pair in turn.
+// The K blocks of one tile: the tile's share [k0, k1), in parts of `span`.
 struct LxRange {
-    int k0, k1, span, segments, part, seg, k;
+    int k0, k1, span, part, k;
     __device__ __forceinline__ LxRange(const LxArgs &a, int tile) {
         const int ks = tile / (a.m_tiles * a.n_tiles);
         k0 = (int)((long long)a.kblocks * ks / a.splits);
         k1 = (int)((long long)a.kblocks * (ks + 1) / a.splits);
-        span = a.span; segments = a.segments;
+        span = a.span;
         part = k = k0;
-        seg = 0;
     }
-    __device__ __forceinline__ bool done() const { return part >= k1; }
-    __device__ __forceinline__ bool first() const { return seg == 0 && k == part; }      // at the beginning of a part (or past the last)
+    __device__ __forceinline__ bool done() const { return k >= k1; }
+    __device__ __forceinline__ bool first() const { return k == part || k >= k1; }       // at the beginning of a part (or past the last)
     __device__ __forceinline__ void next() {
-        k++;
-        if (k < k1 && k < part + span) return;
-        if (++seg < segments) { k = part; return; }
-        seg = 0;
-        part += span;
-        k = part;
+        if (++k == part + span) part = k;
     }
 };
 
@@ -218,14 +214,20 @@ struct LxRange {
 // matrix instructions; eight warps take the accumulators over.
 //
 // A 256 x 256 tile wants 64 bytes per SM and clock from L2 and 256 x 512 wants 48, so the large products bring two boxes of B for
-// each box of A (LX_WIDE, LX_TWO): d_table went from 1137 to 1414 TFLOP/s with it.  The second half of the distance was the
+// each box of A (LX_WIDE, LX_TWO): d_table went from 1137 to 1414 TFLOP/s with it.  fp32 inputs need 43 with all four parts in one
+// stage for their three products; a pass for each product took 708 us instead of 629 for the losses of 4096 tokens over 32000
+// rows, 2440 instead of 2240 with gradients.  The second half of the distance was the
 // matrix thread itself: with descriptors computed in vector registers a K block took 1450 clocks instead of the 1024 of its
 // instructions (stats 1350 -> 1590 TFLOP/s with uniform registers).
 template <int EPI, int MODE, bool HALF>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LX_THREADS, 1) lx_gemm_kernel(const __grid_constant__ LxMaps maps, const __grid_constant__ LxArgs a) {
     constexpr bool A_MN = EPI == LX_DTABLE, B_MN = EPI == LX_DX || EPI == LX_DTABLE;
-    constexpr int BOXES = MODE == LX_PLAIN ? 2 : 3, STAGES = LX_RING_BOXES / BOXES, STAGE_BYTES = BOXES * LX_BOX_BYTES;
-    constexpr int ACCS = MODE == LX_WIDE ? 2 : 1, TILE_N = ACCS * LX_BN;
+    constexpr bool SPLIT = MODE == LX_SPLIT || MODE == LX_NARROW, LOW_B = MODE == LX_TWO || SPLIT, SUMS = SPLIT || EPI == LX_DX || EPI == LX_DTABLE;
+    constexpr int ACC_N = lx_acc_n(MODE), COLS = ACC_N / 2;      // columns of an accumulator, of an epilogue warp
+    constexpr int ACCS = MODE == LX_WIDE ? 2 : 1, TILE_N = ACCS * ACC_N;
+    // a stage: A, one or two boxes of B, A'
+    constexpr int B_BYTES = COLS * LX_BK * 2, B_BOXES = MODE == LX_PLAIN ? 1 : 2, LOW_A = LX_BOX_BYTES + B_BOXES * B_BYTES;
+    constexpr int STAGE_BYTES = LOW_A + (SPLIT ? LX_BOX_BYTES : 0), STAGES = LX_RING_BOXES * LX_BOX_BYTES / STAGE_BYTES;
     extern __shared__ uint8_t raw[];
     const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;       // the same offset in both blocks
     // full and acc_empty are used in the first block only; the others are each block's own
@@ -264,27 +266,31 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LX_THREADS, 1) lx_ge
         bool ok = true;
         for (int tile = pair; tile < tiles && ok; tile += pairs) {
             const int mt = tile % a.m_tiles, nt = tile / a.m_tiles % a.n_tiles;
-            const int am = mt * LX_BM + rank * LX_CTA_M, bn = nt * TILE_N + rank * (LX_BN / 2);
+            const int am = mt * LX_BM + rank * LX_CTA_M, bn = nt * TILE_N + rank * COLS;
             for (LxRange r(a, tile); !r.done(); r.next()) {
                 if (!(ok = __all_sync(0xffffffffu, lx_wait(&empty[st], phase, abort)))) break;
                 if (lx_elect()) {
                     const int k = r.k * LX_BK;
                     const uint32_t sa = base + st * STAGE_BYTES, bar = lx_in_leader(&full[st]);
                     if (rank == 0) mbar_arrive_expect_tx(&full[st], 2 * STAGE_BYTES);
-                    if constexpr (A_MN) {
 #pragma unroll
-                        for (int i = 0; i < LX_CTA_M / 64; i++) lx_load_box(sa + i * 8192, &maps.a[r.seg], am + i * 64, k, bar);
-                    } else {
-                        lx_load_box(sa, &maps.a[r.seg], k, am, bar);
+                    for (int h = 0; h < (SPLIT ? 2 : 1); h++) {
+                        const uint32_t at = sa + h * LOW_A;
+                        if constexpr (A_MN) {
+#pragma unroll
+                            for (int i = 0; i < LX_CTA_M / 64; i++) lx_load_box(at + i * 8192, &maps.a[h], am + i * 64, k, bar);
+                        } else {
+                            lx_load_box(at, &maps.a[h], k, am, bar);
+                        }
                     }
 #pragma unroll
-                    for (int h = 0; h < BOXES - 1; h++) {
-                        const CUtensorMap *map = &maps.b[MODE == LX_TWO ? h : r.seg];
-                        const uint32_t sb = sa + (1 + h) * LX_BOX_BYTES;
-                        const int n = bn + (MODE == LX_WIDE ? h * LX_BN : 0);
+                    for (int h = 0; h < B_BOXES; h++) {
+                        const CUtensorMap *map = &maps.b[LOW_B ? h : 0];
+                        const uint32_t sb = sa + LX_BOX_BYTES + h * B_BYTES;
+                        const int n = bn + (MODE == LX_WIDE ? h * ACC_N : 0);
                         if constexpr (B_MN) {
 #pragma unroll
-                            for (int i = 0; i < LX_BN / 128; i++) lx_load_box(sb + i * 8192, map, n + i * 64, k, bar);
+                            for (int i = 0; i < COLS / 64; i++) lx_load_box(sb + i * 8192, map, n + i * 64, k, bar);
                         } else {
                             lx_load_box(sb, map, k, n, bar);
                         }
@@ -300,9 +306,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LX_THREADS, 1) lx_ge
             uint32_t st = 0, phase = 0, turn = 0;
             bool ok = true;
             const uint64_t da = lx_desc(base, A_MN ? 8192 : 16), db = lx_desc(base, B_MN ? 8192 : 16);
-            // a stage's product with its box `box` of B into accumulator `acc`
-            auto product = [&](uint32_t stage, int box, uint32_t acc, bool more) {
-                const uint64_t sa = da + stage * (STAGE_BYTES >> 4), sb = db + (stage * (STAGE_BYTES >> 4) + box * (LX_BOX_BYTES >> 4));
+            // the product of a stage's A (or A') and box `box` of B into accumulator `acc`
+            auto product = [&](uint32_t stage, bool low_a, int box, uint32_t acc, bool more) {
+                const uint64_t sa = da + (stage * (STAGE_BYTES >> 4) + (low_a ? LOW_A >> 4 : 0)), sb = db + (stage * (STAGE_BYTES >> 4) + ((LX_BOX_BYTES + box * B_BYTES) >> 4));
 #pragma unroll
                 for (int i = 0; i < LX_BK / 16; i++) lx_mma(tmem + acc * LX_BN, sa + i * (A_MN ? 128 : 2), sb + i * (B_MN ? 128 : 2), a.idesc, i > 0 || more);
             };
@@ -324,7 +330,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LX_THREADS, 1) lx_ge
                         uint32_t s = st, ph = phase;
                         for (int j = 0; j < group; j++) {
                             if (!wait(&full[s], ph)) break;
-                            if (lx_elect()) product(s, 1, 0, i + j > 0);
+                            if (lx_elect()) product(s, false, 0, 0, i + j > 0);
                             __syncwarp();
                             if (++s == STAGES) { s = 0; ph ^= 1; }
                         }
@@ -334,7 +340,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LX_THREADS, 1) lx_ge
                         if (i == 0 && !wait(&acc_empty[1], ((turn >> 1) & 1) ^ 1)) break;
                         for (int j = 0; j < group; j++) {
                             if (lx_elect()) {
-                                product(st, 2, 1, i + j > 0);
+                                product(st, false, 1, 1, i + j > 0);
                                 lx_commit(&empty[st]);
                             }
                             __syncwarp();
@@ -356,12 +362,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LX_THREADS, 1) lx_ge
                         r.next();
                         const bool last = r.first();                  // the accumulator is complete
                         if (lx_elect()) {
-                            if constexpr (MODE == LX_TWO) {
-                                product(st, 2, turn & 1, more);
-                                product(st, 1, turn & 1, true);
-                            } else {
-                                product(st, 1, turn & 1, more);
-                            }
+                            if constexpr (SPLIT) product(st, true, 0, turn & 1, more);
+                            if constexpr (LOW_B) product(st, false, 1, turn & 1, more || SPLIT);
+                            product(st, false, 0, turn & 1, more || LOW_B);
                             lx_commit(&empty[st]);
                             if (last) lx_commit(&acc_full[turn & 1]);
                         }
@@ -378,7 +381,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LX_THREADS, 1) lx_ge
         mbar_wait_bounded(&drained, 0);
     } else {
         const int quad = warp & 3, row = quad * 32 + lane;   // a warp reads the accumulator lanes of its place in the group of four
-        const int c0 = warp >= 2 + LX_EPI_WARPS / 2 ? LX_COLS : 0;
+        const int c0 = warp >= 2 + LX_EPI_WARPS / 2 ? COLS : 0;
         uint32_t turn = 0;
         bool ok = true;
         const float unscale = a.scales ? (EPI == LX_DTABLE ? a.scales[0] : EPI == LX_DX ? a.scales[1] : a.scales[0] * a.scales[1]) : 1.0f;
@@ -393,13 +396,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LX_THREADS, 1) lx_ge
             if constexpr (EPI == LX_STATS || EPI == LX_DLOGITS) id = live ? lx_target(a.targets, a.id_u16, a.V, m) : -1;
             if constexpr (EPI == LX_DLOGITS) lse2 = live ? a.lse2[m] : 0.0f;
             for (int h = 0; h < ACCS && ok; h++) {
-                const int n0 = nt * TILE_N + h * LX_BN + c0;
-                const int left = a.n - n0, cols = left < 0 ? 0 : left < LX_COLS ? left : LX_COLS;     // of this warp
-                // This warp's 128 columns into registers; the accumulator is free again before anything is computed.
-                float v[LX_COLS];
-                if constexpr (EPI == LX_DX || EPI == LX_DTABLE) {
+                const int n0 = nt * TILE_N + h * ACC_N + c0;
+                const int left = a.n - n0, cols = left < 0 ? 0 : left < COLS ? left : COLS;     // of this warp
+                // This warp's columns into registers; the accumulator is free again before anything is computed.
+                float v[COLS];
+                if constexpr (SUMS) {
 #pragma unroll
-                    for (int j = 0; j < LX_COLS; j++) v[j] = 0.0f;
+                    for (int j = 0; j < COLS; j++) v[j] = 0.0f;
                 }
                 for (int part = range.k0; part < range.k1; part += a.span, turn++) {
                     ok = __all_sync(0xffffffffu, lx_wait(&acc_full[turn & 1], (turn >> 1) & 1, abort));
@@ -407,12 +410,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LX_THREADS, 1) lx_ge
                     lx_fence_after();
                     const uint32_t t = tmem + (turn & 1) * LX_BN + c0 + ((uint32_t)(quad * 32) << 16);
 #pragma unroll
-                    for (int c = 0; c < LX_COLS; c += 32) {
+                    for (int c = 0; c < COLS; c += 32) {
                         float w[32];
                         lx_tmem_load(t + c, w);
 #pragma unroll
                         for (int j = 0; j < 32; j++) {
-                            if constexpr (EPI == LX_DX || EPI == LX_DTABLE) v[c + j] += w[j];
+                            if constexpr (SUMS) v[c + j] += w[j];
                             else v[c + j] = w[j];
                         }
                     }
@@ -424,28 +427,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LX_THREADS, 1) lx_ge
                 if constexpr (EPI == LX_STATS) {
                     const int tgt = id >= 0 ? id - a.v0 - n0 : -1;     // column of this warp
                     const float k2 = unscale * LX_LOG2E;
-                    if (__any_sync(0xffffffffu, tgt >= 0 && tgt < LX_COLS)) {
+                    if (__any_sync(0xffffffffu, tgt >= 0 && tgt < COLS)) {
                         float hit = 0.0f;
 #pragma unroll
-                        for (int j = 0; j < LX_COLS; j++) hit = tgt == j ? v[j] : hit;
-                        if (tgt >= 0 && tgt < LX_COLS) a.hit[m] = hit * unscale;
+                        for (int j = 0; j < COLS; j++) hit = tgt == j ? v[j] : hit;
+                        if (tgt >= 0 && tgt < COLS) a.hit[m] = hit * unscale;
                     }
-                    if (cols < LX_COLS) {
+                    if (cols < COLS) {
 #pragma unroll
-                        for (int j = 0; j < LX_COLS; j++) if (j >= cols) v[j] = -INFINITY;
+                        for (int j = 0; j < COLS; j++) if (j >= cols) v[j] = -INFINITY;
                     }
                     float top[4] = {v[0], v[1], v[2], v[3]}, sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                    for (int j = 4; j < LX_COLS; j++) top[j & 3] = fmaxf(top[j & 3], v[j]);
+                    for (int j = 4; j < COLS; j++) top[j & 3] = fmaxf(top[j & 3], v[j]);
                     const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * k2;
 #pragma unroll
-                    for (int j = 0; j < LX_COLS; j++) sum[j & 3] += lx_exp2(fmaf(v[j], k2, -mx));
-                    if (live && cols > 0) a.part[(size_t)(a.tile0 + (n0 / LX_COLS)) * a.ldt + m] = make_float2(mx, (sum[0] + sum[1]) + (sum[2] + sum[3]));
+                    for (int j = 0; j < COLS; j++) sum[j & 3] += lx_exp2(fmaf(v[j], k2, -mx));
+                    if (live && cols > 0) a.part[(size_t)(a.tile0 + (n0 / COLS)) * a.ldt + m] = make_float2(mx, (sum[0] + sum[1]) + (sum[2] + sum[3]));
                 } else if constexpr (EPI == LX_DLOGITS) {
                     const int tgt = id >= 0 ? id - a.v0 - n0 : -1;
                     const float k2 = unscale * LX_LOG2E;
                     const float shift = log2f(a.dscale) - lse2;          // a power of two: exp2 brings it in
-                    const bool mine = __any_sync(0xffffffffu, tgt >= 0 && tgt < LX_COLS);
+                    const bool mine = __any_sync(0xffffffffu, tgt >= 0 && tgt < COLS);
                     const int row0 = mt * LX_BM + rank * LX_CTA_M + quad * 32;
                     const uint32_t stage = base + STAGES * STAGE_BYTES + (warp - 2) * LX_STAGING_BYTES;
                     // 32 columns at a time through this warp's shared memory to the copy engine: 64-byte rows, swizzled as it
@@ -453,7 +456,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LX_THREADS, 1) lx_ge
                     // 22.2 us instead of 20.0 for one sequence over 9200 rows, 2.22 ms instead of 2.15 for 8192 tokens over
                     // 151936 (the whole call there: the same within its spread, the power cap sets it).
 #pragma unroll
-                    for (int c = 0; c < LX_COLS; c += 32) {
+                    for (int c = 0; c < COLS; c += 32) {
                         if (c >= cols || row0 >= a.m) break;
                         if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");     // the staging is free again
                         __syncwarp();
@@ -491,10 +494,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LX_THREADS, 1) lx_ge
                     const float k = EPI == LX_DTABLE ? a.alpha * unscale : unscale;
                     if (EPI == LX_DX && a.first) {
 #pragma unroll
-                        for (int j = 0; j < LX_COLS; j++) if (j < cols) out[(size_t)j * a.ldt] = v[j] * k;
+                        for (int j = 0; j < COLS; j++) if (j < cols) out[(size_t)j * a.ldt] = v[j] * k;
                     } else if (!none) {
 #pragma unroll
-                        for (int j = 0; j < LX_COLS; j++) if (j < cols) lx_add(out + (size_t)j * a.ldt, v[j] * k);
+                        for (int j = 0; j < COLS; j++) if (j < cols) lx_add(out + (size_t)j * a.ldt, v[j] * k);
                     }
                 }
             }
@@ -928,33 +931,48 @@ template <int EPI, int MODE, bool HALF> static int lx_start_kernel(cudaStream_t 
 }
 // The type of the operands is the instruction's business; only dlogits writes 16-bit values itself.
 template <int EPI, int MODE> static int lx_start(cudaStream_t st, const LxMaps &maps, const LxArgs &a) {
-    if (EPI == LX_DLOGITS && a.half_type) return lx_start_kernel<EPI, MODE, EPI == LX_DLOGITS>(st, maps, a);
-    return lx_start_kernel<EPI, MODE, false>(st, maps, a);
+    constexpr bool WRITES = EPI == LX_DLOGITS, FP16_ONLY = WRITES && (MODE == LX_SPLIT || MODE == LX_NARROW);
+    if (FP16_ONLY || (WRITES && a.half_type)) return lx_start_kernel<EPI, MODE, WRITES>(st, maps, a);
+    return lx_start_kernel<EPI, MODE, FP16_ONLY>(st, maps, a);
 }
 
 // Time of a product of `tiles` accumulators of 256 x 256 (m x n of them), in K blocks of one accumulator: waves over the SM
 // pairs.  A wide tile takes the time of 1.55 plain ones (clocks per K block, 512 for a plain accumulator's instructions: about
 // 850 plain, 1300 wide).  Losses of 16 tokens over 151936 rows: 84 us wide, 101 plain; all of 8192 tokens: 10.3 against 10.4 ms.
-constexpr double LX_WIDE_COST = 1.55;
-static double lx_cost(int m, int n, int splits, bool can_be_wide, bool *wide) {
-    const double plain = lx_div((long long)m * n * splits, lx_pairs()), w = lx_div((long long)m * lx_div(n, 2) * splits, lx_pairs()) * LX_WIDE_COST;
-    const bool is = can_be_wide && tuning("linear_xent_wide", w < plain) != 0;
+// Split inputs take about two plain ones: four boxes for three products.
+constexpr double LX_WIDE_COST = 1.55, LX_SPLIT_COST = 2.0;
+static double lx_cost(int m, int n, int splits, bool split, bool *wide) {
+    const double plain = lx_div((long long)m * n * splits, lx_pairs()) * (split ? LX_SPLIT_COST : 1.0), w = lx_div((long long)m * lx_div(n, 2) * splits, lx_pairs()) * LX_WIDE_COST;
+    const bool is = !split && tuning("linear_xent_wide", w < plain) != 0;
     if (wide) *wide = is;
     return is ? w : plain;
 }
-// n_tiles of `a` counts accumulators; one operand pair may run wide.
-template <int EPI> static int lx_launch(cudaStream_t st, const LxMaps &maps, LxArgs a) {
+// Tiles of 256 x 128 for products of split inputs with m x (n columns) outputs, where 256 x 256 ones leave pairs idle.  A narrow
+// tile takes about 0.6 of the time.  Losses, 768 channels, 9200 rows, plain / narrow: 256 tokens 40.1 / 34.2 us (36 tiles for 74
+// pairs), 512 42.5 / 41.5, 768 54.6 / 49.8, 1024 57.5 / 57.4, 2048 87.5 / 92.2.
+static bool lx_narrow(int m, int n) {
+    return tuning("linear_xent_narrow", lx_div((long long)m * lx_div(n, LX_BN / 2), lx_pairs()) * 0.6 < lx_div((long long)m * lx_div(n, LX_BN), lx_pairs())) != 0;
+}
+// n_tiles of `a` counts accumulators; operands of one part may run wide.
+template <int EPI> static int lx_launch(cudaStream_t st, const LxMaps &maps, LxArgs a, bool split, bool narrow = false) {
+    if constexpr (EPI == LX_STATS || EPI == LX_DLOGITS) {
+        if (narrow) return lx_start<EPI, LX_NARROW>(st, maps, a);
+    }
+    if (split) return lx_start<EPI, LX_SPLIT>(st, maps, a);
     bool wide = false;
-    lx_cost(a.m_tiles, a.n_tiles, a.splits, a.segments == 1, &wide);
+    lx_cost(a.m_tiles, a.n_tiles, a.splits, false, &wide);
     if (!wide) return lx_start<EPI, LX_PLAIN>(st, maps, a);
     a.n_tiles = lx_div(a.n_tiles, 2);
     return lx_start<EPI, LX_WIDE>(st, maps, a);
 }
 
+// K blocks after which an fp32 sum leaves the accumulator, with `products` steps for every 16 of K.
+static int lx_span(int products) { return LX_STEPS * 16 / (products * LX_BK); }
+
 // Instruction descriptor: fp32 accumulator, 16-bit operands of one type, their layouts, the tile.
-static uint32_t lx_idesc(bool half_type, bool a_mn, bool b_mn) {
+static uint32_t lx_idesc(bool half_type, bool a_mn, bool b_mn, int acc_n = LX_BN) {
     const uint32_t f = half_type ? 0u : 1u;
-    return 1u << 4 | f << 7 | f << 10 | (a_mn ? 1u : 0u) << 15 | (b_mn ? 1u : 0u) << 16 | (uint32_t)(LX_BN >> 3) << 17 | (uint32_t)(LX_BM >> 4) << 24;
+    return 1u << 4 | f << 7 | f << 10 | (a_mn ? 1u : 0u) << 15 | (b_mn ? 1u : 0u) << 16 | (uint32_t)(acc_n >> 3) << 17 | (uint32_t)(LX_BM >> 4) << 24;
 }
 
 struct LxCall {
@@ -976,7 +994,7 @@ struct LxPlan { int chunk, piece_tiles, splits; };
 // stay within 768 MiB (128, 192, 384, 768 MiB: 12.0, 11.4, 10.8, 10.3 ms for 8192 tokens x 151936 rows x 1024
 // channels under the power cap: a launch of dx has one tile per pair and nothing to hide its end behind).  dx has few tiles
 // and a long K: where its tiles leave pairs idle, K is cut into shares.
-static LxPlan lx_plan(int T_all, int D, int V, int segs, bool dx, bool d_table, bool two_parts) {
+static LxPlan lx_plan(int T_all, int D, int V, bool split, bool dx, bool d_table, bool two_parts) {
     LxPlan p;
     const int rounds = lx_div(T_all, 8192), pairs = lx_pairs();
     p.chunk = (int)round_up((size_t)lx_div(T_all, rounds), LX_BM);
@@ -999,9 +1017,9 @@ static LxPlan lx_plan(int T_all, int D, int V, int segs, bool dx, bool d_table, 
         double cost = 0.0;
         for (int i = 0; i < 2; i++) {                       // the whole pieces and the last
             const int tiles = i ? vt - (pieces - 1) * n : n, times = i ? 1 : pieces - 1;
-            double c = lx_cost(mt, tiles, 1, segs == 1, nullptr) * segs * kd + 4;
-            if (dx) c += lx_cost(mt, dt, splits, segs == 1, nullptr) * lx_div((long long)segs * tiles * 4, splits) + 4;
-            if (d_table) c += (double)lx_div((long long)dt * tiles, pairs) * (segs == 3 ? 3 : LX_WIDE_COST) * kt + 4;
+            double c = lx_cost(mt, tiles, 1, split, nullptr) * kd + 4;
+            if (dx) c += lx_cost(mt, dt, splits, split, nullptr) * lx_div((long long)tiles * 4, splits) + 4;
+            if (d_table) c += (double)lx_div((long long)dt * tiles, pairs) * (split ? LX_SPLIT_COST : LX_WIDE_COST) * kt + 4;
             cost += c * times;
         }
         if (cost < best * 0.999) { best = cost; p.piece_tiles = n; p.splits = splits; }
@@ -1068,19 +1086,21 @@ template <typename T, typename H> static int lx_run(const LxCall &c) {
     const size_t ldd = round_up((size_t)D, 8);
     const bool pack_table = split || D % 8 || !aligned16(c.table);
     const bool need_lo = c.d_table || split;
-    const int segs = split ? 3 : 1;
-    const LxPlan plan = lx_plan(T_all, D, V, segs, c.dx != nullptr, c.d_table != nullptr, need_lo);
+    const LxPlan plan = lx_plan(T_all, D, V, split, c.dx != nullptr, c.d_table != nullptr, need_lo);
     const int chunk = plan.chunk, vp = plan.piece_tiles * LX_BN < V ? plan.piece_tiles * LX_BN : V, splits = plan.splits;
     const size_t ldt = round_up((size_t)chunk, 32), ldl = (size_t)plan.piece_tiles * LX_BN;
-    const int halves = lx_div(V, LX_COLS);
     // A table that has to be packed is packed once where that takes up to 256 MiB, else piece by piece.
     const size_t row_bytes = ldd * 2 * (split ? 2 : 1);
     const int vk = !pack_table ? 0 : (size_t)V * row_bytes <= ((size_t)256 << 20) ? V : vp;
+    // statistics: the whole table in one launch, or piece by piece where it is packed so; a (max, sum) pair per epilogue warp's columns
+    const int fstep = pack_table && vk < V ? vp : V;
+    const bool narrow_stats = split && lx_narrow(lx_div(chunk, LX_BM), fstep);
+    const int stat_cols = (narrow_stats ? lx_acc_n(LX_NARROW) : LX_BN) / 2, parts_n = lx_div(V, stat_cols);
 
     size_t off = 0;
     auto take = [&](size_t bytes) { const size_t at = off; off += round_up(bytes, 1024); return at; };
     const size_t o_most = take(split ? 2 * LX_LARGEST_BLOCKS * 4 : 0), o_scales = take(16);
-    const size_t o_tok = take(c.loss_tok ? 0 : (size_t)T_all * 4), o_lse = take(ldt * 4), o_hit = take(ldt * 4), o_part = take((size_t)halves * ldt * 8);
+    const size_t o_tok = take(c.loss_tok ? 0 : (size_t)T_all * 4), o_lse = take(ldt * 4), o_hit = take(ldt * 4), o_part = take((size_t)parts_n * ldt * 8);
     const size_t o_xh = take((size_t)chunk * ldd * 2), o_xl = take(split ? (size_t)chunk * ldd * 2 : 0);
     const size_t o_eh = take((size_t)vk * ldd * 2), o_el = take(split ? (size_t)vk * ldd * 2 : 0);
     const size_t o_lh = take(grad ? (size_t)chunk * ldl * 2 : 0), o_ll = take(grad && need_lo ? (size_t)chunk * ldl * 2 : 0);
@@ -1129,14 +1149,13 @@ template <typename T, typename H> static int lx_run(const LxCall &c) {
         rows_lo = !split ? nullptr : vk < V ? el : el + (size_t)v0 * ldd;
         return ANE_CUDA_OK;
     };
-    // Operand pairs, the ones with a low part first.
-    auto maps_for = [&](LxMaps &m, int n, const void *ah, const void *al, const void *bh, const void *bl, size_t arows, size_t acols, size_t lda, int abox, size_t brows,
-                        size_t bcols, size_t ldb, int bbox) -> int {
-        const void *as[3] = {al, ah, ah}, *bs[3] = {bh, bl, bh};
-        for (int i = 0; i < n; i++) {
-            if (int rc = make_matrix_map(&m.a[i], part, as[3 - n + i], arows, acols, lda, abox)) return rc;
-            if (int rc = make_matrix_map(&m.b[i], part, bs[3 - n + i], brows, bcols, ldb, bbox)) return rc;
-        }
+    // Operands; low parts that are null are not in use.
+    auto maps_for = [&](LxMaps &m, const void *ah, const void *al, const void *bh, const void *bl, size_t arows, size_t acols, size_t lda, int abox, size_t brows, size_t bcols,
+                        size_t ldb, int bbox) -> int {
+        if (int rc = make_matrix_map(&m.a[0], part, ah, arows, acols, lda, abox)) return rc;
+        if (int rc = make_matrix_map(&m.b[0], part, bh, brows, bcols, ldb, bbox)) return rc;
+        if (al) if (int rc = make_matrix_map(&m.a[1], part, al, arows, acols, lda, abox)) return rc;
+        if (bl) if (int rc = make_matrix_map(&m.b[1], part, bl, brows, bcols, ldb, bbox)) return rc;
         return ANE_CUDA_OK;
     };
 
@@ -1148,67 +1167,66 @@ template <typename T, typename H> static int lx_run(const LxCall &c) {
         ANE_LAUNCH_OK(1);
 
         LxArgs a = {};
-        a.segments = segs; a.kblocks = lx_div(D, LX_BK); a.splits = 1; a.span = 1 << 20;
+        a.kblocks = lx_div(D, LX_BK); a.splits = 1; a.span = split ? 3 * lx_span(3) : 1 << 20;
         a.m_tiles = lx_div(n_tok, LX_BM); a.m = n_tok;
-        a.idesc = lx_idesc(half_type, false, false);
         a.targets = tg; a.id_u16 = c.id_u16; a.V = V;
         a.scales = scales;
         a.part = parts; a.hit = hit; a.lse2 = lse2; a.ldt = ldt;
         a.half_type = half_type; a.dscale = half_type ? LX_HALF_SCALE : 1.0f;
         a.status = status;
-        // statistics: the whole table in one launch, or piece by piece where it is packed so
-        const int fstep = pack_table && vk < V ? vp : V;
+        const auto forward_args = [&](int v0, int nv, bool narrow) {
+            const int acc_n = lx_acc_n(narrow ? LX_NARROW : LX_PLAIN);
+            a.n_tiles = lx_div(nv, acc_n); a.n = nv; a.v0 = v0;
+            a.idesc = lx_idesc(half_type, false, false, acc_n);
+        };
         for (int v0 = 0; v0 < V; v0 += fstep) {
             const int nv = V - v0 < fstep ? V - v0 : fstep;
             LxMaps m;
             if (int rc = table_rows(v0, nv)) return rc;
-            if (int rc = maps_for(m, segs, xh, xl, rows_hi, rows_lo, n_tok, D, ldd, LX_CTA_M, nv, D, ld, LX_BN / 2)) return rc;
-            a.n_tiles = lx_div(nv, LX_BN); a.n = nv; a.v0 = v0; a.tile0 = v0 / LX_COLS;
-            if (int rc = lx_launch<LX_STATS>(c.st, m, a)) return rc;
+            if (int rc = maps_for(m, xh, xl, rows_hi, rows_lo, n_tok, D, ldd, LX_CTA_M, nv, D, ld, stat_cols)) return rc;
+            forward_args(v0, nv, narrow_stats);
+            a.tile0 = v0 / stat_cols;
+            if (int rc = lx_launch<LX_STATS>(c.st, m, a, split, narrow_stats)) return rc;
         }
         // few tokens: more threads for each
-        if (n_tok <= 1024) lx_call(lx_join_kernel<4>, dim3(lx_div(n_tok, 4)), dim3(1024), 0, c.st, lse2, loss_tok + t0, parts, hit, tg, c.id_u16, V, halves, n_tok, ldt, status);
-        else lx_call(lx_join_kernel<32>, dim3(lx_div(n_tok, 32)), dim3(1024), 0, c.st, lse2, loss_tok + t0, parts, hit, tg, c.id_u16, V, halves, n_tok, ldt, status);
+        if (n_tok <= 1024) lx_call(lx_join_kernel<4>, dim3(lx_div(n_tok, 4)), dim3(1024), 0, c.st, lse2, loss_tok + t0, parts, hit, tg, c.id_u16, V, parts_n, n_tok, ldt, status);
+        else lx_call(lx_join_kernel<32>, dim3(lx_div(n_tok, 32)), dim3(1024), 0, c.st, lse2, loss_tok + t0, parts, hit, tg, c.id_u16, V, parts_n, n_tok, ldt, status);
         ANE_LAUNCH_OK(1);
         if (!grad) continue;
 
         const float alpha = c.grad_scale / (float)c.S / a.dscale;
         for (int v0 = 0; v0 < V; v0 += vp) {
             const int nv = V - v0 < vp ? V - v0 : vp;
+            const bool narrow = split && lx_narrow(a.m_tiles, nv);
             LxMaps m;
             if (int rc = table_rows(v0, nv)) return rc;
-            if (int rc = maps_for(m, segs, xh, xl, rows_hi, rows_lo, n_tok, D, ldd, LX_CTA_M, nv, D, ld, LX_BN / 2)) return rc;
-            a.n_tiles = lx_div(nv, LX_BN); a.n = nv; a.v0 = v0;
+            if (int rc = maps_for(m, xh, xl, rows_hi, rows_lo, n_tok, D, ldd, LX_CTA_M, nv, D, ld, narrow ? LX_BN / 4 : LX_BN / 2)) return rc;
+            forward_args(v0, nv, narrow);
             if (int rc = make_matrix_map(&m.hi, part, lh, n_tok, nv, ldl, 32, 32)) return rc;
             if (need_lo) if (int rc = make_matrix_map(&m.lo, part, ll, n_tok, nv, ldl, 32, 32)) return rc;
             a.two_parts = need_lo;
-            if (int rc = lx_launch<LX_DLOGITS>(c.st, m, a)) return rc;
+            if (int rc = lx_launch<LX_DLOGITS>(c.st, m, a, split, narrow)) return rc;
             if (c.dx) {
                 LxArgs g = a;
-                if (int rc = maps_for(m, segs, lh, ll, rows_hi, rows_lo, n_tok, nv, ldl, LX_CTA_M, nv, D, ld, LX_BK)) return rc;
+                if (int rc = maps_for(m, lh, split ? ll : nullptr, rows_hi, rows_lo, n_tok, nv, ldl, LX_CTA_M, nv, D, ld, LX_BK)) return rc;
                 g.kblocks = lx_div(nv, LX_BK); g.splits = splits;
-                if (split) g.span = LX_STEPS * 16 / LX_BK;   // a 16-bit result does not show what the accumulator cuts off
+                if (split) g.span = lx_span(3);              // a 16-bit dx does not show what the accumulator cuts off
                 g.n_tiles = lx_div(D, LX_BN); g.n = D;
                 g.idesc = lx_idesc(half_type, false, true);
                 g.out = dxs; g.first = v0 == 0;
-                if (int rc = lx_launch<LX_DX>(c.st, m, g)) return rc;
+                if (int rc = lx_launch<LX_DX>(c.st, m, g, split)) return rc;
             }
             if (c.d_table) {
                 LxArgs g = a;
-                if (split) {
-                    if (int rc = maps_for(m, 3, xh, xl, lh, ll, n_tok, D, ldd, LX_BK, n_tok, nv, ldl, LX_BK)) return rc;
-                    g.span = LX_STEPS * 16 / LX_BK;
-                } else {                                     // both parts of dl beside one box of x: two steps for every 16 of K
-                    if (int rc = maps_for(m, 1, xh, nullptr, lh, nullptr, n_tok, D, ldd, LX_BK, n_tok, nv, ldl, LX_BK)) return rc;
-                    if (int rc = make_matrix_map(&m.b[1], part, ll, n_tok, nv, ldl, LX_BK)) return rc;
-                    g.span = LX_STEPS / 2 * 16 / LX_BK;
-                }
+                // 16-bit inputs: both parts of dl beside one box of x, two steps for every 16 of K
+                if (int rc = maps_for(m, xh, xl, lh, ll, n_tok, D, ldd, LX_BK, n_tok, nv, ldl, LX_BK)) return rc;
+                g.span = lx_span(split ? 3 : 2);
                 g.kblocks = lx_div(n_tok, LX_BK);
                 g.m_tiles = lx_div(D, LX_BM); g.m = D;
                 g.n_tiles = lx_div(nv, LX_BN); g.n = nv;
                 g.idesc = lx_idesc(half_type, true, true);
                 g.out = c.d_table + (size_t)v0 * D; g.ldt = (size_t)D; g.alpha = alpha;
-                if (int rc = split ? lx_start<LX_DTABLE, LX_PLAIN>(c.st, m, g) : lx_start<LX_DTABLE, LX_TWO>(c.st, m, g)) return rc;
+                if (int rc = split ? lx_start<LX_DTABLE, LX_SPLIT>(c.st, m, g) : lx_start<LX_DTABLE, LX_TWO>(c.st, m, g)) return rc;
             }
         }
         if (c.dx) {

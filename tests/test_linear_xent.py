@@ -135,7 +135,7 @@ def test_losses_and_gradients(ops, shape, dt):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("knob", [("linear_xent_few", 0), ("linear_xent_wide", 0), ("linear_xent_wide", 1), ("linear_xent_dep", 0)])
+@pytest.mark.parametrize("knob", [("linear_xent_few", 0), ("linear_xent_wide", 0), ("linear_xent_wide", 1), ("linear_xent_narrow", 0), ("linear_xent_narrow", 1), ("linear_xent_dep", 0)])
 @pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("shape", [(1, 64, 700, 1), (3, 33, 100, 1), (2, 200, 1300, 77), (1, 520, 600, 300)])
 def test_alternate_kernels(ops, shape, dt, knob):
