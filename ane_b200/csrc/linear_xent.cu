@@ -555,80 +555,101 @@ __global__ void __launch_bounds__(256) lx_largest_kernel(uint32_t *most, const f
         most[blockIdx.y * LX_LARGEST_BLOCKS + blockIdx.x] = top;
     }
 }
-// -> scales[0..1] = 1 / scale of x and of the table, scales[2..3] the scales: powers of two that put the largest at 2^13.
-__global__ void __launch_bounds__(64) lx_scales_kernel(float *scales, const uint32_t *most, int blocks) {
-    dep_sync();
-    const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+// The exponent of the power of two that puts the largest magnitude of x (which = 0) or of the table (1) at 2^13.  256 threads;
+// `sh` holds 8 words, each call its own.
+__device__ __forceinline__ int lx_exponent(const uint32_t *most, int blocks, int which, uint32_t *sh) {
     uint32_t top = 0;
-    for (int i = lane; i < blocks; i += 32) { const uint32_t u = most[w * LX_LARGEST_BLOCKS + i]; top = u > top ? u : top; }
+    for (int i = threadIdx.x; i < blocks; i += 256) { const uint32_t u = most[which * LX_LARGEST_BLOCKS + i]; top = u > top ? u : top; }
     top = __reduce_max_sync(0xffffffffu, top);
-    int e = 13 - ((int)(top >> 23) - 127);
-    e = top == 0 ? 0 : e > 60 ? 60 : e < -60 ? -60 : e;
-    if (lane == 0) {
-        scales[w] = __uint_as_float((uint32_t)(127 - e) << 23);
-        scales[2 + w] = __uint_as_float((uint32_t)(127 + e) << 23);
-    }
-}
-
-// x of tokens [t0, t0 + tokens) -> [token][ldx] 16-bit rows, zeros for tokens without a target; fp32 scaled, as two parts.
-template <typename T, typename H>
-__global__ void __launch_bounds__(256) lx_pack_x_kernel(H *hi, H *lo, const T *__restrict__ x, const float *scales, const void *__restrict__ targets, int id_u16, int V, int t0,
-                                                        int tokens, int D, int S, size_t ldx) {
-    __shared__ float tile[32][33];
-    dep_sync();
-    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-    const int t = blockIdx.x * 32 + tx, d0 = blockIdx.y * 32;
-    const bool live = t < tokens && lx_target(targets, id_u16, V, t0 + t) >= 0;
-    const int b = (t0 + t) / S, s = (t0 + t) % S;
-    const float scale = scales ? scales[2] : 1.0f;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const int d = d0 + ty + 8 * i;
-        tile[ty + 8 * i][tx] = live && d < D ? Elt<T>::to_f(x[((size_t)b * D + d) * S + s]) * scale : 0.0f;
-    }
+    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = top;
     __syncthreads();
-    const int d = d0 + tx;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const int r = blockIdx.x * 32 + ty + 8 * i;
-        if (r < tokens && d < (int)ldx) {
-            const float v = tile[tx][ty + 8 * i];
-            const H h = Elt<H>::from_f(v);
-            hi[(size_t)r * ldx + d] = h;
-            if (lo) lo[(size_t)r * ldx + d] = Elt<H>::from_f(v - Elt<H>::to_f(h));
+    for (int i = 0; i < 8; i++) top = sh[i] > top ? sh[i] : top;
+    const int e = 13 - ((int)(top >> 23) - 127);
+    return top == 0 ? 0 : e > 60 ? 60 : e < -60 ? -60 : e;
+}
+__device__ __forceinline__ float lx_power(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+
+// Operands of the products.  The first `x_blocks` blocks: x of tokens [t0, t0 + tokens) -> [token][ld] 16-bit rows, zeros for
+// tokens without a target.  The others: `rows` rows of the table -> [row][ld] with aligned ends; `flat`: rows without a gap on both
+// sides (ld == D), eight elements at a time.  fp32 (most not null) scaled, as two parts; the first block leaves the inverse scales of
+// x and of the table for the products.
+template <typename T, typename H> struct LxPack {
+    H *xh, *xl;
+    const T *x;
+    int x_blocks, t0, tokens, S;
+    const void *targets; int id_u16, V;
+    H *eh, *el;
+    const T *table;
+    int rows, flat;
+    int D; size_t ld;
+    const uint32_t *most; int blocks;
+    float *scales;
+};
+template <typename T, typename H> __global__ void __launch_bounds__(256) lx_pack_kernel(const __grid_constant__ LxPack<T, H> p) {
+    __shared__ float tile[32][33];
+    __shared__ uint32_t sh[2][8];
+    dep_sync();
+    const int D = p.D, bx = blockIdx.x;
+    const size_t ld = p.ld;
+    const bool of_x = bx < p.x_blocks;
+    float scale = 1.0f;
+    if (p.most) {
+        const int e = lx_exponent(p.most, p.blocks, of_x ? 0 : 1, sh[0]);
+        scale = lx_power(e);
+        if (bx == 0) {
+            const int other = lx_exponent(p.most, p.blocks, of_x ? 1 : 0, sh[1]);
+            if (threadIdx.x == 0) { p.scales[of_x ? 0 : 1] = lx_power(-e); p.scales[of_x ? 1 : 0] = lx_power(-other); }
         }
     }
-}
-
-// Rows of the table -> [row][lde] 16-bit rows with aligned ends; fp32 scaled, as two parts.  `flat`: rows without a gap on
-// both sides (lde == D), eight elements at a time.
-template <typename T, typename H>
-__global__ void __launch_bounds__(256) lx_pack_rows_kernel(H *hi, H *lo, const T *__restrict__ src, const float *scales, int rows, int D, size_t lde, int flat) {
-    dep_sync();
-    const float scale = scales ? scales[3] : 1.0f;
-    if (sizeof(T) == 4 && flat) {
-        const size_t n = (size_t)rows * D / 8, step = (size_t)gridDim.x * 256;
-        for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += step) {
+    if (of_x) {
+        const int tiles = (p.tokens + 31) / 32, r0 = bx % tiles * 32, d0 = bx / tiles * 32;
+        const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, t = r0 + tx;
+        const bool live = t < p.tokens && lx_target(p.targets, p.id_u16, p.V, p.t0 + t) >= 0;
+        const int b = (p.t0 + t) / p.S, s = (p.t0 + t) % p.S;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int d = d0 + ty + 8 * i;
+            tile[ty + 8 * i][tx] = live && d < D ? Elt<T>::to_f(p.x[((size_t)b * D + d) * p.S + s]) * scale : 0.0f;
+        }
+        __syncthreads();
+        const int d = d0 + tx;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int r = r0 + ty + 8 * i;
+            if (r < p.tokens && d < (int)ld) {
+                const float v = tile[tx][ty + 8 * i];
+                const H h = Elt<H>::from_f(v);
+                p.xh[(size_t)r * ld + d] = h;
+                if (p.xl) p.xl[(size_t)r * ld + d] = Elt<H>::from_f(v - Elt<H>::to_f(h));
+            }
+        }
+        return;
+    }
+    const int first = bx - p.x_blocks, step = gridDim.x - p.x_blocks;
+    if (sizeof(T) == 4 && p.flat) {
+        const size_t n = (size_t)p.rows * D / 8;
+        for (size_t i = (size_t)first * 256 + threadIdx.x; i < n; i += (size_t)step * 256) {
             float f[8], h[8];
-            Elt<float>::unpack(reinterpret_cast<const uint4 *>(src)[2 * i], f);
-            Elt<float>::unpack(reinterpret_cast<const uint4 *>(src)[2 * i + 1], f + 4);
+            Elt<float>::unpack(reinterpret_cast<const uint4 *>(p.table)[2 * i], f);
+            Elt<float>::unpack(reinterpret_cast<const uint4 *>(p.table)[2 * i + 1], f + 4);
 #pragma unroll
             for (int j = 0; j < 8; j++) f[j] *= scale;
             const uint4 q = Elt<H>::pack(f);
             Elt<H>::unpack(q, h);
-            reinterpret_cast<uint4 *>(hi)[i] = q;
+            reinterpret_cast<uint4 *>(p.eh)[i] = q;
 #pragma unroll
             for (int j = 0; j < 8; j++) f[j] -= h[j];
-            reinterpret_cast<uint4 *>(lo)[i] = Elt<H>::pack(f);
+            reinterpret_cast<uint4 *>(p.el)[i] = Elt<H>::pack(f);
         }
         return;
     }
-    for (int r = blockIdx.x; r < rows; r += gridDim.x)
-        for (int d = threadIdx.x; d < (int)lde; d += 256) {
-            const float v = d < D ? Elt<T>::to_f(src[(size_t)r * D + d]) * scale : 0.0f;
+    for (int r = first; r < p.rows; r += step)
+        for (int d = threadIdx.x; d < (int)ld; d += 256) {
+            const float v = d < D ? Elt<T>::to_f(p.table[(size_t)r * D + d]) * scale : 0.0f;
             const H h = Elt<H>::from_f(v);
-            hi[(size_t)r * lde + d] = h;
-            if (lo) lo[(size_t)r * lde + d] = Elt<H>::from_f(v - Elt<H>::to_f(h));
+            p.eh[(size_t)r * ld + d] = h;
+            if (p.el) p.el[(size_t)r * ld + d] = Elt<H>::from_f(v - Elt<H>::to_f(h));
         }
 }
 
@@ -687,16 +708,38 @@ __global__ void __launch_bounds__(1024) lx_join_kernel(float *__restrict__ lse2,
     loss_tok[token] = loss;
 }
 
+// loss_seq[b] = (sum_t loss_tok[b][t]) / S, fixed summation tree of 256 threads.
+__device__ __forceinline__ void lx_sequence_loss(float *loss_seq, const float *loss_tok, int S, int b, float *sh) {
+    const float *p = loss_tok + (size_t)b * S;
+    float acc = 0.0f;
+    for (int t = threadIdx.x; t < S; t += 256) acc += p[t];
+    acc = warp_sum(acc);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = acc;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        float s = 0.0f;
+        for (int i = 0; i < 8; i++) s += sh[i];
+        loss_seq[b] = s / (float)S;
+    }
+}
+
 // dx[b][d][s] = alpha * sum over the shares of K, in order.  A token without a target has zeros, whatever the table holds.
 template <typename T>
 __global__ void __launch_bounds__(256) lx_finish_dx_kernel(T *__restrict__ dx, const float *__restrict__ sums, const void *__restrict__ targets, int id_u16, int V, int splits,
-                                                           int t0, int tokens, int D, int S, size_t ldt, float alpha) {
+                                                           int t0, int tokens, int D, int S, size_t ldt, float alpha, float *loss_seq, const float *loss_tok, int seqs) {
+    __shared__ float sh[8];
     dep_sync();
+    const int by = loss_seq ? gridDim.y - 1 : gridDim.y;             // the last row of blocks: losses of the sequences
+    if (blockIdx.y == by) {
+        for (int b = blockIdx.x; b < seqs; b += gridDim.x) lx_sequence_loss(loss_seq, loss_tok, S, b, sh);
+        return;
+    }
     const int t = blockIdx.x * 256 + threadIdx.x;
     if (t >= tokens) return;
     const bool live = lx_target(targets, id_u16, V, t0 + t) >= 0;
     const int b = (t0 + t) / S, s = (t0 + t) % S;
-    for (int d = blockIdx.y; d < D; d += gridDim.y) {
+    for (int d = blockIdx.y; d < D; d += by) {
         float v = 0.0f;
         for (int k = 0; k < splits; k++) v += sums[((size_t)k * D + d) * ldt + t];
         dx[((size_t)b * D + d) * S + s] = Elt<T>::from_f(live ? v * alpha : 0.0f);
@@ -883,21 +926,10 @@ __global__ void __launch_bounds__(256) lf_finish_dx_kernel(T *__restrict__ dx, c
     dx[((size_t)(t / S) * D + d) * S + t % S] = Elt<T>::from_f(lx_target(targets, id_u16, V, t) >= 0 ? a * alpha : 0.0f);
 }
 
-// loss_seq[b] = (sum_t loss_tok[b][t]) / S, fixed summation tree.
 __global__ void __launch_bounds__(256) lx_loss_kernel(float *__restrict__ loss_seq, const float *__restrict__ loss_tok, int S) {
     __shared__ float sh[8];
     dep_sync();
-    const float *p = loss_tok + (size_t)blockIdx.x * S;
-    float acc = 0.0f;
-    for (int t = threadIdx.x; t < S; t += 256) acc += p[t];
-    acc = warp_sum(acc);
-    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = acc;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        float s = 0.0f;
-        for (int i = 0; i < 8; i++) s += sh[i];
-        loss_seq[blockIdx.x] = s / (float)S;
-    }
+    lx_sequence_loss(loss_seq, loss_tok, S, blockIdx.x, sh);
 }
 
 static inline int lx_div(long long a, long long b) { return (int)((a + b - 1) / b); }
@@ -1099,7 +1131,7 @@ template <typename T, typename H> static int lx_run(const LxCall &c) {
 
     size_t off = 0;
     auto take = [&](size_t bytes) { const size_t at = off; off += round_up(bytes, 1024); return at; };
-    const size_t o_most = take(split ? 2 * LX_LARGEST_BLOCKS * 4 : 0), o_scales = take(16);
+    const size_t o_most = take(split ? 2 * LX_LARGEST_BLOCKS * 4 : 0), o_scales = take(8);
     const size_t o_tok = take(c.loss_tok ? 0 : (size_t)T_all * 4), o_lse = take(ldt * 4), o_hit = take(ldt * 4), o_part = take((size_t)parts_n * ldt * 8);
     const size_t o_xh = take((size_t)chunk * ldd * 2), o_xl = take(split ? (size_t)chunk * ldd * 2 : 0);
     const size_t o_eh = take((size_t)vk * ldd * 2), o_el = take(split ? (size_t)vk * ldd * 2 : 0);
@@ -1118,16 +1150,26 @@ template <typename T, typename H> static int lx_run(const LxCall &c) {
     const size_t idb = c.id_u16 ? 2 : 4;
     ane_cuda_status *status = ctx().status;
 
+    int largest_blocks = 0;
     if (split) {
         const size_t nx = (size_t)T_all * D, ne = (size_t)V * D;
         const size_t want = ((nx > ne ? nx : ne) + 4095) / 4096;
-        const int blocks = want < LX_LARGEST_BLOCKS ? (int)want : LX_LARGEST_BLOCKS;
-        lx_call(lx_largest_kernel, dim3(blocks, 2), dim3(256), 0, c.st, most, static_cast<const float *>(c.x), nx, static_cast<const float *>(c.table), ne, c.targets, c.id_u16, V, D, c.S);
-        lx_call(lx_scales_kernel, dim3(1), dim3(64), 0, c.st, scales, most, blocks);
-        ANE_LAUNCH_OK(2);
+        largest_blocks = want < LX_LARGEST_BLOCKS ? (int)want : LX_LARGEST_BLOCKS;
+        lx_call(lx_largest_kernel, dim3(largest_blocks, 2), dim3(256), 0, c.st, most, static_cast<const float *>(c.x), nx, static_cast<const float *>(c.table), ne, c.targets, c.id_u16, V,
+                D, c.S);
+        ANE_LAUNCH_OK(1);
     }
-    // Rows [v0, v0 + nv) of the table as 16-bit rows with `ld` elements between them; packs them where that is needed.
-    int packed = 0;                                          // rows from 0 that stay packed
+    // Packs tokens [t0, t0 + n_tok) of x and rows [v0, v0 + nv) of the table; either may be none.
+    auto pack = [&](int t0, int n_tok, int v0, int nv) -> int {
+        const T *from = static_cast<const T *>(c.table) + (size_t)v0 * D;
+        const int flat = split && D % 8 == 0 && aligned16(from), x_blocks = lx_div(n_tok, 32) * lx_div(D, 32);
+        const size_t want = flat ? ((size_t)nv * D / 8 + 255) / 256 : (size_t)nv;
+        const LxPack<T, H> p = {xh, xl, static_cast<const T *>(c.x), x_blocks, t0, n_tok, c.S, c.targets, c.id_u16, V, eh, el, from, nv, flat, D, ldd, most, largest_blocks, scales};
+        lx_call(lx_pack_kernel<T, H>, dim3((unsigned)(x_blocks + (want < 4096 ? want : 4096))), dim3(256), 0, c.st, p);
+        ANE_LAUNCH_OK(1);
+        return ANE_CUDA_OK;
+    };
+    // Rows [v0, v0 + nv) of the table as 16-bit rows with `ld` elements between them; packs them where that is done piece by piece.
     const H *rows_hi = nullptr, *rows_lo = nullptr;
     size_t ld = ldd;
     auto table_rows = [&](int v0, int nv) -> int {
@@ -1136,15 +1178,7 @@ template <typename T, typename H> static int lx_run(const LxCall &c) {
             ld = (size_t)D;
             return ANE_CUDA_OK;
         }
-        if (vk < V || packed < V) {
-            const int lo = vk < V ? v0 : 0, n = vk < V ? nv : V;
-            const T *from = static_cast<const T *>(c.table) + (size_t)lo * D;
-            const int flat = split && D % 8 == 0 && aligned16(from);
-            const size_t want = flat ? ((size_t)n * D / 8 + 255) / 256 : (size_t)n;
-            lx_call(lx_pack_rows_kernel<T, H>, dim3((unsigned)(want < 4096 ? want : 4096)), dim3(256), 0, c.st, eh, el, from, scales, n, D, ldd, flat);
-            ANE_LAUNCH_OK(1);
-            if (vk == V) packed = V;
-        }
+        if (vk < V) if (int rc = pack(0, 0, v0, nv)) return rc;
         rows_hi = vk < V ? eh : eh + (size_t)v0 * ldd;
         rows_lo = !split ? nullptr : vk < V ? el : el + (size_t)v0 * ldd;
         return ANE_CUDA_OK;
@@ -1159,12 +1193,12 @@ template <typename T, typename H> static int lx_run(const LxCall &c) {
         return ANE_CUDA_OK;
     };
 
+    bool with_dx = false;                                    // the sequences' losses are made beside the last dx
     for (int t0 = 0; t0 < T_all; t0 += chunk) {
         const int n_tok = T_all - t0 < chunk ? T_all - t0 : chunk;
         const void *tg = static_cast<const char *>(c.targets) + (size_t)t0 * idb;
-        lx_call(lx_pack_x_kernel<T, H>, dim3(lx_div(n_tok, 32), lx_div(D, 32)), dim3(256), 0, c.st, xh, xl, static_cast<const T *>(c.x), scales, c.targets, c.id_u16, V, t0, n_tok, D,
-                c.S, ldd);
-        ANE_LAUNCH_OK(1);
+        // the whole table with the first tokens, where it stays packed
+        if (int rc = pack(t0, n_tok, 0, t0 == 0 && pack_table && vk == V ? V : 0)) return rc;
 
         LxArgs a = {};
         a.kblocks = lx_div(D, LX_BK); a.splits = 1; a.span = split ? 3 * lx_span(3) : 1 << 20;
@@ -1231,12 +1265,16 @@ template <typename T, typename H> static int lx_run(const LxCall &c) {
         }
         if (c.dx) {
             const int by = D < 1024 ? D : 1024;
-            lx_call(lx_finish_dx_kernel<T>, dim3(lx_div(n_tok, 256), by), dim3(256), 0, c.st, static_cast<T *>(c.dx), dxs, c.targets, c.id_u16, V, splits, t0, n_tok, D, c.S, ldt, alpha);
+            with_dx = t0 + n_tok == T_all && c.B <= 4 * lx_div(n_tok, 256);      // a block takes a few sequences, one after the other
+            lx_call(lx_finish_dx_kernel<T>, dim3(lx_div(n_tok, 256), by + with_dx), dim3(256), 0, c.st, static_cast<T *>(c.dx), dxs, c.targets, c.id_u16, V, splits, t0, n_tok, D, c.S, ldt,
+                    alpha, with_dx ? c.loss_seq : nullptr, loss_tok, c.B);
             ANE_LAUNCH_OK(1);
         }
     }
-    lx_call(lx_loss_kernel, dim3(c.B), dim3(256), 0, c.st, c.loss_seq, loss_tok, c.S);
-    ANE_LAUNCH_OK(1);
+    if (!with_dx) {
+        lx_call(lx_loss_kernel, dim3(c.B), dim3(256), 0, c.st, c.loss_seq, loss_tok, c.S);
+        ANE_LAUNCH_OK(1);
+    }
     return ANE_CUDA_OK;
 }
 
