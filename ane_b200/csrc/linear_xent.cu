@@ -520,21 +520,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(LX_THREADS, 1) lx_ge
 }
 
 // ------------------------------------------------------------------ around the products
-// fp32 inputs: the largest finite magnitude that each block finds in x (blockIdx.y = 0; where a token has a target) and in the
-// table (1), as the bits of a float, which compare like integers.
-constexpr int LX_LARGEST_BLOCKS = 592;
-__global__ void __launch_bounds__(256) lx_largest_kernel(uint32_t *most, const float *__restrict__ x, size_t nx, const float *__restrict__ table, size_t ne,
+// fp32 inputs: the largest finite magnitude that each block finds in x (the first x_blocks; where a token has a target) or in the
+// table, as the bits of a float, which compare like integers.
+constexpr int LX_LARGEST_BLOCKS = 1184;
+__global__ void __launch_bounds__(256) lx_largest_kernel(uint32_t *most, int x_blocks, const float *__restrict__ x, size_t nx, const float *__restrict__ table, size_t ne,
                                                          const void *__restrict__ targets, int id_u16, int V, int D, int S) {
     dep_sync();
-    const bool of_x = blockIdx.y == 0;
+    const bool of_x = blockIdx.x < x_blocks;
+    const int first = of_x ? 0 : x_blocks, blocks = of_x ? x_blocks : gridDim.x - x_blocks;
     const float *p = of_x ? x : table;
     const size_t n = of_x ? nx : ne;
     uint32_t top = 0;
+    const bool small = n <= 0xffffffffu;                     // 64-bit divisions are five times as long
+    auto has_target = [&](size_t i) {
+        const uint32_t j = (uint32_t)i;
+        return lx_target(targets, id_u16, V, small ? (int)(j / ((uint32_t)D * S) * S + j % S) : (int)(i / ((size_t)D * S) * S + i % S)) >= 0;
+    };
     auto look = [&](float f, size_t i) {
         const uint32_t u = __float_as_uint(f) & 0x7fffffffu;
-        if (u > top && u < 0x7f800000u && (!of_x || lx_target(targets, id_u16, V, (int)(i / ((size_t)D * S) * S + i % S)) >= 0)) top = u;
+        if (u > top && u < 0x7f800000u && (!of_x || has_target(i))) top = u;
     };
-    const size_t step = (size_t)gridDim.x * 256, at = (size_t)blockIdx.x * 256 + threadIdx.x, quads = aligned16(p) ? n / 4 : 0;
+    const size_t step = (size_t)blocks * 256, at = (size_t)(blockIdx.x - first) * 256 + threadIdx.x, quads = aligned16(p) ? n / 4 : 0;
     for (size_t i = at; i < quads; i += 4 * step) {
         float4 q[4];
 #pragma unroll
@@ -552,14 +558,14 @@ __global__ void __launch_bounds__(256) lx_largest_kernel(uint32_t *most, const f
     __syncthreads();
     if (threadIdx.x == 0) {
         for (int i = 1; i < 8; i++) top = sh[i] > top ? sh[i] : top;
-        most[blockIdx.y * LX_LARGEST_BLOCKS + blockIdx.x] = top;
+        most[blockIdx.x] = top;
     }
 }
-// The exponent of the power of two that puts the largest magnitude of x (which = 0) or of the table (1) at 2^13.  256 threads;
-// `sh` holds 8 words, each call its own.
-__device__ __forceinline__ int lx_exponent(const uint32_t *most, int blocks, int which, uint32_t *sh) {
+// The exponent of the power of two that puts the largest magnitude of `blocks` blocks at 2^13.  256 threads; `sh` holds 8 words,
+// each call its own.
+__device__ __forceinline__ int lx_exponent(const uint32_t *most, int blocks, uint32_t *sh) {
     uint32_t top = 0;
-    for (int i = threadIdx.x; i < blocks; i += 256) { const uint32_t u = most[which * LX_LARGEST_BLOCKS + i]; top = u > top ? u : top; }
+    for (int i = threadIdx.x; i < blocks; i += 256) { const uint32_t u = most[i]; top = u > top ? u : top; }
     top = __reduce_max_sync(0xffffffffu, top);
     if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = top;
     __syncthreads();
@@ -583,7 +589,7 @@ template <typename T, typename H> struct LxPack {
     const T *table;
     int rows, flat;
     int D; size_t ld;
-    const uint32_t *most; int blocks;
+    const uint32_t *most; int most_x, most_table;      // blocks that looked at x, at the table
     float *scales;
 };
 template <typename T, typename H> __global__ void __launch_bounds__(256) lx_pack_kernel(const __grid_constant__ LxPack<T, H> p) {
@@ -595,10 +601,11 @@ template <typename T, typename H> __global__ void __launch_bounds__(256) lx_pack
     const bool of_x = bx < p.x_blocks;
     float scale = 1.0f;
     if (p.most) {
-        const int e = lx_exponent(p.most, p.blocks, of_x ? 0 : 1, sh[0]);
+        const auto exponent = [&](bool x, uint32_t *sh) { return lx_exponent(x ? p.most : p.most + p.most_x, x ? p.most_x : p.most_table, sh); };
+        const int e = exponent(of_x, sh[0]);
         scale = lx_power(e);
         if (bx == 0) {
-            const int other = lx_exponent(p.most, p.blocks, of_x ? 1 : 0, sh[1]);
+            const int other = exponent(!of_x, sh[1]);
             if (threadIdx.x == 0) { p.scales[of_x ? 0 : 1] = lx_power(-e); p.scales[of_x ? 1 : 0] = lx_power(-other); }
         }
     }
@@ -980,16 +987,14 @@ static double lx_cost(int m, int n, int splits, bool split, bool *wide) {
     return is ? w : plain;
 }
 // Tiles of 256 x 128 for products of split inputs with m x (n columns) outputs, where 256 x 256 ones leave pairs idle.  A narrow
-// tile takes about 0.6 of the time.  Losses, 768 channels, 9200 rows, plain / narrow: 256 tokens 40.1 / 34.2 us (36 tiles for 74
-// pairs), 512 42.5 / 41.5, 768 54.6 / 49.8, 1024 57.5 / 57.4, 2048 87.5 / 92.2.
+// tile takes about 0.6 of the time.  Losses, 768 channels, 9200 rows, plain / narrow: 256 tokens 37.9 / 32.4 us (36 tiles for 74
+// pairs), 512 40.6 / 39.9, 768 53.2 / 48.5, 1024 55.9 / 55.9, 2048 80.5 / 88.4.  d_table of 256 tokens (108 tiles): 21.9 / 17.7.
 static bool lx_narrow(int m, int n) {
     return tuning("linear_xent_narrow", lx_div((long long)m * lx_div(n, LX_BN / 2), lx_pairs()) * 0.6 < lx_div((long long)m * lx_div(n, LX_BN), lx_pairs())) != 0;
 }
 // n_tiles of `a` counts accumulators; operands of one part may run wide.
 template <int EPI> static int lx_launch(cudaStream_t st, const LxMaps &maps, LxArgs a, bool split, bool narrow = false) {
-    if constexpr (EPI == LX_STATS || EPI == LX_DLOGITS) {
-        if (narrow) return lx_start<EPI, LX_NARROW>(st, maps, a);
-    }
+    if (narrow) return lx_start<EPI, LX_NARROW>(st, maps, a);
     if (split) return lx_start<EPI, LX_SPLIT>(st, maps, a);
     bool wide = false;
     lx_cost(a.m_tiles, a.n_tiles, a.splits, false, &wide);
@@ -1019,7 +1024,7 @@ struct LxCall {
 };
 
 // Sizes of one call: tokens of a round, vocabulary tiles of a piece, shares of K for dx.
-struct LxPlan { int chunk, piece_tiles, splits; };
+struct LxPlan { int chunk, piece_tiles, splits; bool narrow_dx; };
 
 // A round has at most 8192 tokens.  A piece has as many vocabulary tiles as fill whole waves of the SM pairs best, counted in
 // waves of K blocks over all pieces and products (with four K blocks for the start of a launch), while the two parts of dl
@@ -1031,7 +1036,9 @@ static LxPlan lx_plan(int T_all, int D, int V, bool split, bool dx, bool d_table
     const int rounds = lx_div(T_all, 8192), pairs = lx_pairs();
     p.chunk = (int)round_up((size_t)lx_div(T_all, rounds), LX_BM);
     if (p.chunk > T_all) p.chunk = T_all;
-    const int mt = lx_div(p.chunk, LX_BM), dt = lx_div(D, LX_BN), vt = lx_div(V, LX_BN);
+    const int mt = lx_div(p.chunk, LX_BM), wide_dt = lx_div(D, LX_BN), vt = lx_div(V, LX_BN);
+    p.narrow_dx = split && pairs / (mt * wide_dt) > 1;      // half as many shares to store and to add up: 19 us instead of 24 for 256 tokens, 768 channels
+    const int dt = p.narrow_dx ? lx_div(D, LX_BN / 2) : wide_dt;
     const int kd = lx_div(D, LX_BK), kt = lx_div(p.chunk, LX_BK);
     long long most = (768ll << 20) / ((long long)p.chunk * LX_BN * (two_parts ? 4 : 2));
     if (most < 1) most = 1;
@@ -1050,8 +1057,8 @@ static LxPlan lx_plan(int T_all, int D, int V, bool split, bool dx, bool d_table
         for (int i = 0; i < 2; i++) {                       // the whole pieces and the last
             const int tiles = i ? vt - (pieces - 1) * n : n, times = i ? 1 : pieces - 1;
             double c = lx_cost(mt, tiles, 1, split, nullptr) * kd + 4;
-            if (dx) c += lx_cost(mt, dt, splits, split, nullptr) * lx_div((long long)tiles * 4, splits) + 4;
-            if (d_table) c += (double)lx_div((long long)dt * tiles, pairs) * (split ? LX_SPLIT_COST : LX_WIDE_COST) * kt + 4;
+            if (dx) c += lx_cost(mt, dt, splits, split, nullptr) * (p.narrow_dx ? 0.5 : 1.0) * lx_div((long long)tiles * 4, splits) + 4;
+            if (d_table) c += (double)lx_div((long long)wide_dt * tiles, pairs) * (split ? LX_SPLIT_COST : LX_WIDE_COST) * kt + 4;
             cost += c * times;
         }
         if (cost < best * 0.999) { best = cost; p.piece_tiles = n; p.splits = splits; }
@@ -1131,7 +1138,7 @@ template <typename T, typename H> static int lx_run(const LxCall &c) {
 
     size_t off = 0;
     auto take = [&](size_t bytes) { const size_t at = off; off += round_up(bytes, 1024); return at; };
-    const size_t o_most = take(split ? 2 * LX_LARGEST_BLOCKS * 4 : 0), o_scales = take(8);
+    const size_t o_most = take(split ? LX_LARGEST_BLOCKS * 4 : 0), o_scales = take(8);
     const size_t o_tok = take(c.loss_tok ? 0 : (size_t)T_all * 4), o_lse = take(ldt * 4), o_hit = take(ldt * 4), o_part = take((size_t)parts_n * ldt * 8);
     const size_t o_xh = take((size_t)chunk * ldd * 2), o_xl = take(split ? (size_t)chunk * ldd * 2 : 0);
     const size_t o_eh = take((size_t)vk * ldd * 2), o_el = take(split ? (size_t)vk * ldd * 2 : 0);
@@ -1150,13 +1157,14 @@ template <typename T, typename H> static int lx_run(const LxCall &c) {
     const size_t idb = c.id_u16 ? 2 : 4;
     ane_cuda_status *status = ctx().status;
 
-    int largest_blocks = 0;
-    if (split) {
+    int most_x = 0, most_table = 0;
+    if (split) {                                             // as many blocks as are resident at once, at least 4096 elements each
         const size_t nx = (size_t)T_all * D, ne = (size_t)V * D;
-        const size_t want = ((nx > ne ? nx : ne) + 4095) / 4096;
-        largest_blocks = want < LX_LARGEST_BLOCKS ? (int)want : LX_LARGEST_BLOCKS;
-        lx_call(lx_largest_kernel, dim3(largest_blocks, 2), dim3(256), 0, c.st, most, static_cast<const float *>(c.x), nx, static_cast<const float *>(c.table), ne, c.targets, c.id_u16, V,
-                D, c.S);
+        const auto share = [](size_t n, int most) { return n / 4096 < 1 ? 1 : n / 4096 < (size_t)most ? (int)(n / 4096) : most; };
+        most_x = share(nx, nx < ne ? LX_LARGEST_BLOCKS / 2 : LX_LARGEST_BLOCKS - share(ne, LX_LARGEST_BLOCKS / 2));
+        most_table = share(ne, LX_LARGEST_BLOCKS - most_x);
+        lx_call(lx_largest_kernel, dim3(most_x + most_table), dim3(256), 0, c.st, most, most_x, static_cast<const float *>(c.x), nx, static_cast<const float *>(c.table), ne, c.targets,
+                c.id_u16, V, D, c.S);
         ANE_LAUNCH_OK(1);
     }
     // Packs tokens [t0, t0 + n_tok) of x and rows [v0, v0 + nv) of the table; either may be none.
@@ -1164,7 +1172,7 @@ template <typename T, typename H> static int lx_run(const LxCall &c) {
         const T *from = static_cast<const T *>(c.table) + (size_t)v0 * D;
         const int flat = split && D % 8 == 0 && aligned16(from), x_blocks = lx_div(n_tok, 32) * lx_div(D, 32);
         const size_t want = flat ? ((size_t)nv * D / 8 + 255) / 256 : (size_t)nv;
-        const LxPack<T, H> p = {xh, xl, static_cast<const T *>(c.x), x_blocks, t0, n_tok, c.S, c.targets, c.id_u16, V, eh, el, from, nv, flat, D, ldd, most, largest_blocks, scales};
+        const LxPack<T, H> p = {xh, xl, static_cast<const T *>(c.x), x_blocks, t0, n_tok, c.S, c.targets, c.id_u16, V, eh, el, from, nv, flat, D, ldd, most, most_x, most_table, scales};
         lx_call(lx_pack_kernel<T, H>, dim3((unsigned)(x_blocks + (want < 4096 ? want : 4096))), dim3(256), 0, c.st, p);
         ANE_LAUNCH_OK(1);
         return ANE_CUDA_OK;
@@ -1245,10 +1253,11 @@ template <typename T, typename H> static int lx_run(const LxCall &c) {
                 if (int rc = maps_for(m, lh, split ? ll : nullptr, rows_hi, rows_lo, n_tok, nv, ldl, LX_CTA_M, nv, D, ld, LX_BK)) return rc;
                 g.kblocks = lx_div(nv, LX_BK); g.splits = splits;
                 if (split) g.span = lx_span(3);              // a 16-bit dx does not show what the accumulator cuts off
-                g.n_tiles = lx_div(D, LX_BN); g.n = D;
-                g.idesc = lx_idesc(half_type, false, true);
+                const int acc_n = lx_acc_n(plan.narrow_dx ? LX_NARROW : LX_PLAIN);
+                g.n_tiles = lx_div(D, acc_n); g.n = D;
+                g.idesc = lx_idesc(half_type, false, true, acc_n);
                 g.out = dxs; g.first = v0 == 0;
-                if (int rc = lx_launch<LX_DX>(c.st, m, g, split)) return rc;
+                if (int rc = lx_launch<LX_DX>(c.st, m, g, split, plan.narrow_dx)) return rc;
             }
             if (c.d_table) {
                 LxArgs g = a;
@@ -1257,10 +1266,12 @@ template <typename T, typename H> static int lx_run(const LxCall &c) {
                 g.span = lx_span(split ? 3 : 2);
                 g.kblocks = lx_div(n_tok, LX_BK);
                 g.m_tiles = lx_div(D, LX_BM); g.m = D;
-                g.n_tiles = lx_div(nv, LX_BN); g.n = nv;
-                g.idesc = lx_idesc(half_type, true, true);
+                const bool narrow_e = split && lx_narrow(g.m_tiles, nv);
+                const int acc_n = lx_acc_n(narrow_e ? LX_NARROW : LX_PLAIN);
+                g.n_tiles = lx_div(nv, acc_n); g.n = nv;
+                g.idesc = lx_idesc(half_type, true, true, acc_n);
                 g.out = c.d_table + (size_t)v0 * D; g.ldt = (size_t)D; g.alpha = alpha;
-                if (int rc = split ? lx_start<LX_DTABLE, LX_SPLIT>(c.st, m, g) : lx_start<LX_DTABLE, LX_TWO>(c.st, m, g)) return rc;
+                if (int rc = !split ? lx_start<LX_DTABLE, LX_TWO>(c.st, m, g) : narrow_e ? lx_start<LX_DTABLE, LX_NARROW>(c.st, m, g) : lx_start<LX_DTABLE, LX_SPLIT>(c.st, m, g)) return rc;
             }
         }
         if (c.dx) {
