@@ -408,7 +408,7 @@ template <typename T, int VEC, int NT, int SM, int NV, int THREADS> struct BnStr
 
 // A cluster per token tile.  LG lanes of VEC tokens per row, NV rows per thread; x2 takes x's place in the strip.
 template <typename T, int VEC, int LG, int NV, int THREADS, int SM>
-__global__ void __launch_bounds__(THREADS, THREADS == 512 ? (NV <= 8 ? 2 : 1) : NV * VEC <= 32 ? 4 : 2)
+__global__ void __launch_bounds__(THREADS, THREADS == 512 ? (NV <= 8 || VEC == 1 ? 2 : 1) : NV * VEC <= 32 ? 4 : 2)
 block_norm_cluster_kernel(T *x2, T *y, const T *x, const T *f, const float *__restrict__ w_post, const float *__restrict__ gate,
                           const float *__restrict__ w_pre, BnShape sh, int rows) {
     constexpr int R = THREADS / LG, TW = LG * VEC;
@@ -663,13 +663,14 @@ static bool bn_ring(int C, const BnSplit &sp, long long tiles) {
 // The cluster form for a shape, if there is one.
 //   many tiles   512 threads per block; 1024 channels to a block (forward 115 us against 138, backward 245 against 250, see above)
 //   few tiles    256 threads, up to eight blocks per tile, so that more SMs take part (5 us for 256 tokens x 768 channels)
-//   rows that break 16-byte alignment: element by element, 32 tokens per row, eight blocks per tile
+//   rows that break 16-byte alignment: element by element, 32 tokens per row, up to eight blocks per tile; blocks of 512 threads
+//                above 1024 channels (8 x 2048 x 1001 in fp16: forward 105 us against 223 in sweeps, backward 186 against 490)
 // -> BN_NONE: none (channels beyond eight blocks, or unaligned sequences so short that most lanes of a row would idle).
 constexpr int BN_NONE = 1;
 template <int V_, int LG_, int NV_, int TH_> struct BnForm { static constexpr int VEC = V_, LG = LG_, NV = NV_, THREADS = TH_; };
 // BIG_LG: lanes per row of the large form (a thread has C / (512 / BIG_LG) rows); BIG_C: channels above which it is used.
-template <typename T, int BIG_LG, int BIG_C, typename Fn> static int bn_pick_cluster(bool vec, int B, int C, int S, Fn &&go) {
-    constexpr int N = Elt<T>::VEC, BR = 512 / BIG_LG;
+template <typename T, bool FORWARD, typename Fn> static int bn_pick_cluster(bool vec, int B, int C, int S, Fn &&go) {
+    constexpr int N = Elt<T>::VEC, BIG_LG = 4, BIG_C = FORWARD ? 0 : 512, BR = 512 / BIG_LG;
     const int knob = tuning("block_norm_cluster", 7);    // bits: 1 small form, 2 large form, 4 backward ring; 0: none
     if (!(knob & 3)) return BN_NONE;
     const long long big_tiles = (long long)B * ((S + BIG_LG * N - 1) / (BIG_LG * N));
@@ -683,7 +684,13 @@ template <typename T, int BIG_LG, int BIG_C, typename Fn> static int bn_pick_clu
     if (vec && C <= 1024) return go(BnForm<N, 8, 4, 256>(), bn_split(C, 256 / 8 * 4));
     if (vec && C <= 2048) return go(BnForm<N, 4, 4, 256>(), bn_split(C, 256 / 4 * 4));
     if (vec && C <= 4096) return go(BnForm<N, 4, 8, 256>(), bn_split(C, 256 / 4 * 8));
-    if (!vec && S >= 16 && C <= 1024) return go(BnForm<1, 32, 16, 256>(), bn_split(C, 256 / 32 * 16));
+    if (!vec && S >= 16 && C <= 2048) {
+        // forward, few channels, many tiles: the sweeps find their tile in L1 (333 x 64 x 1001 in fp16 88 us against 122, 40 channels
+        // 14 against 22; in fp32 124 against 130)
+        if (FORWARD && C <= 512 && (long long)B * ((S + 31) / 32) >= 8LL * ctx().sm_count) return BN_NONE;
+        if (C <= 1024) return go(BnForm<1, 32, 16, 256>(), bn_split(C, 256 / 32 * 16));
+        return go(BnForm<1, 32, 16, 512>(), bn_split(C, 512 / 32 * 16));
+    }
     return BN_NONE;
 }
 // Blocks with more than the default shared memory ask for it once.
@@ -723,7 +730,7 @@ int ane_cuda_block_norm_dev(void *stream, ane_dtype dtype, int B, int C, int S, 
     BnShape sh = {B, C, S, 0, 0, gate_per_seq ? C : 0, alpha, eps};
     ANE_DISPATCH_DTYPE(dtype, T, {
         const bool vec = S % Elt<T>::VEC == 0 && aligned16(x2) && aligned16(y) && aligned16(x) && aligned16(f);
-        const int rc = bn_pick_cluster<T, 4, 0>(vec, B, C, S, [&](auto form, BnSplit sp) -> int {
+        const int rc = bn_pick_cluster<T, true>(vec, B, C, S, [&](auto form, BnSplit sp) -> int {
             using F = decltype(form);
             constexpr int SM = F::VEC == 1 ? 0 : F::THREADS == 512 ? 1 : 2;      // 512 threads: x in shared memory, f in registers
             constexpr size_t smem = BnStrip<T, F::VEC, 2, SM, F::NV, F::THREADS>::BYTES;
@@ -809,7 +816,7 @@ int ane_cuda_block_norm_bwd_dev(void *stream, ane_dtype dtype, int B, int C, int
                         : (dx2 ? go(std::false_type(), std::true_type()) : go(std::false_type(), std::false_type()));
             if (rc != ANE_CUDA_OK) return rc;
         }
-        if (rc == BN_NONE) rc = bn_pick_cluster<T, 4, 512>(vec, B, C, S, [&](auto form, BnSplit sp) -> int {
+        if (rc == BN_NONE) rc = bn_pick_cluster<T, false>(vec, B, C, S, [&](auto form, BnSplit sp) -> int {
             using F = decltype(form);
             constexpr int SM = F::VEC == 1 ? 0 : F::THREADS == 512 ? 3 : 4;      // 512 threads: dx2 in registers
             constexpr size_t smem = BnStrip<T, F::VEC, 4, SM, F::NV, F::THREADS>::BYTES;

@@ -108,6 +108,7 @@ def inputs(shape, dt, post, gate, seed=0):
 
 SHAPES = [(1, 1, 1), (2, 7, 3), (3, 33, 5), (1, 768, 256), (2, 128, 257), (3, 100, 333), (4, 64, 1), (1, 4096, 64), (2, 1024, 48), (70, 16, 2),
           (1, 300, 8), (1, 129, 64), (1, 4099, 8), (3, 2048, 72), (2, 1024, 1032), (1, 6000, 16),
+          (3, 1147, 38), (2, 1025, 333), (1, 2047, 17), (1, 2049, 17), (40, 50, 1001),
           (32, 1024, 512), (40, 96, 1000), (20, 1000, 264), (24, 700, 520)]      # many tiles: the pipelined forms
 
 
