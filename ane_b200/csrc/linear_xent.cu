@@ -651,13 +651,23 @@ template <typename T, typename H> __global__ void __launch_bounds__(256) lx_pack
         }
         return;
     }
-    for (int r = first; r < p.rows; r += step)
-        for (int d = threadIdx.x; d < (int)ld; d += 256) {
-            const float v = d < D ? Elt<T>::to_f(p.table[(size_t)r * D + d]) * scale : 0.0f;
-            const H h = Elt<H>::from_f(v);
-            p.eh[(size_t)r * ld + d] = h;
-            if (p.el) p.el[(size_t)r * ld + d] = Elt<H>::from_f(v - Elt<H>::to_f(h));
-        }
+    // eight columns of a row at a time: whole vectors out, single elements in (a row of the table starts anywhere).  With a block per
+    // row the losses of 200 tokens over 32000 fp16 rows of 1001 took 92 us instead of 48.
+    const uint32_t per = (uint32_t)(ld / 8);
+    for (size_t i = (size_t)first * 256 + threadIdx.x; i < (size_t)p.rows * per; i += (size_t)step * 256) {
+        const uint32_t r = (uint32_t)(i / per), d = (uint32_t)(i - (size_t)r * per) * 8;
+        const T *src = p.table + (size_t)r * D + d;
+        float f[8], h[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) f[j] = d + j < D ? Elt<T>::to_f(src[j]) * scale : 0.0f;
+        const uint4 q = Elt<H>::pack(f);
+        Elt<H>::unpack(q, h);
+        reinterpret_cast<uint4 *>(p.eh)[i] = q;
+        if (!p.el) continue;
+#pragma unroll
+        for (int j = 0; j < 8; j++) f[j] -= h[j];
+        reinterpret_cast<uint4 *>(p.el)[i] = Elt<H>::pack(f);
+    }
 }
 
 // (max, sum) pairs of the vocabulary tiles -> lse and loss of TOK tokens per block: 1024 / TOK threads take turns at the tiles
@@ -1171,7 +1181,7 @@ template <typename T, typename H> static int lx_run(const LxCall &c) {
     auto pack = [&](int t0, int n_tok, int v0, int nv) -> int {
         const T *from = static_cast<const T *>(c.table) + (size_t)v0 * D;
         const int flat = split && D % 8 == 0 && aligned16(from), x_blocks = lx_div(n_tok, 32) * lx_div(D, 32);
-        const size_t want = flat ? ((size_t)nv * D / 8 + 255) / 256 : (size_t)nv;
+        const size_t want = ((size_t)nv * (ldd / 8) + 255) / 256;          // (ldd is D where it is flat)
         const LxPack<T, H> p = {xh, xl, static_cast<const T *>(c.x), x_blocks, t0, n_tok, c.S, c.targets, c.id_u16, V, eh, el, from, nv, flat, D, ldd, most, most_x, most_table, scales};
         lx_call(lx_pack_kernel<T, H>, dim3((unsigned)(x_blocks + (want < 4096 ? want : 4096))), dim3(256), 0, c.st, p);
         ANE_LAUNCH_OK(1);
