@@ -166,6 +166,32 @@ def test_more_tokens_than_one_round(ops, dt):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dt,D,V", [("f32", 1024, 70000), ("f16", 1001, 140000)])
+def test_a_table_that_is_packed_piece_by_piece(ops, dt, D, V):
+    x, E, t = inputs(2, D, V, 130, DT[dt], seed=12)                # more than 256 MiB of packed rows
+    dE = torch.zeros(V, D, device="cuda")
+    loss, dx = ops.linear_cross_entropy(x, E, t, d_table=dE)
+    ref = reference(x, E, t)
+    assert max(off(loss, ref[0])) <= 1e-5
+    check_grads(DT[dt], dx, ref[2], dE, ref[3])
+    alone, _ = ops.linear_cross_entropy(x, E, t, grad=False)
+    assert max(off(alone, ref[0])) <= 1e-5
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("shape", [(40, 64, 300, 7), (300, 64, 300, 1), (8, 64, 300, 40)])
+def test_many_short_sequences(ops, shape, dt):
+    x, E, t = inputs(*shape, DT[dt], seed=13)
+    loss, dx = ops.linear_cross_entropy(x, E, t)
+    ref = reference(x, E, t)
+    assert max(off(loss, ref[0])) <= 1e-5
+    check_grads(DT[dt], dx, ref[2])
+    alone, _ = ops.linear_cross_entropy(x, E, t, grad=False)
+    assert torch.equal(alone, loss)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
 def test_offset_views_and_uint16_targets(ops, dt):
     """A table that starts off a 16-byte boundary, and the id type of the reference."""
