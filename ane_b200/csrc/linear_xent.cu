@@ -15,7 +15,7 @@
 // dl) at 6.5 TB/s are 1.9 ps, 2 * 1024 operations at 1.5 PFLOP/s are 1.4 ps.
 //
 // Measured, 8192 tokens x 151936 rows x 1024 channels in bf16 (cuBLAS on this GPU: 1650 TFLOP/s in a burst, 1410 under the
-// power cap), without overlap of the launches: stats 1.49 ms (1710 TFLOP/s), dlogits 2.15 (1190; it writes 5 GB of dl), dx 1.72
+// power cap), launches one after the other: stats 1.49 ms (1710 TFLOP/s), dlogits 2.15 (1190; it writes 5 GB of dl), dx 1.72
 // (1490), d_table 3.13 for two products (1630).  Back to back under the power cap the whole call takes 9.6 to 10.1 ms, 1290
 // TFLOP/s over the five products that it does and 780 over the three that the result cannot do without.
 //
@@ -767,9 +767,9 @@ __global__ void __launch_bounds__(256) lx_finish_dx_kernel(T *__restrict__ dx, c
 // For so few tokens the operator is the table read once (and once more, with its gradient read and written, for the gradients):
 // plain fp32 arithmetic on the elements as they are, bound by HBM.  A tile of the tensor cores would be 252 rows of nothing,
 // and fp32 tables would have to be packed first.  The few logits of a row are kept for the second pass, [V][T].
-// Against the tensor cores, 151936 rows x 1024 channels, losses / with gradients: fp32 1 token 126 / 435 against 516 / 1176 us,
-// 4 tokens 188 / 583 against 548 / 1228; bf16 1 token 63 / 445 against 76 / 494, 2 tokens 145 / 517 against 72 / 493.  Hence four
-// tokens in fp32 and one in 16 bits.
+// Against the tensor cores, 151936 rows x 1024 channels, losses / with gradients: fp32 1 token 123 / 434 against 453 / 1044 us,
+// 4 tokens 187 / 592 against 464 / 1094 (9200 x 768: 18 / 46 against 36 / 87); bf16 1 token 60 / 440 against 76 / 498, 2 tokens
+// 145 / 517 against 72 / 493.  Hence four tokens in fp32 and one in 16 bits.
 constexpr int LF_TOKENS = 4;
 constexpr size_t LF_SMEM = 96 << 10;                     // of x as fp32
 
@@ -953,8 +953,8 @@ static inline int lx_div(long long a, long long b) { return (int)((a + b - 1) / 
 static inline int lx_pairs() { return ctx().sm_count / 2; }
 
 // Every kernel of the chain is a programmatic dependent launch: its blocks may be placed and set up their barriers and
-// accumulators while the kernel before drains, and stop in dep_sync() until that one has completed.  A call has 4 to 12 short
-// launches where the problem is small: 130 -> 106 us for one fp32 sequence over 9200 rows.
+// accumulators while the kernel before drains, and stop in dep_sync() until that one has completed.  A call has 4 to 8 short
+// launches where the problem is small: 98 -> 81 us for one fp32 sequence over 9200 rows.
 template <typename... KArgs, typename... Args>
 static inline void lx_call(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args &&...args) {
     cudaLaunchConfig_t cfg = {};
